@@ -470,6 +470,28 @@ int unet_clip_adamw_apply(const float* const* grads_host, int32_t n_tensors, flo
                           float* v_flat, const float* coef, const float* step_t, float beta1, float beta2, float eps,
                           float weight_decay, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Gated linear recurrence along the rows of channels-last tensors (no counterpart in the reference: a bottleneck layer
+ * beside its attentions).  Per window and channel, t in row order (reverse != 0: from the last row to the first):
+ *   f_t = sigmoid(g_t),  h_t = f_t h_{t-1} + (1 - f_t) x_t
+ * x, g [n][l][c] with window stride *_ns and row pitch *_ld in elements (channels dense); h [n][l][c] contiguous, all of
+ * one dtype.  h0, last [n][c] fp32: state before the first and after the last row, NULL = zeros / not wanted.
+ * states: NULL (inference), or [n][ceil(l / unet_gated_scan_tile())][c] fp32 for unet_gated_scan_bwd, which recomputes
+ * the states from it.  Backward: dh as x; dlast, dh0 [n][c] fp32 or NULL; dx, dg [n][l][c] contiguous.
+ * workspace: unet_gated_scan_workspace_bytes(...) bytes (may be 0), 8-byte aligned, used by this call only. */
+int32_t unet_gated_scan_tile(void);
+size_t unet_gated_scan_workspace_bytes(int32_t dtype, int32_t n, int32_t l, int32_t c);
+int unet_gated_scan_fwd(int32_t dtype, const void* x, int64_t x_ns, int64_t x_ld, const void* g, int64_t g_ns, int64_t g_ld,
+                        const float* h0, int32_t reverse, int32_t n, int32_t l, int32_t c, void* h, float* last, float* states,
+                        void* workspace, size_t ws_bytes, void* stream);
+int unet_gated_scan_bwd(int32_t dtype, const void* x, int64_t x_ns, int64_t x_ld, const void* g, int64_t g_ns, int64_t g_ld,
+                        const float* states, const void* dh, int64_t dh_ns, int64_t dh_ld, const float* dlast, int32_t reverse,
+                        int32_t n, int32_t l, int32_t c, void* dx, void* dg, float* dh0, void* workspace, size_t ws_bytes,
+                        void* stream);
+/* One row of every sequence: state [n][c] fp32 moves on in place, h [n][c] = the new state in dtype. */
+int unet_gated_scan_step(int32_t dtype, const void* x, int64_t x_ld, const void* g, int64_t g_ld, float* state, void* h,
+                         int32_t n, int32_t c, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,300 @@
+"""The gated linear recurrence (ops.gated_scan, ops.gated_scan_step): refusals on the CPU, values and gradients on the GPU
+against a row-by-row evaluation in float64.
+
+Tolerances come from a running error bound evaluated next to the float64 recurrence.  With u = 2^-24 the kernel's gate has a
+relative error of at most K u: its exponential's argument is rounded twice (2 |g| u for |g| <= 10), exponential, sum, reciprocal
+and product add up to 6 units, and a product of gates adds one rounding a row.  K = 40 covers |g| <= 10 with room for the one
+rounding of each fused step.  So the state's error obeys e_t <= f_t e_{t-1} + K u (f_t |h_{t-1}| + (1 - f_t) |x_t|), the
+adjoint's the same recurrence from the other end, and a bf16 result is half a step, 2^-8 relative, further off."""
+import ctypes as C
+
+import pytest
+import torch
+
+U, K = 2.0 ** -24, 40.0
+
+
+def oracle(x, g, h0, dh, dlast, reverse):
+    """float64 values and error bounds: h, last, dx, dg, dh0 and the bound of each."""
+    x, g = x.double().cpu(), g.double().cpu()
+    if reverse:
+        x, g = x.flip(1), g.flip(1)
+    n, l, c = x.shape
+    f, keep = torch.sigmoid(g), torch.sigmoid(-g)
+    s = torch.zeros(n, c, dtype=torch.float64) if h0 is None else h0.double().cpu()
+    e = torch.zeros_like(s)
+    h, eh, before, eb = (torch.empty_like(x) for _ in range(4))
+    for t in range(l):
+        before[:, t], eb[:, t] = s, e
+        e = f[:, t] * e + K * U * (f[:, t] * s.abs() + keep[:, t] * x[:, t].abs())
+        s = f[:, t] * s + keep[:, t] * x[:, t]
+        h[:, t], eh[:, t] = s, e
+    out = dict(h=(h, eh), last=(s, e))
+    if dh is not None:
+        d = dh.double().cpu()
+        d = d.flip(1) if reverse else d
+        mu = torch.zeros_like(s) if dlast is None else dlast.double().cpu()
+        em = torch.zeros_like(s)
+        dx, dg, ex, eg = (torch.empty_like(x) for _ in range(4))
+        for t in range(l - 1, -1, -1):
+            lam, el = d[:, t] + mu, em + U * (d[:, t].abs() + mu.abs())
+            diff, ed = before[:, t] - x[:, t], eb[:, t] + U * (before[:, t].abs() + x[:, t].abs())
+            fk = f[:, t] * keep[:, t]
+            dx[:, t], ex[:, t] = keep[:, t] * lam, keep[:, t] * (el + 2 * K * U * lam.abs())
+            dg[:, t] = lam * diff * fk
+            eg[:, t] = fk * (el * diff.abs() + lam.abs() * ed + 3 * K * U * (lam * diff).abs())
+            mu, em = f[:, t] * lam, f[:, t] * (el + K * U * lam.abs())
+        out.update(dx=(dx, ex), dg=(dg, eg), dh0=(mu, em))
+    if reverse:
+        for k in ("h", "dx", "dg"):
+            if k in out:
+                out[k] = tuple(v.flip(1) for v in out[k])
+    return out
+
+
+def near(got, want, what=""):
+    value, bound = want
+    half = torch.finfo(got.dtype).eps / 2
+    got = got.detach().double().cpu()
+    tol = bound * (1 + half) + half * value.abs() + 1e-37
+    bad = (got - value).abs() > tol
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()}, worst {float(((got - value).abs() / tol).max()):.2f} tolerances"
+    assert bool(torch.isfinite(got).all())
+
+
+def inputs(n, l, c, dtype, seed=0, dev="cuda", spread=2.0):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen)
+    gate = (r(n, l, c) + spread * r(1, 1, c)).clamp(-10, 10)
+    return (r(n, l, c).to(dtype).to(dev), gate.to(dtype).to(dev), r(n, c).to(dev), r(n, l, c).to(dtype).to(dev), r(n, c).to(dev))
+
+
+def call(x, g, h0, dh, dlast, reverse):
+    from unet_amd import ops
+    x, g = x.detach().requires_grad_(), g.detach().requires_grad_()
+    h0 = None if h0 is None else h0.detach().requires_grad_()
+    h, last = ops.gated_scan(x, g, h0, reverse=reverse, return_state=True)
+    outs, grads = [h], [dh]
+    if dlast is not None:
+        outs.append(last)
+        grads.append(dlast)
+    leaves = [x, g] + ([] if h0 is None else [h0])
+    got = torch.autograd.grad(outs, leaves, grads)
+    return dict(zip(("h", "last", "dx", "dg", "dh0"), (h, last) + got))
+
+
+# ------------------------------------------------------------------------------------------------ CPU
+def test_oracle_gradients_against_autograd_on_cpu():
+    x, g, h0, dh, dlast = (t.double() for t in inputs(2, 9, 3, torch.float32, dev="cpu"))
+    for rev in (False, True):
+        xs, gs, hs = (t.clone().requires_grad_() for t in (x, g, h0))
+        s, rows = hs, [None] * 9
+        for t in (range(8, -1, -1) if rev else range(9)):
+            s = torch.sigmoid(gs[:, t]) * s + (1 - torch.sigmoid(gs[:, t])) * xs[:, t]
+            rows[t] = s
+        want = torch.autograd.grad([torch.stack(rows, 1), s], [xs, gs, hs], [dh, dlast])
+        o = oracle(x, g, h0, dh, dlast, rev)
+        for k, w in zip(("dx", "dg", "dh0"), want):
+            assert float((o[k][0] - w).abs().max()) < 1e-12
+
+
+def test_refusals_on_cpu():
+    from unet_amd import _lib, ops
+    x, g = torch.zeros(2, 4, 6), torch.zeros(2, 4, 6)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        ops.gated_scan(x, g)
+    with pytest.raises(ValueError, match="must both be"):
+        ops.gated_scan(x, g[:, :3])
+    with pytest.raises(ValueError, match="must both be"):
+        ops.gated_scan(x[0], g[0])
+    with pytest.raises(TypeError, match="one dtype"):
+        ops.gated_scan(x, g.bfloat16())
+    with pytest.raises(TypeError, match="bfloat16 or float32"):
+        ops.gated_scan(x.half(), g.half())
+    with pytest.raises(ValueError, match="state must be"):
+        ops.gated_scan(x, g, torch.zeros(2, 5))
+    with pytest.raises(TypeError, match="state must be float32"):
+        ops.gated_scan(x, g, torch.zeros(2, 6, dtype=torch.float64))
+    with pytest.raises(ValueError, match="must both be"):
+        ops.gated_scan_step(x, g, torch.zeros(2, 6))
+    with pytest.raises(ValueError, match="state must be"):
+        ops.gated_scan_step(x[0], g[0], torch.zeros(3, 6))
+    lib = _lib.load()
+    assert lib.unet_gated_scan_fwd(0, None, 0, 0, None, 0, 0, None, 0, 1, 1, 1, None, None, None, None, 0, None) == -1
+    assert b"null" in lib.unet_last_error()
+    assert lib.unet_gated_scan_fwd(7, 16, 0, 0, 16, 0, 0, None, 0, 1, 1, 1, 16, None, None, None, 0, None) == -1
+    assert b"dtype" in lib.unet_last_error()
+    assert lib.unet_gated_scan_fwd(0, 16, 0, 0, 16, 0, 0, None, 0, 1, 0, 1, 16, None, None, None, 0, None) == -1
+    assert b"shape" in lib.unet_last_error()
+    # one long sequence is split into segments and needs its workspace
+    need = lib.unet_gated_scan_workspace_bytes(0, 1, 100000, 64)
+    assert need > 0
+    assert lib.unet_gated_scan_fwd(0, 16, 0, 64, 16, 0, 64, None, 0, 1, 100000, 64, 16, None, None, None, 0, None) == -1
+    assert b"workspace" in lib.unet_last_error()
+    assert lib.unet_gated_scan_bwd(0, 16, 0, 64, 16, 0, 64, 16, 16, 0, 64, None, 0, 1, 100000, 64, 16, 16, None, 16, need - 8, None) == -1
+    assert b"workspace" in lib.unet_last_error()
+    assert lib.unet_gated_scan_step(0, None, 0, None, 0, None, None, 1, 1, None) == -1
+    assert lib.unet_gated_scan_workspace_bytes(0, 64, 1024, 1024) == 0
+
+
+# ------------------------------------------------------------------------------------------------ GPU
+SHAPES = [(1, 1, 1), (2, 1, 130), (3, 2, 7), (1, 63, 2), (2, 64, 64), (2, 65, 66), (5, 333, 199), (3, 129, 128), (64, 40, 96),
+          (1, 5000, 36), (2, 2111, 257), (300, 70, 128)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,l,c", SHAPES)
+def test_values_and_gradients(n, l, c, dtype):
+    for reverse, state in ((False, True), (True, True), (False, False)):
+        x, g, h0, dh, dlast = inputs(n, l, c, dtype, seed=n + l)
+        h0, dlast = (h0, dlast) if state else (None, None)
+        got = call(x, g, h0, dh, dlast, reverse)
+        want = oracle(x, g, h0, dh, dlast, reverse)
+        for k in got:
+            near(got[k], want[k], (k, reverse, state))
+        assert got["h"].dtype == dtype and got["last"].dtype == torch.float32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_alignment_and_broadcast(dtype):
+    """Column ranges of one projection, at even and odd offsets; every second row; one window broadcast over the batch."""
+    n, l, c = 3, 150, 66
+    x, g, h0, dh, dlast = inputs(n, l, 2 * c + 5, dtype, seed=4)
+    for a, b in ((0, c), (1, c + 2), (2, c + 5)):
+        xs, gs, d = x[:, :, a:a + c], g[:, :, b:b + c], dh[:, :, a:a + c]
+        got, want = call(xs, gs, h0[:, :c].contiguous(), d, None, False), oracle(xs, gs, h0[:, :c], d, None, False)
+        for k in got:
+            near(got[k], want[k], (k, a, b))
+    xs, gs, d = x[:, ::2, :c], g[:, 1::2, :c], dh[:, ::2, :c]
+    got, want = call(xs, gs, None, d, None, True), oracle(xs, gs, None, d, None, True)
+    for k in got:
+        near(got[k], want[k], (k, "rows"))
+    one = x[:1, :, :c].contiguous().requires_grad_()
+    from unet_amd import ops
+    gs, d = g[:, :, :c], dh[:, :, :c]
+    h = ops.gated_scan(one.expand(n, l, c), gs)
+    want = oracle(one.detach().expand(n, l, c), gs, None, d, None, False)
+    near(h, want["h"], "broadcast")
+    (dx,) = torch.autograd.grad(h, one, d)
+    half = torch.finfo(dtype).eps / 2      # each window's gradient is rounded before the sum, the sum once more
+    value, bound = want["dx"]
+    tol = (bound + half * value.abs()).sum(0) + 4 * half * value.abs().sum(0)
+    assert bool(((dx[0].double().cpu() - value.sum(0)).abs() <= tol).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saturated_gates(dtype):
+    """Gates of +-inf and +-1e4: the state passes unchanged, or is replaced, and no gradient reaches the gate."""
+    from unet_amd import ops
+    x, g, h0, dh, dlast = inputs(2, 200, 64, dtype, seed=5)
+    for big in (float("inf"), 1e4):
+        got = call(x, torch.full_like(g, big), h0, dh, dlast, False)
+        assert torch.equal(got["h"], h0[:, None].expand(2, 200, 64).to(dtype)) and torch.equal(got["last"], h0)
+        assert float(got["dx"].abs().max()) == 0 and float(got["dg"].abs().max()) == 0
+        want = dlast.double() + dh.double().sum(1)
+        assert float((got["dh0"].double() - want).abs().max()) <= 200 * U * float(dh.double().abs().sum(1).max())
+        got = call(x, torch.full_like(g, -big), h0, dh, dlast, False)
+        assert torch.equal(got["h"], x) and torch.equal(got["last"], x[:, -1].float())
+        assert float(got["dg"].abs().max()) == 0 and float(got["dh0"].abs().max()) == 0
+    # a NaN stays in its window and channel, in the rows behind it
+    x[0, 100, 3] = float("nan")
+    h = ops.gated_scan(x, g)
+    assert bool(torch.isnan(h[0, 100:, 3]).any()) and int(torch.isnan(h).sum()) == int(torch.isnan(h[0, 100:, 3]).sum())
+    assert not bool(torch.isnan(h[0, :100]).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pieces_and_single_rows_continue_each_other(dtype):
+    from unet_amd import ops
+    x, g, h0, _, _ = inputs(3, 150, 70, dtype, seed=6)
+    want = oracle(x, g, h0, None, None, False)
+    a, s = ops.gated_scan(x[:, :101], g[:, :101], h0, return_state=True)
+    b, s = ops.gated_scan(x[:, 101:140], g[:, 101:140], s, return_state=True)
+    rows = [ops.gated_scan_step(x[:, t], g[:, t], s) for t in range(140, 150)]
+    near(torch.cat([a, b, torch.stack(rows, 1)], 1), want["h"], "pieces")
+    near(s, want["last"], "state")
+    empty, last = ops.gated_scan(x[:, :0], g[:, :0], h0, return_state=True)
+    assert empty.shape == (3, 0, 70) and torch.equal(last, h0)
+    assert ops.gated_scan(x[:0], g[:0]).shape == (0, 150, 70)
+    with pytest.raises(ValueError, match="contiguous"):
+        ops.gated_scan_step(x[:, 0], g[:, 0], torch.zeros(70, 3, device="cuda").t())
+
+
+@pytest.mark.gpu
+def test_partial_gradients_and_differences():
+    """Only the final state used; only some inputs want a gradient; a directional difference quotient."""
+    from unet_amd import ops
+    x, g, h0, dh, dlast = inputs(2, 90, 32, torch.float32, seed=7)
+    xr = x.clone().requires_grad_()
+    _, last = ops.gated_scan(xr, g, h0, return_state=True)
+    (dx,) = torch.autograd.grad(last, xr, dlast)
+    near(dx, oracle(x, g, h0, torch.zeros_like(dh), dlast, False)["dx"], "last only")
+    hr = h0.clone().requires_grad_()
+    (d0,) = torch.autograd.grad(ops.gated_scan(x, g, hr), hr, dh)
+    near(d0, oracle(x, g, h0, dh, None, False)["dh0"], "h0 only")
+    got = call(x, g, h0, dh, dlast, True)
+    dirs = [torch.randn_like(t) for t in (x, g, h0)]
+    eps = 2.0 ** -7
+
+    def loss(sign):
+        h, last = ops.gated_scan(*(t + sign * eps * d for t, d in zip((x, g, h0), dirs)), reverse=True, return_state=True)
+        return float((h.double() * dh.double()).sum() + (last.double() * dlast.double()).sum())
+
+    want = sum(float((got[k].double() * d.double()).sum()) for k, d in zip(("dx", "dg", "dh0"), dirs))
+    quotient = (loss(1) - loss(-1)) / (2 * eps)
+    # third-order remainder eps^2 / 6 * |f'''| of a sum over 5760 outputs of unit size, and rounding 1e-7 / eps of the same sum
+    assert abs(quotient - want) <= (eps ** 2 + 1e-6 / eps) * (float(dh.abs().sum()) + abs(want))
+
+
+@pytest.mark.gpu
+def test_side_stream_and_graph_replays():
+    from unet_amd import ops
+    x, g, h0, dh, dlast = inputs(2, 700, 40, torch.bfloat16, seed=8)
+    eager = call(x, g, h0, dh, dlast, False)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = call(x, g, h0, dh, dlast, False)
+    side.synchronize()
+    for k in eager:
+        assert torch.equal(eager[k], other[k]), k
+    del other
+    xs, gs = x.clone().requires_grad_(), g.clone().requires_grad_()
+    state = h0.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h, last = ops.gated_scan(xs, gs, h0, return_state=True)
+        dx, dg = torch.autograd.grad([h, last], [xs, gs], [dh, dlast])
+        row = ops.gated_scan_step(xs.detach()[:, 0], gs.detach()[:, 0], state)
+    want_state = h0.clone()
+    for rep in range(4):
+        x2, g2, _, _, _ = inputs(2, 700, 40, torch.bfloat16, seed=20 + rep)
+        with torch.no_grad():
+            xs.copy_(x2)
+            gs.copy_(g2)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = call(x2, g2, h0, dh, dlast, False)
+        want_row = ops.gated_scan_step(x2[:, 0], g2[:, 0], want_state)
+        for a, b in ((h, want["h"]), (last, want["last"]), (dx, want["dx"]), (dg, want["dg"]), (row, want_row), (state, want_state)):
+            assert torch.equal(a, b), rep
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """2.2e9 elements: the last window's rows lie past 2^31 elements and 2^32 bytes."""
+    from unet_amd import ops
+    n, l, c = 3, 700000, 1024
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn((n, l, c), generator=gen, device="cuda", dtype=torch.bfloat16)
+    g = torch.randn((n, l, c), generator=gen, device="cuda", dtype=torch.bfloat16)
+    h, last = ops.gated_scan(x, g, return_state=True)
+    cut = slice(l - 300, l)
+    state = torch.zeros(1, c)          # 300 rows behind an unknown state: sigmoid(g) products have long forgotten it
+    want = oracle(x[2:, cut], g[2:, cut], state, None, None, False)
+    near(h[2:, -100:], tuple(v[:, -100:] for v in want["h"]), "tail")
+    near(last[2:], want["last"], "last")

@@ -142,6 +142,13 @@ _SIGNATURES = {
     "unet_cfc_attn_bwd_partials": (C.c_size_t, [_i32, _i32, _i32]),
     "unet_cfc_attn_bwd": (C.c_int, [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp,
                                     _vp, _vp, _vp]),
+    "unet_gated_scan_tile": (_i32, []),
+    "unet_gated_scan_workspace_bytes": (C.c_size_t, [_i32, _i32, _i32, _i32]),
+    "unet_gated_scan_fwd": (C.c_int, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp,
+                                      C.c_size_t, _vp]),
+    "unet_gated_scan_bwd": (C.c_int, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i32, _i32, _i32, _i32,
+                                      _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
+    "unet_gated_scan_step": (C.c_int, [_i32, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _i32, _vp]),
     "unet_band_log_power": (C.c_int, [_vp, _vp, _i64, _i32, _i32, C.c_float, _vp, _vp]),
     "unet_overlap_add": (C.c_int, [_i32, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _vp, _vp, _i32, _i32, _i32, _vp]),
 }

@@ -1656,3 +1656,114 @@ class BandProjectFn(torch.autograd.Function):
 
 def band_project(bands: Tensor, wq, bq, wk, bk, wv, bv):
     return BandProjectFn.apply(bands, wq, bq, wk, bk, wv, bv)
+
+
+# ---------------------------------------------------------------------------------------------
+# gated linear recurrence along the rows (csrc/scan.hip)
+# ---------------------------------------------------------------------------------------------
+def _stream_on(t: Tensor) -> C.c_void_p:
+    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def _dense_channels(t: Tensor) -> Tensor:
+    """Any window and row stride will do; the channels of a row must be adjacent."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _check_scan(what: str, x: Tensor, gate: Tensor, state: Optional[Tensor], dims: int):
+    _dt(x)
+    if x.dim() != dims or gate.shape != x.shape:
+        raise ValueError(f"{what}: x and gate must both be {'[N, L, C]' if dims == 3 else '[N, C]'}, got {tuple(x.shape)} and "
+                         f"{tuple(gate.shape)}")
+    if gate.dtype != x.dtype or gate.device != x.device:
+        raise TypeError(f"{what}: x and gate must have one dtype and device, got {x.dtype} on {x.device} and {gate.dtype} on "
+                        f"{gate.device}")
+    if state is not None:
+        if state.shape != (x.shape[0], x.shape[-1]):
+            raise ValueError(f"{what}: the state must be [N, C] = {(x.shape[0], x.shape[-1])}, got {tuple(state.shape)}")
+        if state.dtype != torch.float32 or state.device != x.device:
+            raise TypeError(f"{what}: the state must be float32 on {x.device}, got {state.dtype} on {state.device}")
+    _need_cuda(x)
+
+
+class GatedScanFn(torch.autograd.Function):
+    """(h, last) of ``gated_scan``; keeps the fp32 state in front of every 64th row for backward."""
+
+    @staticmethod
+    def forward(ctx, x, gate, h0, reverse):
+        x, gate = _dense_channels(x.detach()), _dense_channels(gate.detach())
+        h0 = None if h0 is None else h0.detach().contiguous()
+        n, l, c = x.shape
+        lib = _lib.load()
+        keep = any(ctx.needs_input_grad[:3])
+        h = torch.empty((n, l, c), dtype=x.dtype, device=x.device)
+        last = torch.empty((n, c), dtype=torch.float32, device=x.device)
+        tile = int(lib.unet_gated_scan_tile())
+        states = torch.empty((n, -(-l // tile), c), dtype=torch.float32, device=x.device) if keep else None
+        size = int(lib.unet_gated_scan_workspace_bytes(_dt(x), n, l, c))
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        with torch.cuda.device(x.device):
+            check(lib.unet_gated_scan_fwd(_dt(x), _p(x), x.stride(0), x.stride(1), _p(gate), gate.stride(0), gate.stride(1), _p(h0),
+                                          int(reverse), n, l, c, _p(h), _p(last), _p(states), _p(ws), size, _stream_on(x)),
+                  "unet_gated_scan_fwd")
+        if keep:
+            ctx.save_for_backward(x, gate, states)
+        ctx.reverse = reverse
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dlast):
+        if dh is None and dlast is None:
+            return None, None, None, None
+        x, gate, states = ctx.saved_tensors
+        n, l, c = x.shape
+        lib = _lib.load()
+        dh = torch.zeros((n, l, c), dtype=x.dtype, device=x.device) if dh is None else _dense_channels(dh.to(x.dtype))
+        dlast = None if dlast is None else dlast.to(torch.float32).contiguous()
+        dx, dg = (torch.empty((n, l, c), dtype=x.dtype, device=x.device) for _ in range(2))
+        dh0 = torch.empty((n, c), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
+        size = int(lib.unet_gated_scan_workspace_bytes(_dt(x), n, l, c))
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        with torch.cuda.device(x.device):
+            check(lib.unet_gated_scan_bwd(_dt(x), _p(x), x.stride(0), x.stride(1), _p(gate), gate.stride(0), gate.stride(1),
+                                          _p(states), _p(dh), dh.stride(0), dh.stride(1), _p(dlast), int(ctx.reverse), n, l, c,
+                                          _p(dx), _p(dg), _p(dh0), _p(ws), size, _stream_on(x)), "unet_gated_scan_bwd")
+        return dx, dg, dh0, None
+
+
+def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor] = None, reverse: bool = False, return_state: bool = False):
+    """Gated linear recurrence along the rows of ``[N, L, C]`` tensors:
+
+        f_t = sigmoid(gate_t),   h_t = f_t h_{t-1} + (1 - f_t) x_t
+
+    ``x`` and ``gate``: bf16 or fp32, both of one dtype; windows and rows may be strided (column ranges of one projection).
+    ``h0`` ``[N, C]`` fp32: the state in front of the first row (default zeros).  ``reverse``: walk from the last row to the
+    first.  Returns ``h`` ``[N, L, C]`` in ``x``'s dtype, and with ``return_state`` also the state after the last row walked,
+    ``[N, C]`` fp32 (pass it as ``h0`` of the next piece of a long recording).  The state is fp32 throughout.  Differentiable
+    (once) in ``x``, ``gate`` and ``h0``."""
+    _check_scan("gated_scan", x, gate, h0, 3)
+    if x.numel() == 0:                      # nothing to launch: empty rows leave the state as it was
+        h = x * torch.sigmoid(gate)
+        last = h0.clone() if h0 is not None else torch.zeros((x.shape[0], x.shape[2]), dtype=torch.float32, device=x.device)
+    else:
+        h, last = GatedScanFn.apply(x, gate, h0, bool(reverse))
+    return (h, last) if return_state else h
+
+
+@torch.no_grad()
+def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
+    """One row of ``gated_scan`` for every sequence: ``x``, ``gate`` ``[N, C]``; ``state`` ``[N, C]`` fp32 contiguous, moved on
+    IN PLACE.  Returns the new state in ``x``'s dtype.  Inference only."""
+    _check_scan("gated_scan_step", x, gate, state, 2)
+    if not state.is_contiguous():
+        raise ValueError("gated_scan_step: the state is updated in place and must be contiguous")
+    n, c = x.shape
+    h = torch.empty((n, c), dtype=x.dtype, device=x.device)
+    if x.numel():
+        x, gate = _dense_channels(x), _dense_channels(gate)
+        with torch.cuda.device(x.device):
+            check(_lib.load().unet_gated_scan_step(_dt(x), _p(x), x.stride(0), _p(gate), gate.stride(0), _p(state), _p(h), n, c,
+                                                   _stream_on(x)), "unet_gated_scan_step")
+    return h
