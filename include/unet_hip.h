@@ -470,6 +470,25 @@ int unet_clip_adamw_apply(const float* const* grads_host, int32_t n_tensors, flo
                           float* v_flat, const float* coef, const float* step_t, float beta1, float beta2, float eps,
                           float weight_decay, void* stream);
 
+/* AdamW with both moments in 8 bits (the fp32 form is above; train.py:1553-1559 keeps fp32 moments):
+ *   m <- b1 m + (1-b1) g,  r <- sqrt(b2 r^2 + (1-b2) g^2),  p <- (1 - lr wd) p - lr/(1-b1^t) m / (r / sqrt(1-b2^t) + eps)
+ * m and r are e4m3 codes with one fp32 scale per block of 256 elements of a tensor.  Tables of n_tensors <=
+ * UNET_OPT_MAX_TENSORS tensors (device): start256 [n+1] first block of each (absolute; the batch covers blocks start256[0]
+ * .. start256[n]-1 = blocks256 of them), numel [n] < 2^31, slot [n] first block in m8 / r8 and the scale arrays, or
+ * 0x80000000 | first float4 in m32 / v32 for a tensor whose moments stay fp32.  A NULL gradient skips its tensor.
+ * Order of a step with a clip: unet_grad_sqnorm (advances step_t), unet_adamw8_prepare (norm from the partial sums, clip,
+ * bias corrections into bc [n][2]), unet_adamw8_apply.  Without one: prepare with advance = 1 and n_partial = 0, apply with
+ * `partial` (unet_adamw8_blocks(blocks256) floats of g^2 sums), prepare with n_tensors = 0 and those sums for the norm.
+ * coef [8]: [0] clip, [3] norm, [4] lr. */
+int32_t unet_adamw8_blocks(int64_t blocks256);
+int unet_adamw8_prepare(const float* const* grads_host, int32_t n_tensors, const float* partial, int32_t n_partial,
+                        int32_t advance, float max_norm, const float* lr, float* coef, float* step_t, double beta1, double beta2,
+                        float* bc, void* stream);
+int unet_adamw8_apply(const float* const* grads_host, int32_t n_tensors, float* const* p_ptrs, const uint32_t* start256,
+                      const uint32_t* numel, const uint32_t* slot, int64_t blocks256, void* m8, void* r8, float* m_scale,
+                      float* r_scale, float* m32, float* v32, const float* coef, const float* bc, float* partial, double beta1,
+                      double beta2, float eps, float weight_decay, void* stream);
+
 /* ------------------------------------------------------------------------------------
  * Gated linear recurrence along the rows of channels-last tensors (no counterpart in the reference: a bottleneck layer
  * beside its attentions).  Per window and channel, t in row order (reverse != 0: from the last row to the first):

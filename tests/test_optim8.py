@@ -1,0 +1,296 @@
+"""optim.ClipAdamW with 8-bit moments (csrc/optim8.hip): refusals and the storage format on the CPU, steps on the GPU against
+float64.
+
+A step from given codes is compared value by value.  With u = 2^-24: m and v are sums of two products (5 roundings with the
+clip, and a fast reciprocal and square root of 2 units each in the update), so the stored value before its rounding is within
+8 u relative of the terms' magnitudes, and the parameter within u of itself plus 16 u of the step.  The stored code is the
+nearest of that value: at most half a step, 2^-4 relative or 2^-10 of the smallest code's unit, from the exact value, plus the
+8 u (which may move a value across a border to the other neighbour, still within half a step of the value it rounds)."""
+import copy
+import math
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+BETAS = (0.7595905764360957, 0.920298282605139)      # train.py:186-188
+BLOCK = 256
+
+
+def e4m3(y):
+    """Nearest e4m3 value of a float64 tensor, ties to even."""
+    _, ex = torch.frexp(y)
+    step = torch.exp2((ex - 1).clamp(min=-6).double() - 3)
+    return torch.round(y / step) * step
+
+
+# ------------------------------------------------------------------------------------------------ CPU
+def test_storage_format_on_cpu():
+    from unet_amd.optim import FP8_LEAST, dequantise_moment, quantise_moment
+    gen = torch.Generator().manual_seed(0)
+    for n in (1, 255, 256, 257, 4096, 5000):
+        x = torch.randn(n, generator=gen) * 10.0 ** torch.randint(-6, 3, (n,), generator=gen)
+        codes, scale = quantise_moment(x, False)
+        assert codes.dtype == torch.float8_e4m3fn and codes.shape == x.shape and scale.shape == (-(-n // BLOCK),)
+        back = dequantise_moment(codes, scale).double()
+        per = scale.double().repeat_interleave(BLOCK)[:n]
+        assert bool(((back - x.double()).abs() <= (2.0 ** -4 * x.double().abs()).clamp_min(2.0 ** -10 * per) * (1 + 1e-6)).all())
+        # codes of codes: unchanged
+        codes2, scale2 = quantise_moment(back.float(), False)
+        assert torch.allclose(dequantise_moment(codes2, scale2), back.float(), rtol=3e-7, atol=0)
+    r = torch.tensor([1.0, 1e-9, 0.0] + [0.5] * 253)
+    codes, scale = quantise_moment(r, True)
+    assert codes[:3].float().tolist() == [448.0, FP8_LEAST, 0.0]        # a positive root stays positive
+    for tiny in (0.0, 1e-31, 1e-45):                                     # far below any eps: zeros, no overflowing 448 / max
+        codes, scale = quantise_moment(torch.full((300,), tiny), True)
+        assert float(codes.float().abs().max()) == 0 and float(scale.abs().max()) == 0
+
+
+def test_refusals_on_cpu():
+    from unet_amd import _lib
+    from unet_amd.optim import ClipAdamW
+    p = torch.nn.Parameter(torch.zeros(5000))
+    for kw in (dict(state_bits=16), dict(state_bits=8, min_8bit_numel=-1), dict(betas=(1.0, 0.9))):
+        with pytest.raises(ValueError):
+            ClipAdamW([p], **kw)
+    opt = ClipAdamW([p], state_bits=8)
+    with pytest.raises(ValueError, match="state_bits"):
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3))], "state_bits": 4})
+    assert len(opt.param_groups) == 1
+    with pytest.raises(TypeError, match="fp32"):
+        ClipAdamW([torch.nn.Parameter(torch.zeros(5000, dtype=torch.bfloat16))], state_bits=8).moment_buffers()
+    lib = _lib.load()
+    assert lib.unet_adamw8_apply(None, 1, None, None, None, None, 1, None, None, None, None, None, None, None, None, None, 0.9, 0.9,
+                                 1e-8, 0.0, None) == -1 and b"null" in lib.unet_last_error()
+    assert lib.unet_adamw8_prepare(None, 0, None, 0, 0, 5.0, 16, 16, None, 0.9, 0.9, None, None) == -1
+    assert b"clip" in lib.unet_last_error()
+    assert lib.unet_adamw8_prepare(None, 300, None, 0, 0, 0.0, 16, 16, 16, 0.9, 0.9, 16, None) == -1
+    assert b"at most" in lib.unet_last_error()
+    assert lib.unet_adamw8_blocks(1) == 1 and lib.unet_adamw8_blocks(33) == 2
+
+
+# ------------------------------------------------------------------------------------------------ GPU
+SHAPES = [(256, 32, 7), (256,), (1,), (3,), (512, 256, 1), (37, 5), (1024, 130), (2, 3, 5, 7), (8193,), (4096,), (4095,), (90, 99),
+          (0,), (4096, 33)]
+
+
+def make(seed=0, shapes=SHAPES, unaligned=()):
+    gen = torch.Generator().manual_seed(seed)
+    params = []
+    for i, s in enumerate(shapes):
+        t = torch.randn(*s, generator=gen)
+        if i in unaligned:      # storage that starts 4 bytes behind a 16-byte boundary
+            buf = torch.empty(t.numel() + 1, device="cuda")
+            v = buf[1:].view(t.shape)
+            v.copy_(t)
+            params.append(torch.nn.Parameter(v))
+        else:
+            params.append(torch.nn.Parameter(t.cuda()))
+    return params, gen
+
+
+def set_grads(params, gen, scale):
+    for i, p in enumerate(params):
+        g = torch.randn(p.shape, generator=gen) * scale * 10.0 ** (-(i % 4))
+        g *= torch.rand(p.shape, generator=gen) > 0.1
+        p.grad = g.cuda()
+
+
+def snapshot(opt, params):
+    """Every tensor's moments as float64 values, and what they are held in."""
+    from unet_amd.optim import _load_moments
+    out = []
+    for p in params:
+        st = opt.state[p]
+        m, v = (t.double() for t in _load_moments(st))
+        out.append((m.view(p.shape), v.view(p.shape), "exp_avg_scale" in st, float(st["step"])))
+    return out
+
+
+def check_step(opt, params, before_p, before, grads, lr, wd, max_norm, eps=1e-8):
+    b1, b2 = BETAS
+    norm = math.sqrt(sum(float((g.double() ** 2).sum()) for g in grads if g is not None))
+    assert abs(float(opt.total_norm()) - norm) <= 2e-6 * norm
+    clip = min(1.0, max_norm / (norm + 1e-6)) if max_norm else 1.0
+    for p, p0, (m0, v0, small, t0), g, (m1, v1, _, t1) in zip(params, before_p, before, grads, snapshot(opt, params)):
+        if g is None:
+            assert torch.equal(p, p0) and torch.equal(m0, m1) and torch.equal(v0, v1) and t0 == t1
+            continue
+        if not p.numel():
+            continue
+        assert t1 == t0 + 1
+        g = g.double() * clip
+        ma, mb, v = b1 * m0, (1 - b1) * g, b2 * v0 + (1 - b2) * g * g
+        m = ma + mb
+        step = lr * (m / (1 - b1 ** t1)) / ((v / (1 - b2 ** t1)).sqrt() + eps)
+        want = p0.double() * (1 - lr * wd) - step
+        size = lr * ((ma.abs() + mb.abs()) / (1 - b1 ** t1)) / ((v / (1 - b2 ** t1)).sqrt() + eps)
+        # the clip's norm is a float of fp32 partial sums: 2e-6 relative, which only the clipped gradient sees
+        rel = 16 * U + (2e-6 if max_norm else 0.0)
+        tol = 3 * U * p0.double().abs() + rel * size + 1e-37
+        assert bool(((p.double() - want).abs() <= tol).all()), float(((p.double() - want).abs() / tol).max())
+        near = 8 * U + (2e-6 if max_norm else 0.0)
+        if not small:
+            assert bool(((m1 - m).abs() <= near * (ma.abs() + mb.abs()) + 1e-45).all())
+            assert bool(((v1 - v).abs() <= 2 * near * v + 1e-45).all())
+            continue
+        r = v.sqrt()
+        for stored, x, mag in ((m1, m, ma.abs() + mb.abs()), (v1.sqrt(), r, r)):
+            flat = torch.nn.functional.pad(x.reshape(-1).abs(), (0, -x.numel() % BLOCK)).view(-1, BLOCK)
+            unit = (flat.amax(1) / 448).repeat_interleave(BLOCK)[:x.numel()].view(x.shape)      # one code unit of the block
+            half = torch.maximum(2.0 ** -4 * x.abs(), 2.0 ** -10 * unit)
+            err = (stored - x).abs()
+            ok = err <= half * (1 + 1e-5) + near * mag
+            if x is r:           # a positive root below half the smallest code is raised to it
+                ok |= (x > 0) & (x < 2.0 ** -9 * unit) & (err <= 2.0 ** -9 * unit * (1 + 1e-5))
+                assert bool(((stored > 0) == (x > 0)).all() | (unit < 1e-30).any())
+            assert bool(ok.all()), float((err / half).max())
+            # and it is the nearest code: nearly all equal a rounding done in float64
+            if float(unit.min()) > 0:
+                near_all = e4m3(x / unit)
+                if x is r:
+                    near_all = torch.where((x > 0) & (near_all == 0), torch.full_like(near_all, 2.0 ** -9), near_all)
+                differ = ((stored / unit - near_all).abs() > 1e-4 * near_all.abs()).double().mean()
+                # a value lies within `near` of a border with probability 2 * near * 2^4 at most: allow ten times that, plus one
+                assert float(differ) <= 320 * near + 1.0 / x.numel() + 1e-12
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm,scale", [(5.0, 30.0), (5.0, 1e-4), (None, 1.0)])
+@pytest.mark.parametrize("wd", [0.0, 0.01])
+def test_steps_match_float64(max_norm, scale, wd):
+    from unet_amd.optim import ClipAdamW
+    params, gen = make(0, unaligned=(0, 8))
+    opt = ClipAdamW(params, lr=2e-3, betas=BETAS, weight_decay=wd, max_grad_norm=max_norm, state_bits=8)
+    opt.moment_buffers()
+    for it in range(4):
+        set_grads(params, gen, scale)
+        if it == 2:
+            params[0].grad = params[3].grad = None
+        if it == 3:        # a gradient whose storage is not 16-byte aligned
+            g = params[6].grad
+            buf = torch.empty(g.numel() + 1, device="cuda")
+            buf[1:] = g.reshape(-1)
+            params[6].grad = buf[1:].view(g.shape)
+        grads = [None if p.grad is None else p.grad.clone() for p in params]
+        p0, before = [p.detach().clone() for p in params], snapshot(opt, params)
+        opt.step()
+        check_step(opt, params, p0, before, grads, 2e-3, wd, max_norm)
+        for p, g in zip(params, grads):
+            assert g is None or torch.equal(p.grad, g)
+    buf = opt.moment_buffers()
+    assert buf["exp_avg8"].dtype == torch.float8_e4m3fn and buf["exp_avg8"].numel() == 256 * buf["exp_avg8_scale"].numel()
+    small = [p for p in params if p.numel() < 4096]
+    assert all("exp_avg_sq" in opt.state[p] for p in small) and not any("exp_avg_sq" in opt.state[p] for p in params if p.numel() >= 4096)
+
+
+@pytest.mark.gpu
+def test_extreme_gradients():
+    """Zero, tiny and huge gradients stay finite; an infinite one spoils its own block of 256 only."""
+    from unet_amd.optim import ClipAdamW
+    p = torch.nn.Parameter(torch.ones(8192, device="cuda"))
+    opt = ClipAdamW([p], lr=1e-3, betas=BETAS, weight_decay=0.0, state_bits=8)
+    g = torch.zeros(8192, device="cuda")
+    g[256:512] = 1e-38
+    g[512:768] = 1e18
+    g[768:1024] = torch.logspace(-12, 3, 256, device="cuda")
+    for _ in range(5):
+        p.grad = g.clone()
+        opt.step()
+        assert bool(torch.isfinite(p).all())
+        assert float((p - 1).detach().abs().max()) <= 5 * 1e-3 * 3      # no step is blown up by a vanished root
+    assert torch.equal(p[:256], torch.ones(256, device="cuda")) and torch.equal(p[1024:], torch.ones(7168, device="cuda"))
+    g[2000] = float("inf")
+    p.grad = g
+    opt.step()
+    p.grad = torch.zeros_like(g)
+    opt.step()
+    bad = ~torch.isfinite(p)
+    lo = 2000 // 256 * 256
+    assert bool(bad[2000]) and not bool(bad[:lo].any()) and not bool(bad[lo + 256:].any())
+
+
+@pytest.mark.gpu
+def test_checkpoints_convert_both_ways():
+    from unet_amd.optim import ClipAdamW, _load_moments
+    shapes = [(64, 64, 3), (7,), (100, 50)]
+    params, gen = make(3, shapes)
+    opt = ClipAdamW(params, lr=1e-3, betas=BETAS, weight_decay=0.0, state_bits=8, max_grad_norm=1.0)
+    for _ in range(3):
+        set_grads(params, gen, 1.0)
+        opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    assert saved["state"][0]["exp_avg"].dtype == torch.float8_e4m3fn and saved["state"][1]["exp_avg"].dtype == torch.float32
+    set_grads(params, gen, 1.0)
+    grads = [p.grad.clone() for p in params]
+    start = [p.detach().clone() for p in params]
+    opt.step()
+    # 8 -> 8: the same trajectory to the bit
+    other = [torch.nn.Parameter(s.clone()) for s in start]
+    opt2 = ClipAdamW(other, lr=1e-3, betas=BETAS, weight_decay=0.0, state_bits=8, max_grad_norm=1.0)
+    opt2.load_state_dict(saved)
+    for p, g in zip(other, grads):
+        p.grad = g.clone()
+    opt2.step()
+    for a, b in zip(params, other):
+        assert torch.equal(a, b)
+        assert set(opt.state[a]) == set(opt2.state[b])
+        for k, x in opt.state[a].items():
+            assert x.dtype == opt2.state[b][k].dtype and torch.equal(x.float(), opt2.state[b][k].float()), k
+    # 8 -> 32: the values the codes stand for
+    third = [torch.nn.Parameter(s.clone()) for s in start]
+    opt3 = ClipAdamW(third, lr=1e-3, betas=BETAS, weight_decay=0.0, max_grad_norm=1.0)
+    opt3.load_state_dict(saved)
+    assert opt3.param_groups[0]["state_bits"] == 32
+    opt3.moment_buffers()
+    for i, p in enumerate(third):
+        m, v = _load_moments(saved["state"][i])
+        assert torch.equal(opt3.state[p]["exp_avg"].reshape(-1), m.cuda()) and torch.equal(opt3.state[p]["exp_avg_sq"].reshape(-1), v.cuda())
+        assert set(opt3.state[p]) == {"step", "exp_avg", "exp_avg_sq"} and float(opt3.state[p]["step"]) == 3
+    # torch's AdamW -> 8
+    ref = torch.optim.AdamW(third, lr=1e-3, betas=BETAS, weight_decay=0.0)
+    for p, g in zip(third, grads):
+        p.grad = g.clone()
+    ref.step()
+    opt4 = ClipAdamW(third, lr=1e-3, betas=BETAS, weight_decay=0.0, state_bits=8, max_grad_norm=2.0)
+    opt4.load_state_dict(copy.deepcopy(ref.state_dict()))
+    assert opt4.param_groups[0]["state_bits"] == 8 and opt4.param_groups[0]["max_grad_norm"] == 2.0
+    opt4.moment_buffers()
+    m, v = _load_moments(opt4.state[third[0]])
+    want = ref.state[third[0]]
+    top = float(want["exp_avg"].abs().max())
+    assert float((m - want["exp_avg"].reshape(-1)).abs().max()) <= 2.0 ** -4 * top
+    assert float((v.sqrt() - want["exp_avg_sq"].reshape(-1).sqrt()).abs().max()) <= 2.0 ** -4 * float(want["exp_avg_sq"].max().sqrt())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [1.0, None])
+def test_graph_replays_and_many_tensors(max_norm):
+    """300 tensors (two sub-tables) in a captured step: every replay equals an eager optimizer's step, lr read from memory."""
+    from unet_amd.optim import ClipAdamW
+    shapes = [(40 + i, 110) if i % 3 else (17 + i,) for i in range(300)]
+    a, gen = make(5, shapes)
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    lr = torch.tensor(1e-3, device="cuda")
+    kw = dict(betas=BETAS, weight_decay=0.01, max_grad_norm=max_norm, state_bits=8)
+    eager, cap = ClipAdamW(a, lr=1e-3, **kw), ClipAdamW(b, lr=lr, **kw)
+    for p in b:
+        p.grad = torch.zeros_like(p)
+    cap.moment_buffers()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cap.step()
+    for rep in range(4):
+        set_grads(a, gen, 1.0)
+        for p, q in zip(a, b):
+            q.grad.copy_(p.grad)
+        if rep == 2:
+            lr.fill_(5e-4)
+            eager.param_groups[0]["lr"] = 5e-4
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(a, b)), rep
+        assert torch.equal(eager.total_norm(), cap.total_norm())
+    for x, y in zip(eager.moment_buffers().values(), cap.moment_buffers().values()):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))

@@ -15,6 +15,12 @@ the gradients right after the step); ``total_norm(group)`` returns the pre-clip 
 Nothing synchronises with the host, so the step can be captured in a HIP graph.
 
 The moments live in two flat fp32 buffers per group; ``state[p]["exp_avg"]`` etc. are views into them.
+
+``state_bits=8`` (an option of the optimizer or of one group) keeps both moments in 8 bits (``csrc/optim8.hip``): 2 bytes of
+state an element instead of 8, and 16 bytes of memory traffic a step instead of 28.  ``state[p]`` then holds ``exp_avg``
+(e4m3 codes, ``torch.float8_e4m3fn``) and ``exp_avg_sq_root`` (e4m3 codes of sqrt(exp_avg_sq)), each with an fp32 ``*_scale`` per
+block of 256 elements: value = code * scale.  Tensors with fewer than ``min_8bit_numel`` elements (norms, biases) keep fp32
+moments.  Checkpoints convert both ways when they are loaded.
 """
 from __future__ import annotations
 
@@ -67,24 +73,168 @@ class _Group:
         self.n_partial = nb
 
 
+BLOCK = 256                 # csrc/optim8.hip: elements of a tensor that share one scale
+FP8_MAX, FP8_LEAST = 448.0, 2.0 ** -9
+TINY = 2.0 ** -100          # a block below this is stored as zeros
+WIDE = 0x80000000           # include/unet_hip.h unet_adamw8_apply: slot of a tensor with fp32 moments
+
+
+def quantise_moment(x: torch.Tensor, root: bool):
+    """fp32 moment -> (e4m3 codes of x's shape, fp32 scale per block of 256 elements).  ``root``: x is sqrt(exp_avg_sq), whose
+    positive values must not become zero."""
+    n = x.numel()
+    flat = torch.nn.functional.pad(x.reshape(-1).float(), (0, -n % BLOCK)).view(-1, BLOCK)
+    top = flat.abs().amax(1, keepdim=True)
+    some = top >= TINY
+    y = torch.where(some, flat * (top.reciprocal() * FP8_MAX), torch.zeros_like(flat))
+    if root:
+        y = torch.where(some & (flat > 0), y.clamp_min(FP8_LEAST), y)
+    scale = torch.where(some, top / FP8_MAX, torch.zeros_like(top)).view(-1)
+    return y.to(torch.float8_e4m3fn).view(-1)[:n].view(x.shape), scale
+
+
+def dequantise_moment(codes: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
+    """The fp32 values that codes and scales of one tensor stand for."""
+    n = codes.numel()
+    return codes.reshape(-1).float() * scale.float().repeat_interleave(BLOCK)[:n]
+
+
+def _load_moments(st):
+    """(exp_avg, exp_avg_sq) of a state in either form as flat fp32, or None for a tensor that has not been stepped."""
+    if "exp_avg" not in st:
+        return None
+    if "exp_avg_scale" in st:
+        return (dequantise_moment(st["exp_avg"], st["exp_avg_scale"]),
+                dequantise_moment(st["exp_avg_sq_root"], st["exp_avg_sq_root_scale"]).square())
+    return st["exp_avg"].reshape(-1), st["exp_avg_sq"].reshape(-1)
+
+
+class _Group8:
+    """Device tables of a parameter group with 8-bit moments: code buffers for its large tensors, fp32 buffers for the rest."""
+
+    def __init__(self, params: List[torch.nn.Parameter], min_numel: int):
+        dev = params[0].device
+        self.params = params
+        start, slot, blocks, self.end8, self.end32 = [], [], 0, 0, 0
+        for p in params:
+            if p.dtype != torch.float32 or not p.is_contiguous() or p.device != dev:
+                raise TypeError("ClipAdamW: parameters must be contiguous fp32 tensors on one device (fp32 master "
+                                "weights, as in the reference)")
+            if p.numel() >= 1 << 31:
+                raise ValueError("ClipAdamW: a tensor of 2^31 or more elements cannot keep 8-bit moments")
+            start.append(blocks)
+            nb = -(-p.numel() // BLOCK)
+            blocks += nb
+            if p.numel() >= min_numel:
+                slot.append(self.end8 // BLOCK)
+                self.end8 += nb * BLOCK
+            else:
+                slot.append(WIDE | (self.end32 // 4))
+                self.end32 += -(-p.numel() // 4) * 4
+        start.append(blocks)
+        if blocks * (BLOCK // 4) >= 1 << 31 or self.end32 >= 1 << 33:
+            raise ValueError("ClipAdamW: more than 2^33 parameters in one group")
+        as_u32 = lambda v: torch.tensor(v, dtype=torch.int64).to(torch.int32).to(dev)        # the low 32 bits
+        self.start256, self.slot = as_u32(start), as_u32(slot)
+        self.start4 = as_u32([b * (BLOCK // 4) for b in start])
+        self.numel = as_u32([p.numel() for p in params])
+        self.p_ptrs = torch.tensor([p.data_ptr() for p in params], dtype=torch.int64, device=dev)
+        self.ptr_key = tuple(p.data_ptr() for p in params)
+        zeros = lambda n, dt: torch.zeros(max(n, BLOCK), dtype=dt, device=dev)
+        self.m8, self.r8 = (zeros(self.end8, torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+        self.m_scale, self.r_scale = (zeros(self.end8 // BLOCK, torch.float32) for _ in range(2))
+        self.m, self.v = (zeros(self.end32, torch.float32) for _ in range(2))
+        self.step = torch.zeros(len(params), dtype=torch.float32, device=dev)
+        self.bc = torch.zeros((len(params), 2), dtype=torch.float32, device=dev)
+        self.coef = torch.zeros(8, dtype=torch.float32, device=dev)
+        self.lr = torch.zeros((), dtype=torch.float32, device=dev)
+        self.lr_host = None
+        lib = _lib.load()
+        # sub-tables of at most OPT_MAX_TENSORS tensors: (first, count, blocks, first partial of the norm pass / of the step)
+        self.batches, n1, n2 = [], 0, 0
+        for a in range(0, len(params), _lib.OPT_MAX_TENSORS):
+            b = min(len(params), a + _lib.OPT_MAX_TENSORS)
+            nb = start[b] - start[a]
+            if nb == 0:
+                continue
+            self.batches.append((a, b - a, nb, n1, n2))
+            n1 += int(lib.unet_opt_blocks(nb * BLOCK))
+            n2 += int(lib.unet_adamw8_blocks(nb))
+        self.n_norm, self.n_step = n1, n2
+        self.partial = torch.zeros(max(n1, n2, 1), dtype=torch.float32, device=dev)
+        self.views = []
+        for p, s, b in zip(params, slot, start):
+            n = p.numel()
+            if s & WIDE:
+                a = 4 * (s & ~WIDE)
+                self.views.append({"exp_avg": self.m[a:a + n].view_as(p), "exp_avg_sq": self.v[a:a + n].view_as(p)})
+            else:
+                a, nb = s * BLOCK, -(-n // BLOCK)
+                self.views.append({"exp_avg": self.m8[a:a + n].view_as(p), "exp_avg_scale": self.m_scale[s:s + nb],
+                                   "exp_avg_sq_root": self.r8[a:a + n].view_as(p), "exp_avg_sq_root_scale": self.r_scale[s:s + nb]})
+
+    def fill(self, i: int, st) -> None:
+        """Moments of tensor i from a loaded state in either form, or from an earlier table."""
+        view = self.views[i]
+        if "exp_avg" in st:
+            if "exp_avg_scale" in view and "exp_avg_scale" in st:          # codes stay the codes they are
+                new = {k: st[k].to(view[k].dtype) for k in view}
+            elif "exp_avg_scale" in view:
+                m, v = _load_moments(st)
+                new = dict(zip(("exp_avg", "exp_avg_scale"), quantise_moment(m, False)))
+                new.update(zip(("exp_avg_sq_root", "exp_avg_sq_root_scale"), quantise_moment(v.sqrt(), True)))
+            else:
+                new = dict(zip(("exp_avg", "exp_avg_sq"), _load_moments(st)))
+            for k in view:
+                view[k].copy_(new[k].reshape(view[k].shape))
+        for k in ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_root", "exp_avg_sq_root_scale"):
+            st.pop(k, None)
+        st.update(view)
+
+
 class ClipAdamW(torch.optim.Optimizer):
     def __init__(self, params: Iterable, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
-                 max_grad_norm: Optional[float] = None):
+                 max_grad_norm: Optional[float] = None, state_bits: int = 32, min_8bit_numel: int = 4096):
         """Arguments as ``torch.optim.AdamW`` (amsgrad / maximize are not offered: the reference never sets them).
         ``max_grad_norm``: clip the global L2 norm of each parameter group's gradients to this value inside ``step()``
-        (``None`` or 0: no clipping); a group may override it with its own ``max_grad_norm`` entry."""
+        (``None`` or 0: no clipping); a group may override it with its own ``max_grad_norm`` entry.
+        ``state_bits``: 32 (fp32 moments) or 8 (see the module docstring); ``min_8bit_numel``: tensors with fewer elements
+        keep fp32 moments.  A group may override both; a loaded checkpoint does not."""
         if not 0.0 <= eps or not 0.0 <= betas[0] < 1.0 or not 0.0 <= betas[1] < 1.0 or weight_decay < 0.0:
             raise ValueError("ClipAdamW: invalid hyper-parameter")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay,
-                                      max_grad_norm=max_grad_norm))
+                                      max_grad_norm=max_grad_norm, state_bits=state_bits, min_8bit_numel=min_8bit_numel))
         self._groups = {}
         self.clips_gradients = True        # GraphedTrainStep / Trainer: do not clip a second time
 
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        if group["state_bits"] not in (8, 32) or not group["min_8bit_numel"] >= 0:
+            self.param_groups.pop()
+            raise ValueError(f"ClipAdamW: state_bits must be 8 or 32 and min_8bit_numel not negative, got {group['state_bits']} "
+                             f"and {group['min_8bit_numel']}")
+
     # -- tables -------------------------------------------------------------------------------
+    def _tables8(self, gi: int, params, min_numel: int) -> _Group8:
+        g = self._groups.get(gi)
+        if g is None or g.ptr_key != tuple(p.data_ptr() for p in params):
+            g = _Group8(params, min_numel)
+            for i, p in enumerate(params):
+                st = self.state[p]
+                g.fill(i, st)
+                if st.get("step") is not None:
+                    g.step[i] = float(st["step"])
+                st["step"] = g.step[i]
+            self._groups[gi] = g
+        return g
+
     def _tables(self, gi: int, group) -> _Group:
         params = [p for p in group["params"] if p.requires_grad]
         if not params:
             return None
+        if group["state_bits"] == 8:
+            return self._tables8(gi, params, group["min_8bit_numel"])
         g = self._groups.get(gi)
         key = tuple(p.data_ptr() for p in params)
         if g is None or g.ptr_key != key:
@@ -95,9 +245,12 @@ class ClipAdamW(torch.optim.Optimizer):
                 a, n = 4 * starts[i], p.numel()
                 st = self.state[p]
                 # a state loaded from a checkpoint (or moments of a previous table) move into the flat buffers
-                if "exp_avg" in st:
-                    g.m[a:a + n].copy_(st["exp_avg"].reshape(-1))
-                    g.v[a:a + n].copy_(st["exp_avg_sq"].reshape(-1))
+                moments = _load_moments(st)
+                if moments is not None:
+                    g.m[a:a + n].copy_(moments[0])
+                    g.v[a:a + n].copy_(moments[1])
+                for k in ("exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale"):
+                    st.pop(k, None)
                 st["exp_avg"] = g.m[a:a + n].view_as(p)
                 st["exp_avg_sq"] = g.v[a:a + n].view_as(p)
                 prev = st.get("step")
@@ -113,9 +266,10 @@ class ClipAdamW(torch.optim.Optimizer):
         every param_group by the saved one, so a ``torch.optim.AdamW`` checkpoint of the reference (no
         ``max_grad_norm`` key) would silently switch the clip off, and a device-scalar ``lr`` (graph-captured steps
         read it through its pointer) would become a float no captured step sees."""
-        before = [(g.get("max_grad_norm"), g.get("lr")) for g in self.param_groups]
+        before = [(g.get("max_grad_norm"), g.get("lr"), g["state_bits"], g["min_8bit_numel"]) for g in self.param_groups]
         super().load_state_dict(state_dict)
-        for group, (max_norm, lr) in zip(self.param_groups, before):
+        for group, (max_norm, lr, bits, min_numel) in zip(self.param_groups, before):
+            group["state_bits"], group["min_8bit_numel"] = bits, min_numel     # the moments convert, see _load_moments
             if "max_grad_norm" not in group:
                 group["max_grad_norm"] = max_norm
             if isinstance(lr, torch.Tensor):
@@ -127,7 +281,44 @@ class ClipAdamW(torch.optim.Optimizer):
         """Global L2 norm of the group's gradients at the last ``step()`` (before clipping), a device scalar."""
         return self._groups[group_index].coef[3]
 
+    def moment_buffers(self, group_index: int = 0) -> dict:
+        """The flat buffers behind a group's ``state`` (live, not copies), in parameter order.  ``state_bits=32``: ``exp_avg``,
+        ``exp_avg_sq``, tensors padded to 4 elements.  ``state_bits=8``: those hold the tensors below ``min_8bit_numel``; the
+        others are in ``exp_avg8`` / ``exp_avg_sq_root8`` (e4m3 codes, tensors padded to 256 elements) with one fp32 scale per
+        256 codes in ``exp_avg8_scale`` / ``exp_avg_sq_root8_scale``."""
+        g = self._tables(group_index, self.param_groups[group_index])
+        if g is None:
+            return {}
+        if not isinstance(g, _Group8):
+            return {"exp_avg": g.m, "exp_avg_sq": g.v}
+        nb = g.end8 // BLOCK
+        return {"exp_avg": g.m[:g.end32], "exp_avg_sq": g.v[:g.end32], "exp_avg8": g.m8[:g.end8], "exp_avg8_scale": g.m_scale[:nb],
+                "exp_avg_sq_root8": g.r8[:g.end8], "exp_avg_sq_root8_scale": g.r_scale[:nb]}
+
     # -- step -----------------------------------------------------------------------------------
+    def _apply8(self, lib, st, g: _Group8, group, grads, max_norm: float, lr_ptr: int) -> None:
+        """One step of an 8-bit group: norm first if it clips, otherwise the norm falls out of the step."""
+        b1, b2 = (float(b) for b in group["betas"])
+        no_clip = not max_norm > 0.0
+        arrs = [(C.c_void_p * n)(*grads[a:a + n]) for a, n, _, _, _ in g.batches]
+        if not no_clip:
+            for (a, n, nb, p1, _), arr in zip(g.batches, arrs):
+                check(lib.unet_grad_sqnorm(arr, n, g.start4[a:].data_ptr(), g.numel[a:].data_ptr(), nb * BLOCK,
+                                           g.partial[p1:].data_ptr(), g.step[a:].data_ptr(), st), "unet_grad_sqnorm")
+        for (a, n, nb, _, p2), arr in zip(g.batches, arrs):
+            check(lib.unet_adamw8_prepare(arr, n, g.partial.data_ptr(), 0 if no_clip else g.n_norm, int(no_clip), max_norm, lr_ptr,
+                                          g.coef.data_ptr(), g.step[a:].data_ptr(), b1, b2, g.bc[a:].data_ptr(), st),
+                  "unet_adamw8_prepare")
+        for (a, n, nb, _, p2), arr in zip(g.batches, arrs):
+            check(lib.unet_adamw8_apply(arr, n, g.p_ptrs[a:].data_ptr(), g.start256[a:].data_ptr(), g.numel[a:].data_ptr(),
+                                        g.slot[a:].data_ptr(), nb, g.m8.data_ptr(), g.r8.data_ptr(), g.m_scale.data_ptr(),
+                                        g.r_scale.data_ptr(), g.m.data_ptr(), g.v.data_ptr(), g.coef.data_ptr(),
+                                        g.bc[a:].data_ptr(), g.partial[p2:].data_ptr() if no_clip else 0, b1, b2,
+                                        float(group["eps"]), float(group["weight_decay"]), st), "unet_adamw8_apply")
+        if no_clip:
+            check(lib.unet_adamw8_prepare(None, 0, g.partial.data_ptr(), g.n_step, 0, 0.0, lr_ptr, g.coef.data_ptr(), None, b1, b2,
+                                          None, st), "unet_adamw8_prepare")
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -162,6 +353,9 @@ class ClipAdamW(torch.optim.Optimizer):
                 continue
             beta1, beta2 = group["betas"]
             max_norm = group.get("max_grad_norm") or 0.0
+            if isinstance(g, _Group8):
+                self._apply8(lib, st, g, group, grads, float(max_norm), lr_ptr)
+                continue
             arrs = []
             for a, n, flat, p0, blocks in g.batches:
                 arr = (C.c_void_p * n)(*grads[a:a + n])
