@@ -470,6 +470,28 @@ int unet_clip_adamw_apply(const float* const* grads_host, int32_t n_tensors, flo
                           float* v_flat, const float* coef, const float* step_t, float beta1, float beta2, float eps,
                           float weight_decay, void* stream);
 
+/* ------------------------------------------------------------------------------------
+ * Attention with a learned relative-position bias (no counterpart in the reference; beside SelfAttention1D, models.py:75-97):
+ *   S[i][j] = scale <q_i, k_j> + table[bucket(j - i)][head],  out = softmax_j(S) v
+ * q, k, v, out, dout, dq, dk, dv: [n][l][c] contiguous, 16-byte aligned, dtype; head h owns columns h*hd .. h*hd+hd-1, hd = c /
+ * n_heads a multiple of 8 (bf16) or 4 (fp32), at most 256.  table, dtable: [buckets][n_heads], fp32 (table_f32) or bf16.
+ * Buckets 0 .. buckets/2-1 are for j <= i, the others for j > i; starts_host[b] is the smallest |j - i| of bucket b of a side
+ * (starts_host[0] = 0, not decreasing, the last one in 1 .. UNET_REL_MAX_DISTANCE).  A bias of -inf removes its pairs.
+ * lengths: NULL or [n] int32 on the device; positions at or past a window's length are neither keys nor queries: their outputs
+ * and gradients are zero, and what they hold is not read.  A row with nothing to see gives zeros.
+ * lse: [n][n_heads][l] fp32, or NULL when no backward pass follows.  Backward: dtable may be NULL; partials:
+ * unet_rel_attn_bwd_partials(...) floats; delta: scratch of lse's shape. */
+#define UNET_REL_MAX_DISTANCE 512
+#define UNET_REL_MAX_SIDE 128
+int unet_rel_attn_fwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
+                      int32_t buckets, const int32_t* starts_host, const int32_t* lengths, int32_t n, int32_t l, int32_t c,
+                      int32_t n_heads, float scale, void* out, float* lse, void* stream);
+size_t unet_rel_attn_bwd_partials(int32_t dtype, int32_t n, int32_t l, int32_t n_heads, int32_t last_start);
+int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
+                      int32_t buckets, const int32_t* starts_host, const int32_t* lengths, const void* out, const float* lse,
+                      const void* dout, int32_t n, int32_t l, int32_t c, int32_t n_heads, float scale, void* dq, void* dk, void* dv,
+                      void* dtable, float* partials, float* delta, void* stream);
+
 /* AdamW with both moments in 8 bits (the fp32 form is above; train.py:1553-1559 keeps fp32 moments):
  *   m <- b1 m + (1-b1) g,  r <- sqrt(b2 r^2 + (1-b2) g^2),  p <- (1 - lr wd) p - lr/(1-b1^t) m / (r / sqrt(1-b2^t) + eps)
  * m and r are e4m3 codes with one fp32 scale per block of 256 elements of a tensor.  Tables of n_tensors <=

@@ -1,0 +1,54 @@
+// What the bf16 and fp32 kernels of relative-bias attention share: arguments, the bias of an offset, the sums of its gradient.
+#pragma once
+#include "common.h"
+
+struct RelK {
+  const void *q, *k, *v;       // [N][L][C], head h in columns h*hd .. h*hd+hd-1
+  void* out;                   // [N][L][C]
+  float* lse;                  // [N][nh][L] or null; log2 domain: p = exp2(s*scale_log2 + bias - lse); +inf: nothing to see
+  const void* dout;            // [N][L][C]
+  float* delta;                // [N][nh][L]: <dO, O> of a row and head
+  void *dq, *dk, *dv;          // [N][L][C]
+  const void* table;           // [buckets][nh], fp32 or bf16
+  float* part;                 // [nh][parts][2*sat+1] sums of dS by offset, one row per workgroup of the dQ kernel, or null
+  const int* lengths;          // [N] valid positions, or null
+  int n, l, c, nh, hd, buckets, sat, parts, table_f32;
+  float scale, scale_log2;
+  unsigned char bucket[UNET_REL_MAX_DISTANCE + 1];   // of |offset| = 0 .. sat within its side; sat: start of the last one
+};
+
+int unet_rel_attn_fwd_f32(const RelK& p, hipStream_t st);
+int unet_rel_attn_bwd_f32(const RelK& p, hipStream_t st);
+
+namespace {
+
+constexpr float REL_LOG2E = 1.4426950408889634f;
+constexpr float REL_LOWEST = -1e30f;    // finite biases stop here (log2 domain): the type's lowest value must not become -inf
+// LDS copy of a head's biases by offset: index REL_PAD + sat + offset, flat beyond +-sat for REL_PAD entries each way, so a
+// tile that touches the band between -sat and sat reads it without clamping
+constexpr int REL_PAD = 96;
+__device__ __host__ __forceinline__ int rel_width(int sat) { return 2 * sat + 1 + 2 * REL_PAD; }
+
+// bias of key j seen from query i, off = j - i, in the log2 domain.  A NaN entry stays NaN; a finite one is held above
+// REL_LOWEST (the type's lowest value times log2(e) would be -inf, which means "never").
+__device__ __forceinline__ float rel_bias(const RelK& p, int head, int off) {
+  const int a = min(abs(off), p.sat);
+  const int b = p.bucket[a] + (off > 0 ? p.buckets >> 1 : 0);
+  const float v = p.table_f32 ? static_cast<const float*>(p.table)[b * p.nh + head]
+                              : (float)static_cast<const __bf16*>(p.table)[b * p.nh + head];
+  return v == -INFINITY || v != v ? v : fmaxf(v * REL_LOG2E, REL_LOWEST);
+}
+
+__device__ __forceinline__ int rel_length(const RelK& p, int n) {
+  return p.lengths ? max(0, min(p.lengths[n], p.l)) : p.l;
+}
+
+__device__ __forceinline__ void rel_fill(const RelK& p, int head, float* bias, int tid, int threads) {
+  const int w = rel_width(p.sat);
+  for (int i = tid; i < w; i += threads) {
+    const int off = i - REL_PAD - p.sat;
+    bias[i] = rel_bias(p, head, max(-p.sat, min(off, p.sat)));
+  }
+}
+
+}  // namespace

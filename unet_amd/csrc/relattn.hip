@@ -1,0 +1,800 @@
+// Attention with a learned relative-position bias, bf16 MFMA, forward and backward:
+//   S[i, j] = scale <q_i, k_j> + table[bucket(j - i), head],   P = softmax_j S,   O = P V
+// The bias depends on the offset j - i alone: one value per offset up to the last bucket's start `sat`, constant beyond it on
+// either side.  A workgroup keeps its head's values in LDS; a tile whose offsets all lie beyond +-sat adds one scalar (folded
+// into the exponential's fma, so most of a long sequence pays nothing), the others read LDS once per score, conflict-free
+// because neighbouring lanes are neighbouring offsets.  A far bucket of -inf is never walked: attention to a local band costs
+// what the band costs.
+//
+// Forward and the two backward walks are the flash kernels of attn.hip for one band (128 query rows a workgroup, K / V tiles of
+// 64 keys double-buffered in LDS, S^T = K Q^T so that P is the next product's operand as it stands).  delta_i = <dO_i, O_i>,
+// dS = P o (dO V^T - delta); dV = P^T dO, dK = scale dS^T Q, dQ = scale dS K.
+//   d table[b, h] = sum of dS over the pairs of bucket b
+// is taken where dS is in registers anyway, in the dQ walk: far tiles add into one register a side, the others into a wave's
+// own LDS array by offset.  The two half-waves hold overlapping offsets and add one after the other, so every LDS word has one
+// writer an instruction and the order is fixed.  Workgroups write their sums by offset, a last launch adds them in a fixed
+// order: no atomics across workgroups, the same bits every time.
+#include "attn_tiles.h"
+#include "relattn.h"
+
+namespace {
+
+// the far side's constant for a tile with offsets dmin .. dmax, and whether it is one
+struct Far { bool far; float c; };
+__device__ __forceinline__ Far rel_far(int dmin, int dmax, int sat, float cneg, float cpos) {
+  return Far{dmax <= -sat || dmin >= sat, dmax <= -sat ? cneg : cpos};
+}
+
+template <int HDP>
+__global__ __launch_bounds__(AT_THREADS, 1) void rel_attn_fwd_kernel(const RelK p) {
+  typedef Cfg<HDP> G;
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][K tile | V tile], biases
+  float* const bias = reinterpret_cast<float*>(smem + 4 * G::TILE);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, h = lane >> 5;
+
+  int wg = xcd_remap(blockIdx.x, gridDim.x);
+  const int nqt = (p.l + AT_BQ - 1) / AT_BQ;
+  const int qt = wg % nqt; wg /= nqt;
+  const int head = wg % p.nh;
+  const int n = wg / p.nh;
+  const int len = rel_length(p, n);
+  const int hoff = head * p.hd;
+  const long long base = (long long)n * p.l * p.c + hoff;
+  const int q0 = qt * AT_BQ, qrow = q0 + wave * 32 + r;
+  const bool row_ok = qrow < len;
+  __bf16* const op = static_cast<__bf16*>(p.out) + base + (long long)qrow * p.c;
+  float* const lse = p.lse ? p.lse + ((long long)n * p.nh + head) * p.l + qrow : nullptr;
+
+  f32x16 acc[G::DT];
+#pragma unroll
+  for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+  float m = -INFINITY, lsum = 0.f, mtrue = -INFINITY;
+
+  if (q0 < len) {                                        // (uniform over the workgroup)
+    const __bf16* q = static_cast<const __bf16*>(p.q) + base + (long long)qrow * p.c;
+    bf16x8 qf[G::KS];
+#pragma unroll
+    for (int s = 0; s < G::KS; ++s) {
+      const int ch = 2 * s + h;
+      bf16x8 z;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = (__bf16)0.f;
+      qf[s] = (row_ok && ch * 8 < p.hd) ? *reinterpret_cast<const bf16x8*>(q + ch * 8) : z;
+    }
+    TileLoader<HDP> ld;
+    ld.setup(wave, lane, p.c, p.hd);
+    const int a0 = row_read_base<HDP>(lane);
+    const int vb0 = tr_read_base<HDP>(lane, 0), vb1 = tr_read_base<HDP>(lane, 1);
+    const float cneg = rel_bias(p, head, -p.sat), cpos = rel_bias(p, head, p.sat);
+    // key tiles that any row of the workgroup can see
+    const int nkb = (len + AT_BK - 1) / AT_BK;
+    const int kb_lo = cneg == -INFINITY ? max(0, q0 - p.sat + 1) / AT_BK : 0;
+    const int kb_hi = cpos == -INFINITY ? min(nkb, (q0 + AT_BQ - 2 + p.sat) / AT_BK + 1) : nkb;
+    const unsigned tile_step = (unsigned)AT_BK * p.c * 2;
+    auto issue = [&](int kb, int buf) {
+      char* at = smem + buf * 2 * G::TILE;
+      ld.issue(static_cast<const __bf16*>(p.k), base, len, p.c, p.hd, at, (unsigned)kb * tile_step, wave);
+      ld.issue(static_cast<const __bf16*>(p.v), base, len, p.c, p.hd, at + G::TILE, (unsigned)kb * tile_step, wave);
+    };
+    issue(kb_lo, 0);
+    rel_fill(p, head, bias, tid, AT_THREADS);
+    // m: the row maximum of the first tile with anything to see, then fixed (scores up to 2^32 above it stay inside fp32);
+    // a row that exceeds the margin sends the workgroup through a second walk with the true maxima
+    int bad = 0, buf = 0;
+    while (true) {
+      for (int kb = kb_lo; kb < kb_hi; ++kb) {
+        __syncthreads();
+        if (kb + 1 < kb_hi) issue(kb + 1, buf ^ 1);
+        const char* kt = smem + buf * 2 * G::TILE;
+        const char* vt = kt + G::TILE;
+        buf ^= 1;
+        const int key0 = kb * AT_BK, q0w = q0 + wave * 32;
+        const Far far = rel_far(key0 - q0w - 31, key0 + AT_BK - 1 - q0w, p.sat, cneg, cpos);
+        if (far.far && far.c == -INFINITY) continue;
+
+        f32x16 st[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) st[t][e] = 0.f;
+        bf16x8 fk[2][G::SB][2];
+        auto load_k = [&](int b, int slot) {
+#pragma unroll
+          for (int s4 = 0; s4 < G::SB; ++s4)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              fk[slot][s4][t] = *reinterpret_cast<const bf16x8*>(kt + ((a0 ^ ((b * G::SB + s4) << 5)) + t * 32 * G::ROWB));
+        };
+        load_k(0, 0);
+#pragma unroll
+        for (int b = 0; b < G::KS / G::SB; ++b) {
+          if (b + 1 < G::KS / G::SB) load_k(b + 1, (b + 1) & 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int s4 = 0; s4 < G::SB; ++s4)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+              st[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk[b & 1][s4][t], qf[b * G::SB + s4], st[t], 0, 0, 0);
+        }
+        bf16x8 fv[2][G::DT];
+        auto load_v = [&](int g, int slot) {
+          const int rowoff = (32 * (g >> 1) + 16 * (g & 1)) * G::ROWB;
+#pragma unroll
+          for (int d = 0; d < G::DT; ++d)
+            fv[slot][d] = tr_pair(vt + ((vb0 ^ (d << 6)) + rowoff), vt + ((vb1 ^ (d << 6)) + rowoff));
+        };
+        load_v(0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+
+        // score in the log2 domain = st * mul + add
+        float mul = p.scale_log2, add = far.c;
+        if (!far.far) {
+          const float* bl = bias + (key0 + 4 * h - qrow + p.sat + REL_PAD);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st[t][e] = fmaf(st[t][e], p.scale_log2, bl[32 * t + (e & 3) + 8 * (e >> 2)]);
+          mul = 1.f;
+          add = 0.f;
+        }
+        if (key0 + AT_BK > len) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (key0 + 32 * t + (e & 3) + 8 * (e >> 2) + 4 * h >= len) st[t][e] = -INFINITY;
+        }
+        float mx = st[0][0];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) mx = fmaxf(mx, st[t][e]);
+        mx = fmaf(fmaxf(mx, __shfl_xor(mx, 32, 64)), mul, add);
+        mtrue = fmaxf(mtrue, mx);
+        m = m == -INFINITY ? mx : m;
+        bad |= mx > m + 32.f;
+        const float shift = add - (m == -INFINITY ? 0.f : m);
+        auto exp_one = [&](int t, int e) {
+          const float pe = __builtin_amdgcn_exp2f(fmaf(st[t][e], mul, shift));
+          st[t][e] = pe;
+          lsum += pe;
+        };
+#pragma unroll
+        for (int e = 0; e < 8; ++e) exp_one(0, e);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int t = g >> 1, s = g & 1, tn = (g + 1) >> 1, sn = (g + 1) & 1;
+          const bf16x8 pb = pack8(st[t], s);
+          if (g < 3) load_v(g + 1, (g + 1) & 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int d = 0; d < G::DT; ++d) {
+            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv[g & 1][d], pb, acc[d], 0, 0, 0);
+            if (g < 3) {
+#pragma unroll
+              for (int x = d * 8 / G::DT; x < (d + 1) * 8 / G::DT; ++x) exp_one(tn, 8 * sn + x);
+            }
+          }
+        }
+      }
+      if (!(kb_hi - kb_lo > 1 && __syncthreads_or(bad))) break;
+      issue(kb_lo, buf);
+      m = mtrue;
+      lsum = 0.f;
+      bad = 0;
+#pragma unroll
+      for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+    }
+  }
+
+  // rows without a single visible key, and rows behind the window's length, give zeros
+  const float lt = lsum + __shfl_xor(lsum, 32, 64);
+  const bool seen = row_ok && lt > 0.f;
+  const bool spoiled = row_ok && lt != lt;
+  const float inv = seen ? 1.f / lt : spoiled ? lt : 0.f;
+  if (qrow < p.l) {
+    if (lse && h == 0) *lse = seen ? m + __builtin_amdgcn_logf(lt) : spoiled ? lt : INFINITY;
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int dd = 32 * d + 8 * e4 + 4 * h;
+        if (dd < p.hd) {
+          bf16x4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = (__bf16)(inv == 0.f ? 0.f : acc[d][4 * e4 + e] * inv);
+          *reinterpret_cast<bf16x4*>(op + dd) = o;
+        }
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// backward 1/4: delta = <dO, O> of every row and head.  One wave a row, HBM-bound.
+// ---------------------------------------------------------------------------------------------
+constexpr int RD_ROWS = 16, RD_CHUNKS = 1024;
+
+__global__ __launch_bounds__(AT_THREADS) void rel_attn_rowdot_kernel(const RelK p) {
+  __shared__ float part[4][RD_CHUNKS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = blockIdx.y, len = rel_length(p, n);
+  const int chunks = p.c >> 3, cph = p.hd >> 3;
+  for (int rr = 0; rr < RD_ROWS / 4; ++rr) {
+    const int row = blockIdx.x * RD_ROWS + wave * (RD_ROWS / 4) + rr;
+    if (row >= p.l) break;                         // wave-uniform
+    const __bf16* dop = static_cast<const __bf16*>(p.dout) + ((long long)n * p.l + row) * p.c;
+    const __bf16* op = static_cast<const __bf16*>(p.out) + ((long long)n * p.l + row) * p.c;
+    for (int ch = lane; ch < chunks; ch += 64) {
+      const bf16x8 a = *reinterpret_cast<const bf16x8*>(dop + ch * 8);
+      const bf16x8 b = *reinterpret_cast<const bf16x8*>(op + ch * 8);
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s = fmaf((float)a[e], (float)b[e], s);
+      part[wave][ch] = s;
+    }
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_s_waitcnt(0xc07f);            // lgkmcnt(0): the wave's own LDS writes are visible to its lanes
+    for (int head = lane; head < p.nh; head += 64) {
+      float s = 0.f;
+      for (int k = 0; k < cph; ++k) s += part[wave][head * cph + k];
+      p.delta[((long long)n * p.nh + head) * p.l + row] = row < len ? s : 0.f;
+    }
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// backward 2/4: dQ = scale dS K, and the sums of dS by offset
+// ---------------------------------------------------------------------------------------------
+template <int HDP>
+__global__ __launch_bounds__(AT_THREADS, 1) void rel_attn_dq_kernel(const RelK p) {
+  typedef Cfg<HDP> G;
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][K tile | V tile], biases, [4 waves] sums
+  const int w = rel_width(p.sat);
+  float* const bias = reinterpret_cast<float*>(smem + 4 * G::TILE);
+  float* const sums = bias + w;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, h = lane >> 5;
+
+  int wg = xcd_remap(blockIdx.x, gridDim.x);
+  const int nqt = (p.l + AT_BQ - 1) / AT_BQ;
+  const int qt = wg % nqt; wg /= nqt;
+  const int head = wg % p.nh;
+  const int n = wg / p.nh;
+  const int len = rel_length(p, n);
+  const int hoff = head * p.hd;
+  const long long base = (long long)n * p.l * p.c + hoff;
+  const int q0 = qt * AT_BQ, qrow = q0 + wave * 32 + r;
+  const bool row_ok = qrow < len;
+
+  f32x16 acc[G::DT];
+#pragma unroll
+  for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+  if (p.part)
+    for (int i = tid; i < 4 * w; i += AT_THREADS) sums[i] = 0.f;
+  float fneg = 0.f, fpos = 0.f;
+
+  if (q0 < len) {
+    const __bf16* qp = static_cast<const __bf16*>(p.q) + base + (long long)qrow * p.c;
+    const __bf16* dp_ = static_cast<const __bf16*>(p.dout) + base + (long long)qrow * p.c;
+    bf16x8 qf[G::KS], dof[G::KS];
+#pragma unroll
+    for (int s = 0; s < G::KS; ++s) {
+      const int ch = 2 * s + h;
+      bf16x8 z;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = (__bf16)0.f;
+      const bool ok = row_ok && ch * 8 < p.hd;
+      qf[s] = ok ? *reinterpret_cast<const bf16x8*>(qp + ch * 8) : z;
+      dof[s] = ok ? *reinterpret_cast<const bf16x8*>(dp_ + ch * 8) : z;
+    }
+    const long long si = ((long long)n * p.nh + head) * p.l + qrow;
+    const float lse = row_ok ? p.lse[si] : INFINITY;
+    const float delta = row_ok ? p.delta[si] : 0.f;
+    TileLoader<HDP> ld;
+    ld.setup(wave, lane, p.c, p.hd);
+    const int a0 = row_read_base<HDP>(lane);
+    const int vb0 = tr_read_base<HDP>(lane, 0), vb1 = tr_read_base<HDP>(lane, 1);
+    const float cneg = rel_bias(p, head, -p.sat), cpos = rel_bias(p, head, p.sat);
+    const int nkb = (len + AT_BK - 1) / AT_BK;
+    const int kb_lo = cneg == -INFINITY ? max(0, q0 - p.sat + 1) / AT_BK : 0;
+    const int kb_hi = cpos == -INFINITY ? min(nkb, (q0 + AT_BQ - 2 + p.sat) / AT_BK + 1) : nkb;
+    const unsigned tile_step = (unsigned)AT_BK * p.c * 2;
+    auto issue = [&](int kb, int buf) {
+      char* at = smem + buf * 2 * G::TILE;
+      ld.issue(static_cast<const __bf16*>(p.k), base, len, p.c, p.hd, at, (unsigned)kb * tile_step, wave);
+      ld.issue(static_cast<const __bf16*>(p.v), base, len, p.c, p.hd, at + G::TILE, (unsigned)kb * tile_step, wave);
+    };
+    issue(kb_lo, 0);
+    rel_fill(p, head, bias, tid, AT_THREADS);
+    int buf = 0;
+    for (int kb = kb_lo; kb < kb_hi; ++kb) {
+      __syncthreads();
+      if (kb + 1 < kb_hi) issue(kb + 1, buf ^ 1);
+      const char* kt = smem + buf * 2 * G::TILE;
+      const char* vt = kt + G::TILE;
+      buf ^= 1;
+      const int key0 = kb * AT_BK, q0w = q0 + wave * 32;
+      const Far far = rel_far(key0 - q0w - 31, key0 + AT_BK - 1 - q0w, p.sat, cneg, cpos);
+      if (far.far && far.c == -INFINITY) continue;
+
+      f32x16 st[2], dp[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { st[t][e] = 0.f; dp[t][e] = 0.f; }
+      constexpr int SB2 = G::SB < 2 ? G::SB : 2;
+      bf16x8 fk[2][SB2][2], fw[2][SB2][2];
+      auto load_kv = [&](int b, int slot) {
+#pragma unroll
+        for (int s2 = 0; s2 < SB2; ++s2)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const int o = (a0 ^ ((b * SB2 + s2) << 5)) + t * 32 * G::ROWB;
+            fk[slot][s2][t] = *reinterpret_cast<const bf16x8*>(kt + o);
+            fw[slot][s2][t] = *reinterpret_cast<const bf16x8*>(vt + o);
+          }
+      };
+      load_kv(0, 0);
+#pragma unroll
+      for (int b = 0; b < G::KS / SB2; ++b) {
+        if (b + 1 < G::KS / SB2) load_kv(b + 1, (b + 1) & 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s2 = 0; s2 < SB2; ++s2)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            st[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk[b & 1][s2][t], qf[b * SB2 + s2], st[t], 0, 0, 0);
+            dp[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fw[b & 1][s2][t], dof[b * SB2 + s2], dp[t], 0, 0, 0);
+          }
+      }
+      bf16x8 ft[2][G::DT];
+      auto load_t = [&](int g, int slot) {
+        const int rowoff = (32 * (g >> 1) + 16 * (g & 1)) * G::ROWB;
+#pragma unroll
+        for (int d = 0; d < G::DT; ++d)
+          ft[slot][d] = tr_pair(kt + ((vb0 ^ (d << 6)) + rowoff), kt + ((vb1 ^ (d << 6)) + rowoff));
+      };
+      load_t(0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      const bool ragged = key0 + AT_BK > len;
+      const float* bl = bias + (key0 + 4 * h - qrow + p.sat + REL_PAD);
+      float mul = p.scale_log2, add = far.c - lse;
+      if (!far.far) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) st[t][e] = fmaf(st[t][e], p.scale_log2, bl[32 * t + (e & 3) + 8 * (e >> 2)]);
+        mul = 1.f;
+        add = -lse;
+      }
+      float fsum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float pe = __builtin_amdgcn_exp2f(fmaf(st[t][e], mul, add));
+          if (ragged && key0 + 32 * t + (e & 3) + 8 * (e >> 2) + 4 * h >= len) pe = 0.f;
+          const float ds = pe * (dp[t][e] - delta);
+          st[t][e] = ds;
+          fsum += ds;
+        }
+      if (p.part) {
+        if (far.far) {
+          if (key0 < q0w) fneg += fsum; else fpos += fsum;
+        } else {
+          float* own = sums + wave * w + (bl - bias);
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            if (h == half) {
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                  __hip_atomic_fetch_add(own + 32 * t + (e & 3) + 8 * (e >> 2), st[t][e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const bf16x8 db = pack8(st[g >> 1], g & 1);
+        if (g < 3) load_t(g + 1, (g + 1) & 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < G::DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ft[g & 1][d], db, acc[d], 0, 0, 0);
+      }
+    }
+  }
+
+  if (qrow < p.l) {
+    __bf16* yp = static_cast<__bf16*>(p.dq) + base + (long long)qrow * p.c;
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int dd = 32 * d + 8 * e4 + 4 * h;
+        if (dd < p.hd) {
+          bf16x4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = (__bf16)(row_ok ? acc[d][4 * e4 + e] * p.scale : 0.f);
+          *reinterpret_cast<bf16x4*>(yp + dd) = o;
+        }
+      }
+  }
+  if (p.part) {
+    __syncthreads();
+    fneg = wave_sum(fneg);
+    fpos = wave_sum(fpos);
+    if (lane == 0) {
+      sums[wave * w] += fneg;
+      sums[wave * w + w - 1] += fpos;
+    }
+    __syncthreads();
+    float* row = p.part + ((long long)head * p.parts + n * nqt + qt) * (2 * p.sat + 1);
+    for (int i = tid; i < 2 * p.sat + 1; i += AT_THREADS) {
+      float s = 0.f;
+      const int lo = i == 0 ? 0 : i + REL_PAD, hi = i == 2 * p.sat ? w - 1 : i + REL_PAD;      // the flat ends belong to +-sat
+      for (int x = lo; x <= hi; ++x)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) s += sums[v * w + x];
+      row[i] = s;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// backward 3/4: dK = scale dS^T Q, dV = P^T dO.  A workgroup owns 64 keys and walks the query rows, 64 at a time; waves: 2 key
+// groups of 32 x 2 halves of the streamed rows, summed through LDS at the end.
+// ---------------------------------------------------------------------------------------------
+template <int HDP>
+__global__ __launch_bounds__(AT_THREADS, 1) void rel_attn_dkv_kernel(const RelK p) {
+  typedef Cfg<HDP> G;
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][Q tile | dO tile], [2][128] row stats, biases
+  float* const stats = reinterpret_cast<float*>(smem + 4 * G::TILE);
+  float* const bias = stats + 256;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kg = wave & 1, par = wave >> 1;
+  const int r = lane & 31, h = lane >> 5;
+
+  int wg = xcd_remap(blockIdx.x, gridDim.x);
+  const int nkt = (p.l + AT_BK - 1) / AT_BK;
+  const int ktl = wg % nkt; wg /= nkt;
+  const int head = wg % p.nh;
+  const int n = wg / p.nh;
+  const int len = rel_length(p, n);
+  const int hoff = head * p.hd;
+  const long long base = (long long)n * p.l * p.c + hoff;
+  const int key0 = ktl * AT_BK, key = key0 + kg * 32 + r;
+  const bool key_ok = key < len;
+
+  f32x16 dka[G::DT], dva[G::DT];
+#pragma unroll
+  for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) { dka[d][e] = 0.f; dva[d][e] = 0.f; }
+
+  if (key0 < len) {
+    const __bf16* kp = static_cast<const __bf16*>(p.k) + base + (long long)key * p.c;
+    const __bf16* vp = static_cast<const __bf16*>(p.v) + base + (long long)key * p.c;
+    bf16x8 kf[G::KS], vf[G::KS];
+#pragma unroll
+    for (int s = 0; s < G::KS; ++s) {
+      const int ch = 2 * s + h;
+      bf16x8 z;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = (__bf16)0.f;
+      const bool ok = key_ok && ch * 8 < p.hd;
+      kf[s] = ok ? *reinterpret_cast<const bf16x8*>(kp + ch * 8) : z;
+      vf[s] = ok ? *reinterpret_cast<const bf16x8*>(vp + ch * 8) : z;
+    }
+    TileLoader<HDP> ld;
+    ld.setup(wave, lane, p.c, p.hd);
+    const int a0 = row_read_base<HDP>(lane) + par * 32 * G::ROWB;
+    const int vb0 = tr_read_base<HDP>(lane, 0) + par * 32 * G::ROWB, vb1 = tr_read_base<HDP>(lane, 1) + par * 32 * G::ROWB;
+    const float cneg = rel_bias(p, head, -p.sat), cpos = rel_bias(p, head, p.sat);
+    // row tiles that can see any of the keys: row - key < sat if the left side is closed, key - row < sat if the right one is
+    const int nqb = (len + AT_BK - 1) / AT_BK;
+    const int qb_lo = cpos == -INFINITY ? max(0, key0 - p.sat + 1) / AT_BK : 0;
+    const int qb_hi = cneg == -INFINITY ? min(nqb, (key0 + AT_BK - 2 + p.sat) / AT_BK + 1) : nqb;
+    const unsigned tile_step = (unsigned)AT_BK * p.c * 2;
+    auto issue = [&](int qb, int buf) {
+      char* at = smem + buf * 2 * G::TILE;
+      ld.issue(static_cast<const __bf16*>(p.q), base, len, p.c, p.hd, at, (unsigned)qb * tile_step, wave);
+      ld.issue(static_cast<const __bf16*>(p.dout), base, len, p.c, p.hd, at + G::TILE, (unsigned)qb * tile_step, wave);
+    };
+    const long long sbase = ((long long)n * p.nh + head) * p.l;
+    auto load_stat = [&](int qb) {                   // threads 0..63: lse, 64..127: delta of the tile's rows
+      float v = tid < 64 ? INFINITY : 0.f;           // rows past the end: p = 0, delta = 0
+      const int row = qb * AT_BK + (tid & 63);
+      if (tid < 128 && row < len) v = tid < 64 ? p.lse[sbase + row] : p.delta[sbase + row];
+      return v;
+    };
+    issue(qb_lo, 0);
+    rel_fill(p, head, bias, tid, AT_THREADS);
+    if (tid < 128) stats[tid] = load_stat(qb_lo);
+    int buf = 0;
+    for (int qb = qb_lo; qb < qb_hi; ++qb, buf ^= 1) {
+      __syncthreads();   // the tile and its stats are in LDS; every wave is done with the other buffer
+      float stat_next = 0.f;
+      if (qb + 1 < qb_hi) {
+        issue(qb + 1, buf ^ 1);
+        stat_next = load_stat(qb + 1);
+      }
+      const char* qtile = smem + buf * 2 * G::TILE;
+      const char* dtile = qtile + G::TILE;
+      const float* st_in = stats + buf * 128;
+      const int row0w = qb * AT_BK + 32 * par, key0w = key0 + kg * 32;
+      const Far far = rel_far(key0w - row0w - 31, key0w + 31 - row0w, p.sat, cneg, cpos);
+      if (!(far.far && far.c == -INFINITY)) {
+        f32x16 st, dp;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) { st[e] = 0.f; dp[e] = 0.f; }
+        constexpr int SBK = G::SB < 2 ? G::SB : 2;
+        bf16x8 fq[2][SBK], fd[2][SBK];
+        auto load_qd = [&](int b, int slot) {
+#pragma unroll
+          for (int s4 = 0; s4 < SBK; ++s4) {
+            const int o = a0 ^ ((b * SBK + s4) << 5);
+            fq[slot][s4] = *reinterpret_cast<const bf16x8*>(qtile + o);
+            fd[slot][s4] = *reinterpret_cast<const bf16x8*>(dtile + o);
+          }
+        };
+        load_qd(0, 0);
+#pragma unroll
+        for (int b = 0; b < G::KS / SBK; ++b) {
+          if (b + 1 < G::KS / SBK) load_qd(b + 1, (b + 1) & 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int s4 = 0; s4 < SBK; ++s4) {
+            st = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fq[b & 1][s4], kf[b * SBK + s4], st, 0, 0, 0);
+            dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fd[b & 1][s4], vf[b * SBK + s4], dp, 0, 0, 0);
+          }
+        }
+        constexpr int NTB = 2 * G::DT;               // batches over (k-step s, d)
+        bf16x8 tq[2], td[2];
+        auto load_tt = [&](int b, int slot) {
+          const int s = b / G::DT, d0 = b % G::DT;
+          const int o0 = (vb0 ^ (d0 << 6)) + 16 * s * G::ROWB, o1 = (vb1 ^ (d0 << 6)) + 16 * s * G::ROWB;
+          td[slot] = tr_pair(dtile + o0, dtile + o1);
+          tq[slot] = tr_pair(qtile + o0, qtile + o1);
+        };
+        load_tt(0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        const float* bl = bias + (key - row0w - 4 * h - 27 + p.sat + REL_PAD);     // bl[27 - x]: local row x + 4h
+        float mul = p.scale_log2, add = far.c;
+        if (!far.far) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) st[e] = fmaf(st[e], p.scale_log2, bl[27 - 8 * (e >> 2) - (e & 3)]);
+          mul = 1.f;
+          add = 0.f;
+        }
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int rl = 32 * par + 8 * e4 + 4 * h;
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(st_in + rl);
+          const f32x4 de = *reinterpret_cast<const f32x4*>(st_in + 64 + rl);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float pe = __builtin_amdgcn_exp2f(fmaf(st[4 * e4 + e], mul, add - ls[e]));
+            st[4 * e4 + e] = pe;
+            dp[4 * e4 + e] = pe * (dp[4 * e4 + e] - de[e]);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < NTB; ++b) {
+          const int s = b / G::DT, d0 = b % G::DT;
+          const bf16x8 pb = pack8(st, s), db = pack8(dp, s);
+          if (b + 1 < NTB) load_tt(b + 1, (b + 1) & 1);
+          __builtin_amdgcn_sched_barrier(0);
+          dva[d0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(td[b & 1], pb, dva[d0], 0, 0, 0);
+          dka[d0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tq[b & 1], db, dka[d0], 0, 0, 0);
+        }
+      }
+      if (qb + 1 < qb_hi && tid < 128) stats[(buf ^ 1) * 128 + tid] = stat_next;
+    }
+  }
+
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);         // [kg][dk|dv][DT*16][64 lanes]
+  if (par == 1) {
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        red[((kg * 2 + 0) * G::DT * 16 + d * 16 + e) * 64 + lane] = dka[d][e];
+        red[((kg * 2 + 1) * G::DT * 16 + d * 16 + e) * 64 + lane] = dva[d][e];
+      }
+  }
+  __syncthreads();
+  if (par == 0 && key < p.l) {
+    __bf16* dk = static_cast<__bf16*>(p.dk) + base + (long long)key * p.c;
+    __bf16* dv = static_cast<__bf16*>(p.dv) + base + (long long)key * p.c;
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int dd = 32 * d + 8 * e4 + 4 * h;
+        if (dd < p.hd) {
+          bf16x4 ok, ov;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int x = d * 16 + 4 * e4 + e;
+            ok[e] = (__bf16)(key_ok ? (dka[d][4 * e4 + e] + red[((kg * 2 + 0) * G::DT * 16 + x) * 64 + lane]) * p.scale : 0.f);
+            ov[e] = (__bf16)(key_ok ? dva[d][4 * e4 + e] + red[((kg * 2 + 1) * G::DT * 16 + x) * 64 + lane] : 0.f);
+          }
+          *reinterpret_cast<bf16x4*>(dk + dd) = ok;
+          *reinterpret_cast<bf16x4*>(dv + dd) = ov;
+        }
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// backward 4/4: d table[b][head] = the sums of dS over the offsets of bucket b, added up over the dQ kernel's workgroups
+// ---------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(AT_THREADS) void rel_attn_dtable_kernel(const RelK p, void* dtable) {
+  __shared__ int range[2];
+  __shared__ float wsum[4];
+  const int b = blockIdx.x, head = blockIdx.y, side = p.buckets >> 1, tid = threadIdx.x;
+  const int local = b < side ? b : b - side;
+  if (tid == 0) { range[0] = p.sat + 1; range[1] = -1; }
+  __syncthreads();
+  for (int a = tid; a <= p.sat; a += AT_THREADS)
+    if (p.bucket[a] == local && !(a == 0 && b >= side)) { atomicMin(&range[0], a); atomicMax(&range[1], a); }
+  __syncthreads();
+  const int a0 = range[0], cnt = range[1] - range[0] + 1;      // distances a0 .. a0+cnt-1; none: cnt <= 0
+  float s = 0.f;
+  if (cnt > 0) {
+    const float* src = p.part + (long long)head * p.parts * (2 * p.sat + 1);
+    const int first = b < side ? p.sat - (a0 + cnt - 1) : p.sat + a0;
+    const long long total = (long long)p.parts * cnt;
+    for (long long i = tid; i < total; i += AT_THREADS) {
+      const long long row = i / cnt;
+      s += src[row * (2 * p.sat + 1) + first + (int)(i - row * cnt)];
+    }
+  }
+  s = wave_sum(s);
+  if ((tid & 63) == 0) wsum[tid >> 6] = s;
+  __syncthreads();
+  if (tid == 0) {
+    s = wsum[0] + wsum[1] + wsum[2] + wsum[3];
+    if (p.table_f32) static_cast<float*>(dtable)[b * p.nh + head] = s;
+    else static_cast<__bf16*>(dtable)[b * p.nh + head] = (__bf16)s;
+  }
+}
+
+#define REL_INSTANTIATE(HDP)                                     \
+  template __global__ void rel_attn_fwd_kernel<HDP>(const RelK); \
+  template __global__ void rel_attn_dq_kernel<HDP>(const RelK);  \
+  template __global__ void rel_attn_dkv_kernel<HDP>(const RelK);
+REL_INSTANTIATE(32)
+REL_INSTANTIATE(64)
+REL_INSTANTIATE(128)
+REL_INSTANTIATE(256)
+#undef REL_INSTANTIATE
+
+size_t bias_bytes(int sat, int copies) { return (size_t)rel_width(sat) * sizeof(float) * copies; }
+
+template <typename K> int set_lds(K kernel, size_t bytes, const char* what) {
+  if (bytes > 64 * 1024) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    UNET_REQUIRE(e == hipSuccess, "%s: hipFuncSetAttribute failed: %s", what, hipGetErrorString(e));
+  }
+  return 0;
+}
+
+template <int HDP> int launch_fwd(const RelK& p, hipStream_t st) {
+  const size_t lds = 4 * (size_t)Cfg<HDP>::TILE + bias_bytes(p.sat, 1);
+  if (set_lds(&rel_attn_fwd_kernel<HDP>, lds, "rel_attn_fwd")) return -1;
+  hipLaunchKernelGGL(rel_attn_fwd_kernel<HDP>, dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ))), dim3(AT_THREADS), lds, st, p);
+  UNET_LAUNCH_CHECK("rel_attn_fwd");
+  return 0;
+}
+
+template <int HDP> int launch_bwd(const RelK& p, hipStream_t st) {
+  const size_t lds_q = 4 * (size_t)Cfg<HDP>::TILE + bias_bytes(p.sat, p.part ? 5 : 1);
+  const size_t lds_kv = 4 * (size_t)Cfg<HDP>::TILE + 1024 + bias_bytes(p.sat, 1);
+  if (set_lds(&rel_attn_dq_kernel<HDP>, lds_q, "rel_attn_bwd (dq)") || set_lds(&rel_attn_dkv_kernel<HDP>, lds_kv, "rel_attn_bwd (dk, dv)"))
+    return -1;
+  hipLaunchKernelGGL(rel_attn_dq_kernel<HDP>, dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ))), dim3(AT_THREADS), lds_q, st, p);
+  UNET_LAUNCH_CHECK("rel_attn_bwd (dq)");
+  hipLaunchKernelGGL(rel_attn_dkv_kernel<HDP>, dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BK))), dim3(AT_THREADS), lds_kv, st, p);
+  UNET_LAUNCH_CHECK("rel_attn_bwd (dk, dv)");
+  return 0;
+}
+
+// argument checks shared by the entry points; fills everything of RelK but the tensors
+int make_rel(const char* what, RelK& p, int32_t dtype, int32_t n, int32_t l, int32_t c, int32_t nh, float scale, const void* table,
+             int32_t table_f32, int32_t buckets, const int32_t* starts_host, const int32_t* lengths) {
+  UNET_REQUIRE(dtype == UNET_BF16 || dtype == UNET_F32, "%s: bad dtype %d", what, dtype);
+  UNET_REQUIRE(table && starts_host, "%s: null pointer", what);
+  UNET_REQUIRE(n > 0 && l > 0 && c > 0 && nh > 0 && nh <= 256 && n <= 65535, "%s: bad shape n=%d l=%d c=%d heads=%d", what, n, l, c, nh);
+  const int unit = dtype == UNET_BF16 ? 8 : 4;
+  UNET_REQUIRE(c % nh == 0 && (c / nh) % unit == 0 && c / nh <= 256 && c <= 8 * RD_CHUNKS,
+               "%s: head_dim %d must be a multiple of %d and at most 256, channels at most %d (c=%d heads=%d)", what, c / nh, unit,
+               8 * RD_CHUNKS, c, nh);
+  UNET_REQUIRE((long long)l * c * (dtype == UNET_BF16 ? 2 : 4) < (1ll << 31), "%s: one [L, C] slab of %lld bytes exceeds a buffer descriptor",
+               what, (long long)l * c * (dtype == UNET_BF16 ? 2 : 4));
+  UNET_REQUIRE((long long)n * nh * cdiv(l, 32) < (1ll << 31), "%s: grid too large", what);
+  UNET_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite, got %g", what, (double)scale);
+  UNET_REQUIRE(buckets >= 4 && buckets % 2 == 0 && buckets <= 2 * UNET_REL_MAX_SIDE, "%s: %d buckets, must be even and 4 .. %d", what,
+               buckets, 2 * UNET_REL_MAX_SIDE);
+  const int side = buckets / 2;
+  UNET_REQUIRE(starts_host[0] == 0, "%s: the first bucket must start at distance 0", what);
+  for (int i = 1; i < side; ++i)
+    UNET_REQUIRE(starts_host[i] >= starts_host[i - 1], "%s: bucket starts must not decrease", what);
+  const int sat = starts_host[side - 1];
+  UNET_REQUIRE(sat >= 1 && sat <= UNET_REL_MAX_DISTANCE, "%s: the last bucket must start at distance 1 .. %d, got %d", what,
+               UNET_REL_MAX_DISTANCE, sat);
+  p.n = n; p.l = l; p.c = c; p.nh = nh; p.hd = c / nh; p.buckets = buckets; p.sat = sat;
+  p.table = table; p.table_f32 = table_f32; p.lengths = lengths;
+  p.scale = scale; p.scale_log2 = scale * REL_LOG2E;
+  for (int a = 0, b = 0; a <= sat; ++a) {
+    while (b + 1 < side && starts_host[b + 1] <= a) ++b;
+    p.bucket[a] = (unsigned char)b;
+  }
+  return 0;
+}
+
+int rel_parts(int dtype, int n, int l) { return n * cdiv(l, dtype == UNET_BF16 ? AT_BQ : 64); }
+
+}  // namespace
+
+extern "C" int unet_rel_attn_fwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
+                                 int32_t buckets, const int32_t* starts_host, const int32_t* lengths, int32_t n, int32_t l, int32_t c,
+                                 int32_t n_heads, float scale, void* out, float* lse, void* stream) {
+  RelK p = {};
+  UNET_REQUIRE(q && k && v && out, "rel_attn_fwd: null pointer");
+  if (make_rel("rel_attn_fwd", p, dtype, n, l, c, n_heads, scale, table, table_f32, buckets, starts_host, lengths)) return -1;
+  UNET_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), "rel_attn_fwd: pointers must be 16-byte aligned");
+  p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (dtype == UNET_F32) return unet_rel_attn_fwd_f32(p, st);
+  if (p.hd <= 32) return launch_fwd<32>(p, st);
+  if (p.hd <= 64) return launch_fwd<64>(p, st);
+  if (p.hd <= 128) return launch_fwd<128>(p, st);
+  return launch_fwd<256>(p, st);
+}
+
+extern "C" size_t unet_rel_attn_bwd_partials(int32_t dtype, int32_t n, int32_t l, int32_t n_heads, int32_t last_start) {
+  if (n <= 0 || l <= 0 || n_heads <= 0 || last_start < 0) return 0;
+  return (size_t)n_heads * rel_parts(dtype, n, l) * (2 * (size_t)last_start + 1);
+}
+
+extern "C" int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
+                                 int32_t buckets, const int32_t* starts_host, const int32_t* lengths, const void* out, const float* lse,
+                                 const void* dout, int32_t n, int32_t l, int32_t c, int32_t n_heads, float scale, void* dq, void* dk,
+                                 void* dv, void* dtable, float* partials, float* delta, void* stream) {
+  RelK p = {};
+  UNET_REQUIRE(q && k && v && out && lse && dout && dq && dk && dv && delta, "rel_attn_bwd: null pointer");
+  UNET_REQUIRE(!dtable || partials, "rel_attn_bwd: the table's gradient needs the partial sums");
+  if (make_rel("rel_attn_bwd", p, dtype, n, l, c, n_heads, scale, table, table_f32, buckets, starts_host, lengths)) return -1;
+  UNET_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(dout) && aligned16(dq) && aligned16(dk) &&
+                   aligned16(dv), "rel_attn_bwd: pointers must be 16-byte aligned");
+  p.q = q; p.k = k; p.v = v; p.out = const_cast<void*>(out); p.lse = const_cast<float*>(lse); p.dout = dout;
+  p.dq = dq; p.dk = dk; p.dv = dv; p.delta = delta; p.part = dtable ? partials : nullptr; p.parts = rel_parts(dtype, n, l);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  int rc;
+  if (dtype == UNET_F32) rc = unet_rel_attn_bwd_f32(p, st);
+  else {
+    hipLaunchKernelGGL(rel_attn_rowdot_kernel, dim3(cdiv(l, RD_ROWS), n), dim3(AT_THREADS), 0, st, p);
+    UNET_LAUNCH_CHECK("rel_attn_bwd (rowdot)");
+    rc = p.hd <= 32 ? launch_bwd<32>(p, st) : p.hd <= 64 ? launch_bwd<64>(p, st) : p.hd <= 128 ? launch_bwd<128>(p, st)
+                                                                                               : launch_bwd<256>(p, st);
+  }
+  if (rc || !dtable) return rc;
+  hipLaunchKernelGGL(rel_attn_dtable_kernel, dim3(buckets, n_heads), dim3(AT_THREADS), 0, st, p, dtable);
+  UNET_LAUNCH_CHECK("rel_attn_bwd (dtable)");
+  return 0;
+}

@@ -1767,3 +1767,117 @@ def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
             check(_lib.load().unet_gated_scan_step(_dt(x), _p(x), x.stride(0), _p(gate), gate.stride(0), _p(state), _p(h), n, c,
                                                    _stream_on(x)), "unet_gated_scan_step")
     return h
+
+
+# ---------------------------------------------------------------------------------------------
+# attention with a learned relative-position bias (csrc/relattn.hip, csrc/relattn_f32.hip)
+# ---------------------------------------------------------------------------------------------
+@functools.lru_cache(maxsize=None)
+def rel_bucket_starts(n_buckets: int, max_distance: int) -> Tuple[int, ...]:
+    """The smallest distance |j - i| of every bucket of one side (``n_buckets / 2`` of them).  The first half of a side's
+    buckets hold one distance each; the others grow geometrically, the last starts at the largest distance whose bucket the
+    geometric rule gives, at most ``max_distance``, and holds everything beyond.  Bucket e + k starts at the smallest a with
+    (a / e)^m >= (max_distance / e)^k, e single-distance and m growing buckets; in whole numbers, so no border depends on how a
+    logarithm rounds."""
+    side = n_buckets // 2
+    single = side // 2
+    grow = side - single
+    if n_buckets % 2 or n_buckets < 4 or side > _lib.REL_MAX_SIDE:
+        raise ValueError(f"relative-position buckets: an even number from 4 to {2 * _lib.REL_MAX_SIDE} is wanted, got {n_buckets}")
+    if not single < max_distance <= _lib.REL_MAX_DISTANCE:
+        raise ValueError(f"relative-position buckets: max_distance must be in {single + 1} .. {_lib.REL_MAX_DISTANCE} for {n_buckets} "
+                         f"buckets, got {max_distance}")
+    starts = list(range(single))
+    a = single
+    for k in range(grow):
+        while a ** grow * single ** k < max_distance ** k * single ** grow:
+            a += 1
+        starts.append(a)
+    return tuple(starts)
+
+
+def rel_bucket(offset: Tensor, n_buckets: int, max_distance: int) -> Tensor:
+    """Bucket of key j seen from query i for ``offset = j - i`` (any integer tensor): the second half of the buckets is for keys
+    behind the query (j > i)."""
+    starts = torch.tensor(rel_bucket_starts(n_buckets, max_distance), device=offset.device)
+    return torch.bucketize(offset.abs(), starts, right=True) - 1 + (offset > 0) * (n_buckets // 2)
+
+
+class RelBiasAttnFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, n_heads, scale, starts, lengths):
+        q, k, v, table = (t.detach().contiguous() for t in (q, k, v, table))
+        n, l, c = q.shape
+        keep = any(ctx.needs_input_grad[:4])
+        out = torch.empty_like(q)
+        lse = torch.empty((n, n_heads, l), dtype=torch.float32, device=q.device) if keep else None
+        arr = (C.c_int32 * len(starts))(*starts)
+        with torch.cuda.device(q.device):
+            check(_lib.load().unet_rel_attn_fwd(_dt(q), _p(q), _p(k), _p(v), _p(table), _dt(table), table.shape[0], arr, _p(lengths),
+                                                n, l, c, n_heads, scale, _p(out), _p(lse), _stream_on(q)), "unet_rel_attn_fwd")
+        if keep:
+            ctx.save_for_backward(q, k, v, table, out, lse, lengths)
+        ctx.n_heads, ctx.scale, ctx.starts = n_heads, scale, starts
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, table, out, lse, lengths = ctx.saved_tensors
+        n, l, c = q.shape
+        lib = _lib.load()
+        dout = dout.to(q.dtype).contiguous()
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        delta = torch.empty_like(lse)
+        dtable = partials = None
+        if ctx.needs_input_grad[3]:
+            dtable = torch.empty_like(table)
+            partials = torch.empty(int(lib.unet_rel_attn_bwd_partials(_dt(q), n, l, ctx.n_heads, ctx.starts[-1])), dtype=torch.float32,
+                                   device=q.device)
+        arr = (C.c_int32 * len(ctx.starts))(*ctx.starts)
+        with torch.cuda.device(q.device):
+            check(lib.unet_rel_attn_bwd(_dt(q), _p(q), _p(k), _p(v), _p(table), _dt(table), table.shape[0], arr, _p(lengths), _p(out),
+                                        _p(lse), _p(dout), n, l, c, ctx.n_heads, ctx.scale, _p(dq), _p(dk), _p(dv), _p(dtable),
+                                        _p(partials), _p(delta), _stream_on(q)), "unet_rel_attn_bwd")
+        return dq, dk, dv, dtable, None, None, None, None
+
+
+def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: int, scale: Optional[float] = None,
+                       max_distance: int = 128, lengths: Optional[Tensor] = None) -> Tensor:
+    """Multi-head self-attention with a learned bias for the relative position of key and query:
+
+        S[i, j] = scale <q_i, k_j> + table[bucket(j - i), head],   out_i = sum_j softmax_j(S[i, :]) v_j
+
+    ``q``, ``k``, ``v``: ``[N, L, C]``, all bf16 or all fp32; head h owns columns ``h*hd .. h*hd+hd-1``, ``hd = C / n_heads`` a
+    multiple of 8 (bf16) or 4 (fp32), at most 256.  ``table``: ``[n_buckets, n_heads]`` fp32 or bf16 (``rel_bucket`` gives the
+    buckets; ``max_distance`` at most 512); an entry of -inf removes its pairs, and a far bucket of -inf also their cost.
+    ``lengths``: ``[N]`` int32 valid positions of a padded batch (values are clamped to 0 .. L): positions behind them are
+    neither keys nor queries, their outputs and gradients are zero.  A row with nothing to see gives zeros.  ``scale`` defaults
+    to ``hd ** -0.5`` and must be positive.
+
+    Scores, softmax statistics and all sums are fp32; in bf16 the probabilities and dS are rounded to bf16 as operands of the
+    next product.  Differentiable (once) in q, k, v and table; the table's gradient is added up in a fixed order."""
+    if q.dim() != 3 or k.shape != q.shape or v.shape != q.shape:
+        raise ValueError(f"rel_bias_attention: q, k, v must all be [N, L, C], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    unit = 8 if _dt(q) == _lib.BF16 else 4
+    if k.dtype != q.dtype or v.dtype != q.dtype or any(t.device != q.device for t in (k, v, table)):
+        raise TypeError("rel_bias_attention: q, k and v must have one dtype and all tensors one device")
+    n, l, c = q.shape
+    if n_heads < 1 or n_heads > 256 or c % n_heads or (c // n_heads) % unit or c // n_heads > 256 or c > 8192:
+        raise ValueError(f"rel_bias_attention: {c} channels in {n_heads} heads: the head size must be a multiple of {unit} for {q.dtype} "
+                         "and at most 256 (at most 256 heads and 8192 channels)")
+    if table.dim() != 2 or table.shape[1] != n_heads:
+        raise ValueError(f"rel_bias_attention: the table must be [n_buckets, {n_heads}], got {tuple(table.shape)}")
+    _dt(table)
+    starts = rel_bucket_starts(table.shape[0], int(max_distance))
+    scale = (c // n_heads) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"rel_bias_attention: scale must be positive and finite, got {scale}")
+    if lengths is not None:
+        if lengths.shape != (n,) or lengths.dtype != torch.int32 or lengths.device != q.device:
+            raise ValueError(f"rel_bias_attention: lengths must be int32 [{n}] on {q.device}")
+        lengths = lengths.contiguous()
+    _need_cuda(q)
+    if q.numel() == 0:
+        return q * k * v + 0 * table.sum().to(q.dtype)
+    return RelBiasAttnFn.apply(q, k, v, table, n_heads, scale, starts, lengths)
