@@ -73,9 +73,9 @@ def parse():
     ap.add_argument("--cpu-windows", type=int, default=8, help="windows per CPU-baseline step (1 warm-up + 3 timed steps "
                     "at each thread count)")
     ap.add_argument("--no-kernel-timing", action="store_true")
-    ap.add_argument("--optimizer", default="native", choices=["native", "torch"],
-                    help="native: unet_amd.optim.ClipAdamW (clip + AdamW in three HIP launches); torch: "
-                         "clip_grad_norm_ + torch.optim.AdamW(fused=True)")
+    ap.add_argument("--optimizer", default="native", choices=["native", "native8", "torch"],
+                    help="native: unet_amd.optim.ClipAdamW (clip + AdamW in three HIP launches); native8: the same with its "
+                         "moments in 8 bits; torch: clip_grad_norm_ + torch.optim.AdamW(fused=True)")
     ap.add_argument("--conditioning", default="odor_onehot", choices=["odor_onehot", "spectro_temporal"],
                     help="spectro_temporal: the SpectroTemporalEncoder (train.py --conditioning default) runs inside the "
                          "step and trains with the model; the headline config is odor_onehot")
@@ -196,12 +196,12 @@ def main():
     BETAS = (0.7595905764360957, 0.920298282605139)                         # train.py:183-193
 
     def make_optimizer(capturable):
-        if args.optimizer == "native":     # K17: clip 5.0 + AdamW as three HIP launches (the encoder keeps its own clip)
+        if args.optimizer != "torch":      # K17: clip 5.0 + AdamW as three HIP launches (the encoder keeps its own clip)
             from unet_amd.optim import ClipAdamW
             groups[0]["max_grad_norm"] = 5.0
             for grp in groups[1:]:
                 grp["max_grad_norm"] = None
-            return ClipAdamW(groups, lr=2e-4, betas=BETAS, weight_decay=0.0)
+            return ClipAdamW(groups, lr=2e-4, betas=BETAS, weight_decay=0.0, state_bits=8 if args.optimizer == "native8" else 32)
         return torch.optim.AdamW(groups, lr=2e-4, betas=BETAS, weight_decay=0.0, fused=True, capturable=capturable)
 
     opt = make_optimizer(not args.eager)

@@ -214,6 +214,86 @@ class SelfAttention1D(nn.Module):
         return _as_ncl(self.forward_nlc(_to_nlc(x)))
 
 
+class RelativeSelfAttention1D(SelfAttention1D):
+    """``SelfAttention1D`` whose scores know how far key and query are apart (no counterpart in the reference, whose attention
+    sees no positions; ``attention_type="relative"``): each of the ``reduction`` heads of value channels adds a learned bias for
+    the bucket of the offset to the shared scores.  A zero ``rel_table`` -- its initial value -- is ``SelfAttention1D``, so a
+    checkpoint of that module continues from where it was."""
+
+    def __init__(self, channels: int, reduction: int = 8, n_buckets: int = 32, max_distance: int = 128):
+        if channels % reduction or (channels // reduction) % 8 or channels // reduction > 256:
+            raise ValueError(f"RelativeSelfAttention1D: channels / reduction must be a multiple of 8 up to 256, got {channels} / {reduction}")
+        super().__init__(channels, reduction)
+        self.max_distance = max_distance
+        ops.rel_bucket_starts(n_buckets, max_distance)            # checks both
+        self.rel_table = nn.Parameter(torch.zeros(n_buckets, reduction))
+
+    def forward_nlc(self, x: Tensor, lengths: Optional[Tensor] = None) -> Tensor:
+        """``lengths``: ``[N]`` int32 valid rows of a padded batch; the rows behind them pass through unchanged."""
+        g1 = ops.geom_conv(1)
+        l, heads = x.shape[1], self.rel_table.shape[1]
+        q, k, v = (ops.conv(x, m.weight.permute(2, 0, 1), m.bias, g1, l) for m in (self.query, self.key, self.value))
+        # every head sees the same q and k (tiled as SelfAttention1D does); its own bias tells its scores apart
+        out = ops.rel_bias_attention(q.repeat(1, 1, heads), k.repeat(1, 1, heads), v, self.rel_table, heads, 1.0, self.max_distance,
+                                     lengths)
+        return (x.float() + self.gamma.float() * out.float()).to(x.dtype)
+
+    def extra_repr(self) -> str:
+        return f"channels={self.channels}, buckets={self.rel_table.shape[0]}, max_distance={self.max_distance}"
+
+
+class GatedRecurrence1D(nn.Module):
+    """Mixes rows by a gated linear recurrence instead of attention: linear in the window's length (no counterpart in the
+    reference; ``attention_type="recurrent"``).  Per direction a value and a forget-gate projection feed ``ops.gated_scan``; the
+    directions' states meet in one 1x1 conv, and a gated residual that starts at zero adds the result.  The forget gates
+    start with memories from 1 to 256 rows, spread over the channels.
+
+    ``bidirectional=False`` is causal and can run row by row: ``forward_step``."""
+
+    def __init__(self, channels: int, bidirectional: bool = True):
+        super().__init__()
+        self.channels, self.bidirectional = channels, bidirectional
+        dirs = 2 if bidirectional else 1
+        self.value = nn.ModuleList([nn.Conv1d(channels, channels, 1) for _ in range(dirs)])
+        self.forget = nn.ModuleList([nn.Conv1d(channels, channels, 1) for _ in range(dirs)])
+        self.out_proj = nn.Conv1d(dirs * channels, channels, 1)
+        self.gamma = nn.Parameter(torch.zeros(1))
+        with torch.no_grad():
+            for m in self.forget:
+                m.bias.copy_(torch.linspace(0.0, math.log(256.0), channels))
+
+    def train(self, mode: bool = True):
+        if mode:
+            ops.clear_pack_cache()          # as CondUNet1D.train: fused optimizers do not bump the parameters' versions
+        return super().train(mode)
+
+    @staticmethod
+    def _proj(m: nn.Conv1d, x: Tensor, x2: Optional[Tensor] = None) -> Tensor:
+        return ops.conv(x, m.weight.permute(2, 0, 1), m.bias, ops.geom_conv(1), x.shape[1], x2=x2, params=(m.weight, m.bias))
+
+    def forward_nlc(self, x: Tensor) -> Tensor:
+        h = [ops.gated_scan(self._proj(v, x), self._proj(f, x), reverse=bool(i)) for i, (v, f) in enumerate(zip(self.value, self.forget))]
+        out = self._proj(self.out_proj, h[0], h[1] if self.bidirectional else None)
+        return (x.float() + self.gamma.float() * out.float()).to(x.dtype)
+
+    def forward(self, x: Tensor) -> Tensor:
+        return _as_ncl(self.forward_nlc(_to_nlc(x)))
+
+    @torch.no_grad()
+    def forward_step(self, x: Tensor, state: Tensor) -> Tensor:
+        """One new row of every recording: ``x`` ``[N, C]``, ``state`` ``[N, C]`` fp32 (zeros at the start), moved on in place.
+        Row by row this is ``forward`` of the causal module."""
+        if self.bidirectional:
+            raise ValueError("GatedRecurrence1D.forward_step: the backward direction needs the whole window (bidirectional=False)")
+        row = x[:, None, :]
+        h = ops.gated_scan_step(self._proj(self.value[0], row)[:, 0], self._proj(self.forget[0], row)[:, 0], state)
+        out = self._proj(self.out_proj, h[:, None, :])[:, 0]
+        return (x.float() + self.gamma.float() * out.float()).to(x.dtype)
+
+    def extra_repr(self) -> str:
+        return f"channels={self.channels}, bidirectional={self.bidirectional}"
+
+
 def _band_pair_attention(q: Tensor, k: Tensor, v: Tensor, coupling: Tensor, n_heads: int, scale: float) -> Tensor:
     """q, k, v: [nb, M, l, C] stacks of the per-band projections -> [M, l, nb*C]:
     out[:, :, i*C + h*hd + d] = sum_j coupling[i, j] * softmax(q_i k_j^T * scale) v_j   (models.py:431-462 / 191-216).
@@ -868,7 +948,12 @@ class CondUNet1D(nn.Module):
             return CrossFrequencyCouplingAttentionV2(channels, n_heads=self.n_heads)
         if attention_type == "cross_freq":
             return CrossFrequencyCouplingAttention(channels, n_heads=self.n_heads)
-        raise ValueError(f"Unknown attention_type: {attention_type}. Available: none, basic, cross_freq, cross_freq_v2")
+        if attention_type == "relative":
+            return RelativeSelfAttention1D(channels)
+        if attention_type == "recurrent":
+            return GatedRecurrence1D(channels)
+        raise ValueError(f"Unknown attention_type: {attention_type}. Available: none, basic, cross_freq, cross_freq_v2, relative, "
+                         "recurrent")
 
     def set_gradient_checkpointing(self, enable: bool = True):
         self.gradient_checkpointing = enable

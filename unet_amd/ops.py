@@ -290,25 +290,30 @@ class MergeBranchesFn(torch.autograd.Function):
 # ---------------------------------------------------------------------------------------------
 # conv launchers
 # ---------------------------------------------------------------------------------------------
+def _pitch(t: Tensor) -> int:
+    """Row pitch of [N, L, C]; the only row of a window may carry any stride (a transposed [N, C, 1] has 1)."""
+    return t.stride(1) if t.shape[1] > 1 else max(t.stride(1), t.shape[2])
+
+
 def _desc(geom: ConvGeom, x1: Tensor, x2: Optional[Tensor], y: Tensor, res: Optional[Tensor], act: int = 0) -> ConvDesc:
     if geom.n_taps > _lib.MAX_TAPS:
         raise ValueError(f"{geom.n_taps} taps exceed UNET_MAX_TAPS={_lib.MAX_TAPS}")
     d = ConvDesc()
     d.dtype = _dt(x1)
     d.n, d.l_in, d.c1 = x1.shape
-    d.x1_ld, d.x1_ns = x1.stride(1), x1.stride(0)
+    d.x1_ld, d.x1_ns = _pitch(x1), x1.stride(0)
     if x2 is not None:
         if x2.shape[:2] != x1.shape[:2] or x2.dtype != x1.dtype:
             raise ValueError("concat sources must agree in batch, length and dtype")
-        d.c2, d.x2_ld, d.x2_ns = x2.shape[2], x2.stride(1), x2.stride(0)
+        d.c2, d.x2_ld, d.x2_ns = x2.shape[2], _pitch(x2), x2.stride(0)
     else:
         d.c2, d.x2_ld, d.x2_ns = 0, 0, 0
     d.l_out, d.c_out = y.shape[1], y.shape[2]
-    d.y_ld, d.y_ns = y.stride(1), y.stride(0)
+    d.y_ld, d.y_ns = _pitch(y), y.stride(0)
     if res is not None:
         if res.shape != y.shape or res.dtype != y.dtype:
             raise ValueError(f"residual {tuple(res.shape)}/{res.dtype} does not match output {tuple(y.shape)}/{y.dtype}")
-        d.res_ld, d.res_ns = res.stride(1), res.stride(0)
+        d.res_ld, d.res_ns = _pitch(res), res.stride(0)
     d.stride, d.up, d.n_taps = geom.stride, geom.up, geom.n_taps
     for j, (o, r) in enumerate(zip(geom.offs, geom.phases)):
         d.tap_off[j] = o

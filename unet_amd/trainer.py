@@ -47,9 +47,10 @@ class Trainer:
                  use_graph: bool = False, bucket_bytes: int = 64 << 20, nan_check_every: int = 50, process_group=None,
                  cond_encoder: Optional[torch.nn.Module] = None, noise_augmentor: Optional[torch.nn.Module] = None,
                  loss_fn: Optional[Callable] = None, normalize_target: Optional[Callable] = None,
-                 optimizer: Optional[str] = None):
+                 optimizer: Optional[str] = None, state_bits: int = 32):
         """``optimizer``: "native" (``optim.ClipAdamW``: clip + AdamW as three HIP launches, the default on a GPU) or
         "torch" (``clip_grad_norm_`` + ``torch.optim.AdamW``, the default on CPU).
+        ``state_bits``: 8 keeps the native optimizer's moments in 8 bits (a quarter of the state's memory).
         ``loss_fn(pred, target)`` / ``normalize_target(target)`` default to the reference's step
         (``weight_l1 * l1_crop_loss`` on the HIP kernels after ``per_channel_normalize``); the host-logic tests
         pass plain torch callables so that the data-parallel protocol runs on CPU under gloo."""
@@ -75,12 +76,14 @@ class Trainer:
         self.use_graph = use_graph
         if optimizer is None:
             optimizer = "native" if next(model.parameters()).is_cuda else "torch"
+        if state_bits != 32 and optimizer != "native":
+            raise ValueError(f"state_bits={state_bits} needs the native optimizer, not {optimizer!r}")
         if optimizer == "native":     # K17: clip + AdamW in three HIP launches (unet_amd/optim.py); the model's clip runs
             from .optim import ClipAdamW   # inside step(), the encoder's stays in front of its gradient average
             groups[0]["max_grad_norm"] = grad_clip
             for g in groups[1:]:
                 g["max_grad_norm"] = None
-            self.opt = ClipAdamW(groups, lr=lr, betas=betas, weight_decay=weight_decay)
+            self.opt = ClipAdamW(groups, lr=lr, betas=betas, weight_decay=weight_decay, state_bits=state_bits)
         elif optimizer == "torch":
             self.opt = torch.optim.AdamW(groups, lr=lr, betas=betas, weight_decay=weight_decay, fused=True,
                                          capturable=use_graph)
