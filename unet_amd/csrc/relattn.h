@@ -27,7 +27,7 @@ constexpr float REL_LOWEST = -1e30f;    // finite biases stop here (log2 domain)
 // LDS copy of a head's biases by offset: index REL_PAD + sat + offset, flat beyond +-sat for REL_PAD entries each way, so a
 // tile that touches the band between -sat and sat reads it without clamping
 constexpr int REL_PAD = 96;
-__device__ __host__ __forceinline__ int rel_width(int sat) { return 2 * sat + 1 + 2 * REL_PAD; }
+__device__ __host__ __forceinline__ int rel_width(int sat) { return (2 * sat + 1 + 2 * REL_PAD + 3) & ~3; }      // 16-byte multiple
 
 // bias of key j seen from query i, off = j - i, in the log2 domain.  A NaN entry stays NaN; a finite one is held above
 // REL_LOWEST (the type's lowest value times log2(e) would be -inf, which means "never").
