@@ -17,8 +17,10 @@
 namespace {
 
 constexpr int A8_THREADS = 256;
-constexpr int A8_PER_WAVE = 8;                                   // blocks of 256 elements
-constexpr int A8_PER_WG = A8_PER_WAVE * (A8_THREADS / 64);
+// Blocks of 256 elements a wave: eight when they fill the chip (two workgroups a CU at least), otherwise one, so that a small
+// model's step is as short as one block's (126 k parameters: 17 workgroups took 19 us, 124 take 6).
+constexpr int A8_WAVES = A8_THREADS / 64, A8_MANY = 8;
+int per_wave(long long blocks256) { return blocks256 >= 512ll * A8_MANY * A8_WAVES ? A8_MANY : 1; }
 constexpr unsigned A8_WIDE = 0x80000000u;                        // slot flag: 32-bit moments
 constexpr float A8_MAX = 448.f, A8_LEAST = 0.001953125f;         // largest and smallest positive e4m3 value
 constexpr float A8_TINY = 7.888609052210118e-31f;                // 2^-100
@@ -89,10 +91,11 @@ __device__ __forceinline__ int find_tensor(const unsigned* start, int n, unsigne
   return lo;
 }
 
+template <int A8_PER_WAVE>
 __global__ __launch_bounds__(A8_THREADS) void adamw8_apply_kernel(const Adam8 k, const GradPtrs gp) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned end = k.start[k.n];
-  const unsigned b0 = k.start[0] + blockIdx.x * A8_PER_WG + wave * A8_PER_WAVE;
+  const unsigned b0 = k.start[0] + (blockIdx.x * A8_WAVES + wave) * A8_PER_WAVE;
   const unsigned b1 = b0 + A8_PER_WAVE < end ? b0 + A8_PER_WAVE : end;
   const float clip = k.coef[0], keep = 1.f - k.coef[4] * k.weight_decay;
   float sq = 0.f;
@@ -107,7 +110,7 @@ __global__ __launch_bounds__(A8_THREADS) void adamw8_apply_kernel(const Adam8 k,
       // the usual case: eight whole blocks of one tensor
       if (g0) {
         const float2 bc = k.bc[t];
-        constexpr int Q = 4;
+        constexpr int Q = A8_PER_WAVE < 4 ? A8_PER_WAVE : 4;
 #pragma unroll
         for (int h = 0; h < A8_PER_WAVE / Q; ++h) {
           f32x4 gv[Q], pv[Q];
@@ -248,7 +251,10 @@ __global__ __launch_bounds__(PREP_THREADS) void adamw8_prepare_kernel(const Grad
 
 }  // namespace
 
-extern "C" int32_t unet_adamw8_blocks(int64_t blocks256) { return (int32_t)((blocks256 + A8_PER_WG - 1) / A8_PER_WG); }
+extern "C" int32_t unet_adamw8_blocks(int64_t blocks256) {
+  const int per = per_wave(blocks256) * A8_WAVES;
+  return (int32_t)((blocks256 + per - 1) / per);
+}
 
 extern "C" int unet_adamw8_prepare(const float* const* grads_host, int32_t n_tensors, const float* partial, int32_t n_partial,
                                    int32_t advance, float max_norm, const float* lr, float* coef, float* step_t, double beta1,
@@ -286,8 +292,9 @@ extern "C" int unet_adamw8_apply(const float* const* grads_host, int32_t n_tenso
   k.eps = eps; k.weight_decay = weight_decay; k.n = n_tensors;
   GradPtrs gp;
   for (int i = 0; i < UNET_OPT_MAX_TENSORS; ++i) gp.g[i] = i < n_tensors ? grads_host[i] : nullptr;
-  hipLaunchKernelGGL(adamw8_apply_kernel, dim3(unet_adamw8_blocks(blocks256)), dim3(A8_THREADS), 0, static_cast<hipStream_t>(stream),
-                     k, gp);
+  const dim3 grid(unet_adamw8_blocks(blocks256));
+  if (per_wave(blocks256) == 1) hipLaunchKernelGGL(adamw8_apply_kernel<1>, grid, dim3(A8_THREADS), 0, static_cast<hipStream_t>(stream), k, gp);
+  else hipLaunchKernelGGL(adamw8_apply_kernel<A8_MANY>, grid, dim3(A8_THREADS), 0, static_cast<hipStream_t>(stream), k, gp);
   UNET_LAUNCH_CHECK("adamw8_apply");
   return 0;
 }

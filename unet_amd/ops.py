@@ -1666,8 +1666,28 @@ def band_project(bands: Tensor, wq, bq, wk, bk, wv, bv):
 # ---------------------------------------------------------------------------------------------
 # gated linear recurrence along the rows (csrc/scan.hip)
 # ---------------------------------------------------------------------------------------------
-def _stream_on(t: Tensor) -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+def _run(what: str, t: Tensor, *args):
+    """Library call ``what`` on ``t``'s device and that device's current stream (its last argument).  Tensors go in as their
+    pointers; a call of a few microseconds notices every Python object made on the way."""
+    dev = t.device.index
+    fn = getattr(_lib.load(), what)
+    args = [a.data_ptr() if isinstance(a, Tensor) else a for a in args]
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        check(rc, what)
+
+
+def _wants_grad(*tensors: Optional[Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _once_differentiable(what: str):
+    if torch.is_grad_enabled():        # create_graph=True: the kernels' outputs would enter the second graph as constants
+        raise RuntimeError(f"{what} is differentiable once: its backward pass cannot be differentiated (create_graph=True)")
 
 
 def _dense_channels(t: Tensor) -> Tensor:
@@ -1691,50 +1711,52 @@ def _check_scan(what: str, x: Tensor, gate: Tensor, state: Optional[Tensor], dim
     _need_cuda(x)
 
 
+def _scan_workspace(x: Tensor, n: int, l: int, c: int):
+    size = int(_lib.load().unet_gated_scan_workspace_bytes(_dt(x), n, l, c))
+    return (torch.empty(size, dtype=torch.uint8, device=x.device) if size else None), size
+
+
+def _scan_forward(x: Tensor, gate: Tensor, h0: Optional[Tensor], reverse: bool, keep: bool):
+    """(h, last, states): ``states`` is what backward starts from, the fp32 state in front of every tile of rows."""
+    n, l, c = x.shape
+    h = torch.empty((n, l, c), dtype=x.dtype, device=x.device)
+    last = torch.empty((n, c), dtype=torch.float32, device=x.device)
+    states = None
+    if keep:
+        states = torch.empty((n, -(-l // _lib.load().unet_gated_scan_tile()), c), dtype=torch.float32, device=x.device)
+    ws, size = _scan_workspace(x, n, l, c)
+    _run("unet_gated_scan_fwd", x, _dt(x), x, x.stride(0), x.stride(1), gate, gate.stride(0), gate.stride(1), h0, reverse, n, l, c, h,
+         last, states, ws, size)
+    return h, last, states
+
+
 class GatedScanFn(torch.autograd.Function):
     """(h, last) of ``gated_scan``; keeps the fp32 state in front of every 64th row for backward."""
 
     @staticmethod
     def forward(ctx, x, gate, h0, reverse):
-        x, gate = _dense_channels(x.detach()), _dense_channels(gate.detach())
-        h0 = None if h0 is None else h0.detach().contiguous()
-        n, l, c = x.shape
-        lib = _lib.load()
-        keep = any(ctx.needs_input_grad[:3])
-        h = torch.empty((n, l, c), dtype=x.dtype, device=x.device)
-        last = torch.empty((n, c), dtype=torch.float32, device=x.device)
-        tile = int(lib.unet_gated_scan_tile())
-        states = torch.empty((n, -(-l // tile), c), dtype=torch.float32, device=x.device) if keep else None
-        size = int(lib.unet_gated_scan_workspace_bytes(_dt(x), n, l, c))
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        with torch.cuda.device(x.device):
-            check(lib.unet_gated_scan_fwd(_dt(x), _p(x), x.stride(0), x.stride(1), _p(gate), gate.stride(0), gate.stride(1), _p(h0),
-                                          int(reverse), n, l, c, _p(h), _p(last), _p(states), _p(ws), size, _stream_on(x)),
-                  "unet_gated_scan_fwd")
-        if keep:
-            ctx.save_for_backward(x, gate, states)
+        h, last, states = _scan_forward(x, gate, h0, reverse, True)
+        ctx.save_for_backward(x, gate, states)
         ctx.reverse = reverse
         ctx.set_materialize_grads(False)
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast):
+        _once_differentiable("gated_scan")
         if dh is None and dlast is None:
             return None, None, None, None
         x, gate, states = ctx.saved_tensors
         n, l, c = x.shape
-        lib = _lib.load()
-        dh = torch.zeros((n, l, c), dtype=x.dtype, device=x.device) if dh is None else _dense_channels(dh.to(x.dtype))
-        dlast = None if dlast is None else dlast.to(torch.float32).contiguous()
-        dx, dg = (torch.empty((n, l, c), dtype=x.dtype, device=x.device) for _ in range(2))
+        dh = torch.zeros((n, l, c), dtype=x.dtype, device=x.device) if dh is None else _dense_channels(dh)
+        if dlast is not None:
+            dlast = dlast.contiguous()
+        dx = torch.empty((n, l, c), dtype=x.dtype, device=x.device)
+        dg = torch.empty_like(dx)
         dh0 = torch.empty((n, c), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
-        size = int(lib.unet_gated_scan_workspace_bytes(_dt(x), n, l, c))
-        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        with torch.cuda.device(x.device):
-            check(lib.unet_gated_scan_bwd(_dt(x), _p(x), x.stride(0), x.stride(1), _p(gate), gate.stride(0), gate.stride(1),
-                                          _p(states), _p(dh), dh.stride(0), dh.stride(1), _p(dlast), int(ctx.reverse), n, l, c,
-                                          _p(dx), _p(dg), _p(dh0), _p(ws), size, _stream_on(x)), "unet_gated_scan_bwd")
+        ws, size = _scan_workspace(x, n, l, c)
+        _run("unet_gated_scan_bwd", x, _dt(x), x, x.stride(0), x.stride(1), gate, gate.stride(0), gate.stride(1), states, dh,
+             dh.stride(0), dh.stride(1), dlast, ctx.reverse, n, l, c, dx, dg, dh0, ws, size)
         return dx, dg, dh0, None
 
 
@@ -1753,11 +1775,15 @@ def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor] = None, reverse: bo
         h = x * torch.sigmoid(gate)
         last = h0.clone() if h0 is not None else torch.zeros((x.shape[0], x.shape[2]), dtype=torch.float32, device=x.device)
     else:
-        h, last = GatedScanFn.apply(x, gate, h0, bool(reverse))
+        x, gate = _dense_channels(x), _dense_channels(gate)
+        h0 = None if h0 is None else h0.contiguous()
+        if _wants_grad(x, gate, h0):
+            h, last = GatedScanFn.apply(x, gate, h0, bool(reverse))
+        else:
+            h, last, _ = _scan_forward(x, gate, h0, bool(reverse), False)
     return (h, last) if return_state else h
 
 
-@torch.no_grad()
 def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
     """One row of ``gated_scan`` for every sequence: ``x``, ``gate`` ``[N, C]``; ``state`` ``[N, C]`` fp32 contiguous, moved on
     IN PLACE.  Returns the new state in ``x``'s dtype.  Inference only."""
@@ -1766,11 +1792,9 @@ def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
         raise ValueError("gated_scan_step: the state is updated in place and must be contiguous")
     n, c = x.shape
     h = torch.empty((n, c), dtype=x.dtype, device=x.device)
-    if x.numel():
+    if h.numel():
         x, gate = _dense_channels(x), _dense_channels(gate)
-        with torch.cuda.device(x.device):
-            check(_lib.load().unet_gated_scan_step(_dt(x), _p(x), x.stride(0), _p(gate), gate.stride(0), _p(state), _p(h), n, c,
-                                                   _stream_on(x)), "unet_gated_scan_step")
+        _run("unet_gated_scan_step", x, _dt(x), x, x.stride(0), gate, gate.stride(0), state, h, n, c)
     return h
 
 
@@ -1808,42 +1832,43 @@ def rel_bucket(offset: Tensor, n_buckets: int, max_distance: int) -> Tensor:
     return torch.bucketize(offset.abs(), starts, right=True) - 1 + (offset > 0) * (n_buckets // 2)
 
 
+@functools.lru_cache(maxsize=None)
+def _starts_array(starts: Tuple[int, ...]):
+    return (C.c_int32 * len(starts))(*starts)
+
+
+def _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, keep: bool):
+    n, l, c = q.shape
+    out = torch.empty_like(q)
+    lse = torch.empty((n, n_heads, l), dtype=torch.float32, device=q.device) if keep else None
+    _run("unet_rel_attn_fwd", q, _dt(q), q, k, v, table, _dt(table), table.shape[0], _starts_array(starts), lengths, n, l, c, n_heads,
+         scale, out, lse)
+    return out, lse
+
+
 class RelBiasAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, n_heads, scale, starts, lengths):
-        q, k, v, table = (t.detach().contiguous() for t in (q, k, v, table))
-        n, l, c = q.shape
-        keep = any(ctx.needs_input_grad[:4])
-        out = torch.empty_like(q)
-        lse = torch.empty((n, n_heads, l), dtype=torch.float32, device=q.device) if keep else None
-        arr = (C.c_int32 * len(starts))(*starts)
-        with torch.cuda.device(q.device):
-            check(_lib.load().unet_rel_attn_fwd(_dt(q), _p(q), _p(k), _p(v), _p(table), _dt(table), table.shape[0], arr, _p(lengths),
-                                                n, l, c, n_heads, scale, _p(out), _p(lse), _stream_on(q)), "unet_rel_attn_fwd")
-        if keep:
-            ctx.save_for_backward(q, k, v, table, out, lse, lengths)
+        out, lse = _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, True)
+        ctx.save_for_backward(q, k, v, table, out, lse, lengths)
         ctx.n_heads, ctx.scale, ctx.starts = n_heads, scale, starts
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _once_differentiable("rel_bias_attention")
         q, k, v, table, out, lse, lengths = ctx.saved_tensors
         n, l, c = q.shape
-        lib = _lib.load()
-        dout = dout.to(q.dtype).contiguous()
+        dout = dout.contiguous()
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         delta = torch.empty_like(lse)
         dtable = partials = None
         if ctx.needs_input_grad[3]:
             dtable = torch.empty_like(table)
-            partials = torch.empty(int(lib.unet_rel_attn_bwd_partials(_dt(q), n, l, ctx.n_heads, ctx.starts[-1])), dtype=torch.float32,
-                                   device=q.device)
-        arr = (C.c_int32 * len(ctx.starts))(*ctx.starts)
-        with torch.cuda.device(q.device):
-            check(lib.unet_rel_attn_bwd(_dt(q), _p(q), _p(k), _p(v), _p(table), _dt(table), table.shape[0], arr, _p(lengths), _p(out),
-                                        _p(lse), _p(dout), n, l, c, ctx.n_heads, ctx.scale, _p(dq), _p(dk), _p(dv), _p(dtable),
-                                        _p(partials), _p(delta), _stream_on(q)), "unet_rel_attn_bwd")
+            size = int(_lib.load().unet_rel_attn_bwd_partials(_dt(q), n, l, ctx.n_heads, ctx.starts[-1]))
+            partials = torch.empty(size, dtype=torch.float32, device=q.device)
+        _run("unet_rel_attn_bwd", q, _dt(q), q, k, v, table, _dt(table), table.shape[0], _starts_array(ctx.starts), lengths, out, lse,
+             dout, n, l, c, ctx.n_heads, ctx.scale, dq, dk, dv, dtable, partials, delta)
         return dq, dk, dv, dtable, None, None, None, None
 
 
@@ -1885,4 +1910,7 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
     _need_cuda(q)
     if q.numel() == 0:
         return q * k * v + 0 * table.sum().to(q.dtype)
-    return RelBiasAttnFn.apply(q, k, v, table, n_heads, scale, starts, lengths)
+    q, k, v, table = q.contiguous(), k.contiguous(), v.contiguous(), table.contiguous()
+    if _wants_grad(q, k, v, table):
+        return RelBiasAttnFn.apply(q, k, v, table, n_heads, scale, starts, lengths)
+    return _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, False)[0]

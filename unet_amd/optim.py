@@ -139,7 +139,8 @@ class _Group8:
         self.start4 = as_u32([b * (BLOCK // 4) for b in start])
         self.numel = as_u32([p.numel() for p in params])
         self.p_ptrs = torch.tensor([p.data_ptr() for p in params], dtype=torch.int64, device=dev)
-        self.ptr_key = tuple(p.data_ptr() for p in params)
+        self.ptrs = [p.data_ptr() for p in params]
+        self.device = dev.index
         zeros = lambda n, dt: torch.zeros(max(n, BLOCK), dtype=dt, device=dev)
         self.m8, self.r8 = (zeros(self.end8, torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
         self.m_scale, self.r_scale = (zeros(self.end8 // BLOCK, torch.float32) for _ in range(2))
@@ -151,17 +152,26 @@ class _Group8:
         self.lr_host = None
         lib = _lib.load()
         # sub-tables of at most OPT_MAX_TENSORS tensors: (first, count, blocks, first partial of the norm pass / of the step)
-        self.batches, n1, n2 = [], 0, 0
+        batches, n1, n2 = [], 0, 0
         for a in range(0, len(params), _lib.OPT_MAX_TENSORS):
             b = min(len(params), a + _lib.OPT_MAX_TENSORS)
             nb = start[b] - start[a]
             if nb == 0:
                 continue
-            self.batches.append((a, b - a, nb, n1, n2))
+            batches.append((a, b - a, nb, n1, n2))
             n1 += int(lib.unet_opt_blocks(nb * BLOCK))
             n2 += int(lib.unet_adamw8_blocks(nb))
         self.n_norm, self.n_step = n1, n2
         self.partial = torch.zeros(max(n1, n2, 1), dtype=torch.float32, device=dev)
+        # the fixed arguments of a batch's three calls (tables of 4-byte entries, but 8 bytes a pointer and a bias correction)
+        part, at = self.partial.data_ptr(), lambda t, a: t.data_ptr() + a * t.element_size()
+        self.calls = [(a, n,
+                       (at(self.start4, a), at(self.numel, a), nb * BLOCK, part + 4 * p1, at(self.step, a)),
+                       (at(self.step, a), at(self.bc, 2 * a)),
+                       (at(self.p_ptrs, a), at(self.start256, a), at(self.numel, a), at(self.slot, a), nb, self.m8.data_ptr(),
+                        self.r8.data_ptr(), self.m_scale.data_ptr(), self.r_scale.data_ptr(), self.m.data_ptr(), self.v.data_ptr(),
+                        self.coef.data_ptr(), at(self.bc, 2 * a)), part + 4 * p2)
+                      for a, n, nb, p1, p2 in batches]
         self.views = []
         for p, s, b in zip(params, slot, start):
             n = p.numel()
@@ -173,23 +183,39 @@ class _Group8:
                 self.views.append({"exp_avg": self.m8[a:a + n].view_as(p), "exp_avg_scale": self.m_scale[s:s + nb],
                                    "exp_avg_sq_root": self.r8[a:a + n].view_as(p), "exp_avg_sq_root_scale": self.r_scale[s:s + nb]})
 
-    def fill(self, i: int, st) -> None:
-        """Moments of tensor i from a loaded state in either form, or from an earlier table."""
-        view = self.views[i]
-        if "exp_avg" in st:
-            if "exp_avg_scale" in view and "exp_avg_scale" in st:          # codes stay the codes they are
-                new = {k: st[k].to(view[k].dtype) for k in view}
-            elif "exp_avg_scale" in view:
+    def fill(self, states) -> None:
+        """Moments and step counts from the tensors' loaded states, in either form, or from an earlier table's views."""
+        for names, flat, code in ((("exp_avg", "exp_avg_sq_root"), (self.m8, self.r8), True),
+                                  (("exp_avg_scale", "exp_avg_sq_root_scale"), (self.m_scale, self.r_scale), False)):
+            # the usual case, all of the large tensors held in codes already: one gather a buffer
+            group = [(st, v) for st, v in zip(states, self.views) if "exp_avg_scale" in v]
+            if group and all("exp_avg_scale" in st for st, _ in group):
+                for name, buf in zip(names, flat):
+                    parts = []
+                    for st, v in group:
+                        parts.append(st[name].reshape(-1).float())
+                        if code and v[name].numel() % BLOCK:
+                            parts.append(parts[-1].new_zeros(-v[name].numel() % BLOCK))
+                    buf[:self.end8 if code else self.end8 // BLOCK].copy_(torch.cat(parts))
+        for st, view in zip(states, self.views):
+            if "exp_avg" in st and not ("exp_avg_scale" in view and "exp_avg_scale" in st):
                 m, v = _load_moments(st)
-                new = dict(zip(("exp_avg", "exp_avg_scale"), quantise_moment(m, False)))
-                new.update(zip(("exp_avg_sq_root", "exp_avg_sq_root_scale"), quantise_moment(v.sqrt(), True)))
-            else:
-                new = dict(zip(("exp_avg", "exp_avg_sq"), _load_moments(st)))
-            for k in view:
-                view[k].copy_(new[k].reshape(view[k].shape))
-        for k in ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_root", "exp_avg_sq_root_scale"):
-            st.pop(k, None)
-        st.update(view)
+                if "exp_avg_scale" in view:
+                    new = quantise_moment(m, False) + quantise_moment(v.sqrt(), True)
+                    keys = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
+                else:
+                    new, keys = (m, v), ("exp_avg", "exp_avg_sq")
+                for k, t in zip(keys, new):
+                    view[k].copy_(t.reshape(view[k].shape))
+        steps = [st.get("step") for st in states]
+        on_device = [t for t in steps if isinstance(t, torch.Tensor) and t.is_cuda]
+        fetched = iter(torch.stack([t.float() for t in on_device]).tolist() if on_device else ())
+        self.step.copy_(torch.tensor([0.0 if t is None else next(fetched) if isinstance(t, torch.Tensor) and t.is_cuda else float(t)
+                                      for t in steps]))
+        for st, view, step in zip(states, self.views, self.step.unbind()):
+            for k in ("exp_avg", "exp_avg_scale", "exp_avg_sq", "exp_avg_sq_root", "exp_avg_sq_root_scale"):
+                st.pop(k, None)
+            st.update(view, step=step)
 
 
 class ClipAdamW(torch.optim.Optimizer):
@@ -216,25 +242,24 @@ class ClipAdamW(torch.optim.Optimizer):
                              f"and {group['min_8bit_numel']}")
 
     # -- tables -------------------------------------------------------------------------------
-    def _tables8(self, gi: int, params, min_numel: int) -> _Group8:
+    def _tables8(self, gi: int, group) -> Optional[_Group8]:
         g = self._groups.get(gi)
-        if g is None or g.ptr_key != tuple(p.data_ptr() for p in params):
-            g = _Group8(params, min_numel)
-            for i, p in enumerate(params):
-                st = self.state[p]
-                g.fill(i, st)
-                if st.get("step") is not None:
-                    g.step[i] = float(st["step"])
-                st["step"] = g.step[i]
+        ptrs = [p.data_ptr() for p in group["params"] if p.requires_grad]
+        if g is None or g.ptrs != ptrs:
+            params = [p for p in group["params"] if p.requires_grad]
+            if not params:
+                return None
+            g = _Group8(params, group["min_8bit_numel"])
+            g.fill([self.state[p] for p in params])
             self._groups[gi] = g
         return g
 
     def _tables(self, gi: int, group) -> _Group:
+        if group["state_bits"] == 8:
+            return self._tables8(gi, group)
         params = [p for p in group["params"] if p.requires_grad]
         if not params:
             return None
-        if group["state_bits"] == 8:
-            return self._tables8(gi, params, group["min_8bit_numel"])
         g = self._groups.get(gi)
         key = tuple(p.data_ptr() for p in params)
         if g is None or g.ptr_key != key:
@@ -286,7 +311,7 @@ class ClipAdamW(torch.optim.Optimizer):
         ``exp_avg_sq``, tensors padded to 4 elements.  ``state_bits=8``: those hold the tensors below ``min_8bit_numel``; the
         others are in ``exp_avg8`` / ``exp_avg_sq_root8`` (e4m3 codes, tensors padded to 256 elements) with one fp32 scale per
         256 codes in ``exp_avg8_scale`` / ``exp_avg_sq_root8_scale``."""
-        g = self._tables(group_index, self.param_groups[group_index])
+        g = self._groups.get(group_index) or self._tables(group_index, self.param_groups[group_index])
         if g is None:
             return {}
         if not isinstance(g, _Group8):
@@ -296,28 +321,24 @@ class ClipAdamW(torch.optim.Optimizer):
                 "exp_avg_sq_root8": g.r8[:g.end8], "exp_avg_sq_root8_scale": g.r_scale[:nb]}
 
     # -- step -----------------------------------------------------------------------------------
-    def _apply8(self, lib, st, g: _Group8, group, grads, max_norm: float, lr_ptr: int) -> None:
+    def _apply8(self, lib, g: _Group8, group, grads, max_norm: float, lr_ptr: int) -> None:
         """One step of an 8-bit group: norm first if it clips, otherwise the norm falls out of the step."""
+        st = torch._C._cuda_getCurrentRawStream(g.device)
         b1, b2 = (float(b) for b in group["betas"])
-        no_clip = not max_norm > 0.0
-        arrs = [(C.c_void_p * n)(*grads[a:a + n]) for a, n, _, _, _ in g.batches]
-        if not no_clip:
-            for (a, n, nb, p1, _), arr in zip(g.batches, arrs):
-                check(lib.unet_grad_sqnorm(arr, n, g.start4[a:].data_ptr(), g.numel[a:].data_ptr(), nb * BLOCK,
-                                           g.partial[p1:].data_ptr(), g.step[a:].data_ptr(), st), "unet_grad_sqnorm")
-        for (a, n, nb, _, p2), arr in zip(g.batches, arrs):
-            check(lib.unet_adamw8_prepare(arr, n, g.partial.data_ptr(), 0 if no_clip else g.n_norm, int(no_clip), max_norm, lr_ptr,
-                                          g.coef.data_ptr(), g.step[a:].data_ptr(), b1, b2, g.bc[a:].data_ptr(), st),
+        eps, decay = float(group["eps"]), float(group["weight_decay"])
+        clips, part, coef = max_norm > 0.0, g.partial.data_ptr(), g.coef.data_ptr()
+        arrs = [(C.c_void_p * c[1])(*grads[c[0]:c[0] + c[1]]) for c in g.calls]
+        if clips:
+            for (_, n, norm, _, _, _), arr in zip(g.calls, arrs):
+                check(lib.unet_grad_sqnorm(arr, n, *norm, st), "unet_grad_sqnorm")
+        for (_, n, _, prep, _, _), arr in zip(g.calls, arrs):
+            check(lib.unet_adamw8_prepare(arr, n, part, g.n_norm if clips else 0, int(not clips), max_norm, lr_ptr, coef, prep[0], b1,
+                                          b2, prep[1], st), "unet_adamw8_prepare")
+        for (_, n, _, _, table, p2), arr in zip(g.calls, arrs):
+            check(lib.unet_adamw8_apply(arr, n, *table, None if clips else p2, b1, b2, eps, decay, st), "unet_adamw8_apply")
+        if not clips:
+            check(lib.unet_adamw8_prepare(None, 0, part, g.n_step, 0, 0.0, lr_ptr, coef, None, b1, b2, None, st),
                   "unet_adamw8_prepare")
-        for (a, n, nb, _, p2), arr in zip(g.batches, arrs):
-            check(lib.unet_adamw8_apply(arr, n, g.p_ptrs[a:].data_ptr(), g.start256[a:].data_ptr(), g.numel[a:].data_ptr(),
-                                        g.slot[a:].data_ptr(), nb, g.m8.data_ptr(), g.r8.data_ptr(), g.m_scale.data_ptr(),
-                                        g.r_scale.data_ptr(), g.m.data_ptr(), g.v.data_ptr(), g.coef.data_ptr(),
-                                        g.bc[a:].data_ptr(), g.partial[p2:].data_ptr() if no_clip else 0, b1, b2,
-                                        float(group["eps"]), float(group["weight_decay"]), st), "unet_adamw8_apply")
-        if no_clip:
-            check(lib.unet_adamw8_prepare(None, 0, g.partial.data_ptr(), g.n_step, 0, 0.0, lr_ptr, g.coef.data_ptr(), None, b1, b2,
-                                          None, st), "unet_adamw8_prepare")
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -340,6 +361,19 @@ class ClipAdamW(torch.optim.Optimizer):
                     g.lr.fill_(lr)
                     g.lr_host = lr
                 lr_ptr = g.lr.data_ptr()
+            if isinstance(g, _Group8):
+                grads = [p.grad for p in g.params]
+                if not all(gr is None or (gr.dtype == torch.float32 and not gr.is_sparse and gr.is_contiguous()) for gr in grads):
+                    raise TypeError("ClipAdamW: gradients must be contiguous dense fp32 tensors")
+                ptrs = [None if gr is None else gr.data_ptr() for gr in grads]
+                if any(ptrs) and g.calls:
+                    max_norm = float(group.get("max_grad_norm") or 0.0)
+                    if g.device == torch._C._cuda_getDevice():
+                        self._apply8(lib, g, group, ptrs, max_norm, lr_ptr)
+                    else:
+                        with torch.cuda.device(g.device):
+                            self._apply8(lib, g, group, ptrs, max_norm, lr_ptr)
+                continue
             grads = []
             for p in g.params:
                 gr = p.grad
@@ -353,9 +387,6 @@ class ClipAdamW(torch.optim.Optimizer):
                 continue
             beta1, beta2 = group["betas"]
             max_norm = group.get("max_grad_norm") or 0.0
-            if isinstance(g, _Group8):
-                self._apply8(lib, st, g, group, grads, float(max_norm), lr_ptr)
-                continue
             arrs = []
             for a, n, flat, p0, blocks in g.batches:
                 arr = (C.c_void_p * n)(*grads[a:a + n])
