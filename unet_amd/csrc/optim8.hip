@@ -10,17 +10,17 @@
 //
 // HBM-bound: p, g and two codes read, p and two codes written = 16 bytes an element (the fp32 form: 28), plus 4 for the
 // norm's pass over g when a clip needs it first.  Without a clip the squares are summed while the step runs.
-// A wave owns a block of 256 elements, four a lane, so a block's maximum is one wave reduction; eight blocks a wave keep four
-// blocks' loads in flight.
+// A wave owns ONE block of 256 elements, four a lane, so a block's maximum is a wave reduction and the many short waves hide each
+// other's loads (with eight blocks a wave, four in flight, a model of 126 k parameters took 19 us instead of 5).  Parameters and
+// codes are not needed again before the next step: their accesses are non-temporal, which leaves the caches to the gradient,
+// read twice (at 42 M parameters the norm's pass 48 -> 32 us, this kernel 131 -> 113; at 446.6 M 335 -> 299 and 1363 -> 1203 us,
+// 6.0 TB/s).
 #include "common.h"
 
 namespace {
 
 constexpr int A8_THREADS = 256;
-// Blocks of 256 elements a wave: eight when they fill the chip (two workgroups a CU at least), otherwise one, so that a small
-// model's step is as short as one block's (126 k parameters: 17 workgroups took 19 us, 124 take 6).
-constexpr int A8_WAVES = A8_THREADS / 64, A8_MANY = 8;
-int per_wave(long long blocks256) { return blocks256 >= 512ll * A8_MANY * A8_WAVES ? A8_MANY : 1; }
+constexpr int A8_WAVES = A8_THREADS / 64;                          // blocks of 256 elements a workgroup
 constexpr unsigned A8_WIDE = 0x80000000u;                        // slot flag: 32-bit moments
 constexpr float A8_MAX = 448.f, A8_LEAST = 0.001953125f;         // largest and smallest positive e4m3 value
 constexpr float A8_TINY = 7.888609052210118e-31f;                // 2^-100
@@ -91,114 +91,81 @@ __device__ __forceinline__ int find_tensor(const unsigned* start, int n, unsigne
   return lo;
 }
 
-template <int A8_PER_WAVE>
 __global__ __launch_bounds__(A8_THREADS) void adamw8_apply_kernel(const Adam8 k, const GradPtrs gp) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned end = k.start[k.n];
-  const unsigned b0 = k.start[0] + (blockIdx.x * A8_WAVES + wave) * A8_PER_WAVE;
-  const unsigned b1 = b0 + A8_PER_WAVE < end ? b0 + A8_PER_WAVE : end;
-  const float clip = k.coef[0], keep = 1.f - k.coef[4] * k.weight_decay;
+  const unsigned b = k.start[0] + blockIdx.x * A8_WAVES + wave;
   float sq = 0.f;
-  if (b0 < b1) {
-    int t = find_tensor(k.start, k.n, b0);
-    const float* g0 = gp.g[t];
-    float* p0 = k.p[t];
-    unsigned slot = k.slot[t];
-    const unsigned off = b0 - k.start[t];
-    if (b1 - b0 == A8_PER_WAVE && (off + A8_PER_WAVE) * 256u <= k.numel[t] && !(slot & A8_WIDE) &&
-        !((reinterpret_cast<uintptr_t>(g0) | reinterpret_cast<uintptr_t>(p0)) & 15)) {
-      // the usual case: eight whole blocks of one tensor
-      if (g0) {
-        const float2 bc = k.bc[t];
-        constexpr int Q = A8_PER_WAVE < 4 ? A8_PER_WAVE : 4;
+  const int t = b < k.start[k.n] ? find_tensor(k.start, k.n, b) : -1;
+  const float* gt = t >= 0 ? gp.g[t] : nullptr;
+  if (gt) {                                           // no gradient this step: the tensor and its moments stay as they are
+    const float clip = k.coef[0], keep = 1.f - k.coef[4] * k.weight_decay;
+    float* pt = k.p[t];
+    const unsigned slot = k.slot[t], ne = k.numel[t], bo = b - k.start[t], i = bo * 256u + lane * 4;
+    const float2 bc = k.bc[t];
+    float g[4] = {0.f, 0.f, 0.f, 0.f}, p[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool whole = (bo + 1) * 256u <= ne && !((reinterpret_cast<uintptr_t>(gt) | reinterpret_cast<uintptr_t>(pt)) & 15);
+    const int cnt = i >= ne ? 0 : (ne - i < 4 ? (int)(ne - i) : 4);
+    const bool wide = slot & A8_WIDE;
+    const size_t cb = (size_t)slot + bo;
+    unsigned* const mc = reinterpret_cast<unsigned*>(k.m8 + cb * 256 + lane * 4);
+    unsigned* const rc = reinterpret_cast<unsigned*>(k.r8 + cb * 256 + lane * 4);
+    unsigned mw = 0, rw = 0;
+    float ms = 0.f, rs = 0.f;
+    if (!wide) {
+      mw = __builtin_nontemporal_load(mc);
+      rw = __builtin_nontemporal_load(rc);
+      ms = k.sm[cb];
+      rs = k.sr[cb];
+    }
+    if (whole) {
+      const f32x4 gv = *reinterpret_cast<const f32x4*>(gt + i);
+      const f32x4 pv = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(pt + i));
 #pragma unroll
-        for (int h = 0; h < A8_PER_WAVE / Q; ++h) {
-          f32x4 gv[Q], pv[Q];
-          unsigned mc[Q], rc[Q];
-          float ms[Q], rs[Q];
-          const size_t e0 = (size_t)(off + h * Q) * 256 + lane * 4, c0 = (size_t)(slot + off + h * Q);
-#pragma unroll
-          for (int u = 0; u < Q; ++u) {
-            gv[u] = *reinterpret_cast<const f32x4*>(g0 + e0 + u * 256);
-            pv[u] = *reinterpret_cast<const f32x4*>(p0 + e0 + u * 256);
-            mc[u] = *reinterpret_cast<const unsigned*>(k.m8 + (c0 + u) * 256 + lane * 4);
-            rc[u] = *reinterpret_cast<const unsigned*>(k.r8 + (c0 + u) * 256 + lane * 4);
-            ms[u] = k.sm[c0 + u];
-            rs[u] = k.sr[c0 + u];
-          }
-#pragma unroll
-          for (int u = 0; u < Q; ++u) {
-            float m[4], r[4];
-            decode(mc[u], ms[u], m);
-            decode(rc[u], rs[u], r);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              sq = fmaf(gv[u][e], gv[u][e], sq);
-              moments(gv[u][e] * clip, m[e], r[e], k);
-              float pe = pv[u][e];
-              move(pe, m[e], r[e], keep, bc, k.eps);
-              pv[u][e] = pe;
-            }
-            float s1, s2;
-            const unsigned w1 = store_block<false>(m, s1), w2 = store_block<true>(r, s2);
-            *reinterpret_cast<f32x4*>(p0 + e0 + u * 256) = pv[u];
-            *reinterpret_cast<unsigned*>(k.m8 + (c0 + u) * 256 + lane * 4) = w1;
-            *reinterpret_cast<unsigned*>(k.r8 + (c0 + u) * 256 + lane * 4) = w2;
-            if (lane == 0) { k.sm[c0 + u] = s1; k.sr[c0 + u] = s2; }
-          }
-        }
-      }
+      for (int e = 0; e < 4; ++e) { g[e] = gv[e]; p[e] = pv[e]; }
     } else {
-      for (unsigned b = b0; b < b1; ++b) {
-        while (b >= k.start[t + 1]) ++t;
-        const float* gt = gp.g[t];
-        if (!gt) continue;                          // no gradient this step: the tensor and its moments stay as they are
-        float* pt = k.p[t];
-        slot = k.slot[t];
-        const unsigned ne = k.numel[t], bo = b - k.start[t], i = bo * 256u + lane * 4;
-        const float2 bc = k.bc[t];
-        const int cnt = i >= ne ? 0 : (ne - i < 4 ? (int)(ne - i) : 4);
-        float g[4] = {0.f, 0.f, 0.f, 0.f}, p[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < cnt) { g[e] = gt[(size_t)i + e]; p[e] = pt[(size_t)i + e]; sq = fmaf(g[e], g[e], sq); }
-        if (slot & A8_WIDE) {
-          const size_t at = (size_t)(slot & ~A8_WIDE) * 4 + i;
+      for (int e = 0; e < 4; ++e)
+        if (e < cnt) { g[e] = gt[(size_t)i + e]; p[e] = pt[(size_t)i + e]; }
+    }
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < cnt) {
-              const float gc = g[e] * clip;
-              const float m1 = k.beta1 * k.m32[at + e] + k.grow1 * gc;
-              const float v1 = k.beta2 * k.v32[at + e] + k.grow2 * gc * gc;
-              k.m32[at + e] = m1;
-              k.v32[at + e] = v1;
-              move(p[e], m1, sqrtf(v1), keep, bc, k.eps);
-            }
-        } else {
-          const size_t cb = (size_t)slot + bo;
-          decode(*reinterpret_cast<const unsigned*>(k.m8 + cb * 256 + lane * 4), k.sm[cb], m);
-          decode(*reinterpret_cast<const unsigned*>(k.r8 + cb * 256 + lane * 4), k.sr[cb], r);
+    for (int e = 0; e < 4; ++e) sq = fmaf(g[e], g[e], sq);
+    if (wide) {
+      const size_t at = (size_t)(slot & ~A8_WIDE) * 4 + i;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (e < cnt) {
-              moments(g[e] * clip, m[e], r[e], k);
-              move(p[e], m[e], r[e], keep, bc, k.eps);
-            } else m[e] = r[e] = 0.f;
-          }
-          float s1, s2;
-          const unsigned w1 = store_block<false>(m, s1), w2 = store_block<true>(r, s2);
-          *reinterpret_cast<unsigned*>(k.m8 + cb * 256 + lane * 4) = w1;
-          *reinterpret_cast<unsigned*>(k.r8 + cb * 256 + lane * 4) = w2;
-          if (lane == 0) { k.sm[cb] = s1; k.sr[cb] = s2; }
+      for (int e = 0; e < 4; ++e)
+        if (e < cnt) {
+          const float gc = g[e] * clip;
+          const float m1 = k.beta1 * k.m32[at + e] + k.grow1 * gc;
+          const float v1 = k.beta2 * k.v32[at + e] + k.grow2 * gc * gc;
+          k.m32[at + e] = m1;
+          k.v32[at + e] = v1;
+          move(p[e], m1, sqrtf(v1), keep, bc, k.eps);
         }
+    } else {
+      decode(mw, ms, m);
+      decode(rw, rs, r);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (e < cnt) pt[(size_t)i + e] = p[e];
+      for (int e = 0; e < 4; ++e) {
+        if (e < cnt) {
+          moments(g[e] * clip, m[e], r[e], k);
+          move(p[e], m[e], r[e], keep, bc, k.eps);
+        } else m[e] = r[e] = 0.f;
       }
+      float s1, s2;
+      __builtin_nontemporal_store(store_block<false>(m, s1), mc);
+      __builtin_nontemporal_store(store_block<true>(r, s2), rc);
+      if (lane == 0) { k.sm[cb] = s1; k.sr[cb] = s2; }
+    }
+    if (whole) {
+      __builtin_nontemporal_store(f32x4{p[0], p[1], p[2], p[3]}, reinterpret_cast<f32x4*>(pt + i));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < cnt) pt[(size_t)i + e] = p[e];
     }
   }
   if (k.partial) {
-    __shared__ float red[A8_THREADS / 64];
+    __shared__ float red[A8_WAVES];
     sq = wave_sum(sq);
     if (lane == 0) red[wave] = sq;
     __syncthreads();
@@ -251,10 +218,7 @@ __global__ __launch_bounds__(PREP_THREADS) void adamw8_prepare_kernel(const Grad
 
 }  // namespace
 
-extern "C" int32_t unet_adamw8_blocks(int64_t blocks256) {
-  const int per = per_wave(blocks256) * A8_WAVES;
-  return (int32_t)((blocks256 + per - 1) / per);
-}
+extern "C" int32_t unet_adamw8_blocks(int64_t blocks256) { return (int32_t)((blocks256 + A8_WAVES - 1) / A8_WAVES); }
 
 extern "C" int unet_adamw8_prepare(const float* const* grads_host, int32_t n_tensors, const float* partial, int32_t n_partial,
                                    int32_t advance, float max_norm, const float* lr, float* coef, float* step_t, double beta1,
@@ -292,9 +256,8 @@ extern "C" int unet_adamw8_apply(const float* const* grads_host, int32_t n_tenso
   k.eps = eps; k.weight_decay = weight_decay; k.n = n_tensors;
   GradPtrs gp;
   for (int i = 0; i < UNET_OPT_MAX_TENSORS; ++i) gp.g[i] = i < n_tensors ? grads_host[i] : nullptr;
-  const dim3 grid(unet_adamw8_blocks(blocks256));
-  if (per_wave(blocks256) == 1) hipLaunchKernelGGL(adamw8_apply_kernel<1>, grid, dim3(A8_THREADS), 0, static_cast<hipStream_t>(stream), k, gp);
-  else hipLaunchKernelGGL(adamw8_apply_kernel<A8_MANY>, grid, dim3(A8_THREADS), 0, static_cast<hipStream_t>(stream), k, gp);
+  hipLaunchKernelGGL(adamw8_apply_kernel, dim3(unet_adamw8_blocks(blocks256)), dim3(A8_THREADS), 0, static_cast<hipStream_t>(stream),
+                     k, gp);
   UNET_LAUNCH_CHECK("adamw8_apply");
   return 0;
 }
