@@ -15,6 +15,11 @@
 // Few windows with many rows cannot fill 256 CUs that way.  Their rows are split into segments: a first launch reduces each
 // segment to its pair (reads two of the inputs a second time), and a segment's workgroup composes the pairs in front of it.
 //
+// HBM-bound.  Inputs and outputs are touched once and are larger than the caches where it matters: their accesses are
+// non-temporal (forward at [64, 1024, 1024] bf16 83 -> 71 us, and a kernel that reads h afterwards does not lose it).  Measured
+// there: forward 71 us (403 MB, 5.7 TB/s), backward 123 us (671 MB, 5.5 TB/s); [1, 75000, 1024] forward 134 us, of which the
+// segment launch takes 55 (461 + 307 MB).
+//
 // Everything between loads and stores is fp32.  sigmoid: with t = exp(-|g|), small = t / (1 + t), big = 1 - small; both sides
 // keep full relative precision where 1 - f would cancel.
 #include "common.h"
@@ -23,6 +28,7 @@ namespace {
 
 constexpr int SC_THREADS = 512;
 constexpr int SC_TILE = 64;      // rows of a tile, and the distance of the kept states
+constexpr int NT = 2;            // buffer accesses: non-temporal
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct ScanK {
@@ -36,41 +42,25 @@ struct ScanK {
   int n, l, c, tiles, segs, seg_tiles, ncb, reverse;
 };
 
-// V consecutive values of a row
+// V consecutive values of a row: one fp32 or bf16, or two bf16
 template <typename T, int V> struct Raw;
 template <> struct Raw<float, 1> { typedef float type; };
-template <> struct Raw<float, 2> { typedef f32x2 type; };
 template <> struct Raw<__bf16, 1> { typedef unsigned short type; };
 template <> struct Raw<__bf16, 2> { typedef unsigned int type; };
-template <> struct Raw<__bf16, 4> { typedef u32x2 type; };
 
 template <typename T, int V> __device__ __forceinline__ void unpack(const typename Raw<T, V>::type& r, float (&f)[V]) {
-  if constexpr (std::is_same<T, float>::value) {
-    if constexpr (V == 1) f[0] = r;
-    else { f[0] = r[0]; f[1] = r[1]; }
-  } else {
-    if constexpr (V == 1) f[0] = __builtin_bit_cast(float, (unsigned)r << 16);
-    else if constexpr (V == 2) {
-      f[0] = __builtin_bit_cast(float, r << 16);
-      f[1] = __builtin_bit_cast(float, r & 0xffff0000u);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        f[2 * i] = __builtin_bit_cast(float, r[i] << 16);
-        f[2 * i + 1] = __builtin_bit_cast(float, r[i] & 0xffff0000u);
-      }
-    }
+  if constexpr (std::is_same<T, float>::value) f[0] = r;
+  else {
+    f[0] = __builtin_bit_cast(float, (unsigned)r << 16);
+    if constexpr (V == 2) f[1] = __builtin_bit_cast(float, r & 0xffff0000u);
   }
 }
-template <typename T, int V> __device__ __forceinline__ void put(T* p, const float (&f)[V]) {
+template <typename T, int V> __device__ __forceinline__ typename Raw<T, V>::type pack(const float (&f)[V]) {
   typedef __attribute__((ext_vector_type(V))) T vec;
-  if constexpr (V == 1) *p = (T)f[0];
-  else {
-    vec v;
+  vec v;
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (T)f[i];
-    *reinterpret_cast<vec*>(p) = v;
-  }
+  for (int i = 0; i < V; ++i) v[i] = (T)f[i];
+  return __builtin_bit_cast(typename Raw<T, V>::type, v);
 }
 
 __device__ __forceinline__ void gate(float g, float& f, float& keep) {     // f = sigmoid(g), keep = 1 - f
@@ -79,44 +69,104 @@ __device__ __forceinline__ void gate(float g, float& f, float& keep) {     // f 
   const float big = 1.f - small;
   f = g >= 0.f ? big : small;
   keep = g >= 0.f ? small : big;
-  if (g != g) f = keep = g;
 }
 
-// one thread's rows of a tile: raw values, loaded a tile ahead
+// One tensor [l][ld] of a window, as a thread walks it: R rows at `row` (a multiple of R inside the tile) of V channels.  Whole
+// tiles go through buffer instructions: the tile's base and the rows' offsets are scalars, a lane holds one 32-bit offset.
 template <typename T, int V, int R> struct Rows {
   typedef typename Raw<T, V>::type raw;
-  raw r[R];
-  // rows t0 .. t0+R-1 (walk order); rows at or past l are not read
-  __device__ __forceinline__ void load(const T* base, long long ld, int t0, int l, int reverse) {
-    if (t0 + R <= l) {
-      const T* p = base + (long long)(reverse ? l - 1 - t0 : t0) * ld;
-      const long long step = reverse ? -ld : ld;
+  const T* base;                  // the window's row 0, channel 0 (uniform)
+  long long ld;
+  int l, reverse, c;
+  unsigned voff;
+  __device__ __forceinline__ void init(const void* window, long long ld_, int l_, int reverse_, int row, int c_) {
+    base = static_cast<const T*>(window);
+    ld = ld_; l = l_; reverse = reverse_; c = c_;
+    voff = (unsigned)(((reverse ? SC_TILE - R - row : row) * ld + c) * sizeof(T));
+  }
+  __device__ __forceinline__ auto rsrc(int tile) const {
+    const int lo = reverse ? l - (tile + 1) * SC_TILE : tile * SC_TILE;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(base + lo * ld), 0, 0x80000000u, 0x00020000);
+  }
+  __device__ __forceinline__ int soff(int i) const { return (int)((reverse ? R - 1 - i : i) * ld * sizeof(T)); }
+  __device__ __forceinline__ void load(raw (&r)[R], int tile) const {
+    const auto d = rsrc(tile);
 #pragma unroll
-      for (int i = 0; i < R; ++i) r[i] = *reinterpret_cast<const raw*>(p + i * step);
-    } else {
+    for (int i = 0; i < R; ++i) {
+      if constexpr (sizeof(raw) == 2) r[i] = (raw)__builtin_amdgcn_raw_buffer_load_b16(d, voff, soff(i), NT);
+      else r[i] = __builtin_bit_cast(raw, __builtin_amdgcn_raw_buffer_load_b32(d, voff, soff(i), NT));
+    }
+  }
+  __device__ __forceinline__ const T* at(int t) const { return base + (long long)(reverse ? l - 1 - t : t) * ld + c; }
+  // rows t .. t+R-1 of a tile that the window's end cuts: rows at or past l read as zero
+  __device__ __forceinline__ void load_cut(raw (&r)[R], int t) const {
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        r[i] = raw{};
-        if (t0 + i < l) r[i] = *reinterpret_cast<const raw*>(base + (long long)(reverse ? l - 1 - t0 - i : t0 + i) * ld);
-      }
+    for (int i = 0; i < R; ++i) {
+      r[i] = raw{};
+      if (t + i < l) r[i] = *reinterpret_cast<const raw*>(at(t + i));
+    }
+  }
+  __device__ __forceinline__ void store(int tile, int i, const float (&f)[V]) const {
+    const raw w = pack<T, V>(f);
+    const auto d = rsrc(tile);
+    if constexpr (sizeof(raw) == 2) __builtin_amdgcn_raw_buffer_store_b16(w, d, voff, soff(i), NT);
+    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, w), d, voff, soff(i), NT);
+  }
+  __device__ __forceinline__ void store_cut(int t, const float (&f)[V]) const {
+    if (t < l) *reinterpret_cast<raw*>(const_cast<T*>(at(t))) = pack<T, V>(f);
+  }
+};
+
+// R rows anywhere, by their addresses
+template <typename T, int V, int R> struct Walk {
+  typename Raw<T, V>::type r[R];
+  const T* p;
+  long long step;
+  __device__ __forceinline__ void start(const T* base, long long ld, int t0, int l, int reverse) {
+    step = reverse ? -ld : ld;
+    p = base + (long long)(reverse ? l - 1 : 0) * ld + (long long)t0 * step;
+  }
+  __device__ __forceinline__ void load() {
+#pragma unroll
+    for (int i = 0; i < R; ++i) r[i] = *reinterpret_cast<const typename Raw<T, V>::type*>(p + i * step);
+  }
+  __device__ __forceinline__ void load(int rows) {         // the first `rows` of them; the others read as zero
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      r[i] = typename Raw<T, V>::type{};
+      if (i < rows) r[i] = *reinterpret_cast<const typename Raw<T, V>::type*>(p + i * step);
     }
   }
 };
 
-// start value of segment `seg`: the pairs of the segments before it (walk order DIR) applied to `s`
-template <int V, int DIR>
-__device__ __forceinline__ void compose(const ScanK& p, int n, int c, int seg, bool ok, float (&s)[V]) {
-  if (!p.agg || !ok) return;
-  const float2* a = p.agg + (long long)n * p.segs * p.c + c;
-  if (DIR > 0) {
-    for (int k = 0; k < seg; ++k)
+// Start value of segment `seg`: the pairs of the segments before it (walk order DIR) applied to `s`.  Each group composes a
+// contiguous share of them, the groups' pairs meet in LDS (`a`, `b`, free again after the call).
+template <int V, int CL, int DIR>
+__device__ __forceinline__ void compose(const ScanK& p, int n, int c, int seg, int grp, float (*a)[CL * V], float (*b)[CL * V], float (&s)[V]) {
+  constexpr int G = SC_THREADS / CL;
+  if (!p.agg) return;                              // uniform
+  const int cl = threadIdx.x % CL, before = DIR > 0 ? seg : p.segs - 1 - seg, share = (before + G - 1) / G;
+  const int lo = min(before, grp * share), hi = min(before, lo + share);
+  const float2* q = p.agg + ((long long)n * p.segs + (DIR > 0 ? 0 : p.segs - 1)) * p.c + c;       // k-th pair in walk order: q[DIR * k * c]
+  float A[V], B[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) { const float2 ab = a[(long long)k * p.c + v]; s[v] = fmaf(ab.x, s[v], ab.y); }
-  } else {
-    for (int k = p.segs - 1; k > seg; --k)
+  for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
+#pragma unroll 4
+  for (int k = lo; k < hi; ++k)
 #pragma unroll
-      for (int v = 0; v < V; ++v) { const float2 ab = a[(long long)k * p.c + v]; s[v] = fmaf(ab.x, s[v], ab.y); }
-  }
+    for (int v = 0; v < V; ++v) {
+      const float2 ab = q[(long long)DIR * k * p.c + v];
+      A[v] *= ab.x;
+      B[v] = fmaf(ab.x, B[v], ab.y);
+    }
+#pragma unroll
+  for (int v = 0; v < V; ++v) { a[grp][cl * V + v] = A[v]; b[grp][cl * V + v] = B[v]; }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < G; ++k)
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = fmaf(a[k][cl * V + v], s[v], b[k][cl * V + v]);
+  __syncthreads();
 }
 
 template <typename T, int V, int CL>
@@ -128,43 +178,42 @@ __global__ __launch_bounds__(SC_THREADS) void scan_fwd_kernel(const ScanK p) {
   const int seg = blockIdx.y;
   const bool ok = c < p.c;                         // c % V == 0 and p.c % V == 0: a thread's channels are all in or all out
   const int cc = ok ? c : 0;
-  const T* x = static_cast<const T*>(p.x) + n * p.x_ns + cc;
-  const T* g = static_cast<const T*>(p.g) + n * p.g_ns + cc;
-  T* h = static_cast<T*>(p.h) + (long long)n * p.l * p.c + cc;
-
+  const int first = seg * p.seg_tiles, end = min(p.tiles, first + p.seg_tiles);
+  const int full = min(end, p.l / SC_TILE);        // tiles whose rows all exist
+  Rows<T, V, R> rx, rg, rh;
+  rx.init(static_cast<const T*>(p.x) + n * p.x_ns, p.x_ld, p.l, p.reverse, grp * R, cc);
+  rg.init(static_cast<const T*>(p.g) + n * p.g_ns, p.g_ld, p.l, p.reverse, grp * R, cc);
+  rh.init(static_cast<const T*>(p.h) + (long long)n * p.l * p.c, p.c, p.l, p.reverse, grp * R, cc);
+  typename Rows<T, V, R>::raw qx[R], qg[R];
+  if (first < full) { rx.load(qx, first); rg.load(qg, first); }
   float s[V];                                      // state in front of the tile (the same in every group)
 #pragma unroll
   for (int v = 0; v < V; ++v) s[v] = p.h0 ? p.h0[(long long)n * p.c + cc + v] : 0.f;
-  compose<V, 1>(p, n, cc, seg, ok, s);
+  compose<V, CL, 1>(p, n, cc, seg, grp, sa[0], sb[0], s);
 
-  const int first = seg * p.seg_tiles, end = min(p.tiles, first + p.seg_tiles);
-  Rows<T, V, R> rx, rg;
-  rx.load(x, p.x_ld, first * SC_TILE + grp * R, p.l, p.reverse);
-  rg.load(g, p.g_ld, first * SC_TILE + grp * R, p.l, p.reverse);
-  for (int tile = first; tile < end; ++tile) {
-    const int t0 = tile * SC_TILE + grp * R, buf = tile & 1;
+  auto work = [&](int tile, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    const int buf = tile & 1, t0 = tile * SC_TILE + grp * R;
     float f[R][V], b[R][V], A[V], B[V];
+    if (!WHOLE) { rx.load_cut(qx, t0); rg.load_cut(qg, t0); }
 #pragma unroll
     for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float xv[V], gv[V];
-      unpack<T, V>(rx.r[i], xv);
-      unpack<T, V>(rg.r[i], gv);
+      unpack<T, V>(qx[i], xv);
+      unpack<T, V>(qg[i], gv);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float keep;
         gate(gv[v], f[i][v], keep);
         b[i][v] = keep * xv[v];
-        if (t0 + i >= p.l) { f[i][v] = 1.f; b[i][v] = 0.f; }
+        if (!WHOLE && t0 + i >= p.l) { f[i][v] = 1.f; b[i][v] = 0.f; }
         A[v] *= f[i][v];
         B[v] = fmaf(f[i][v], B[v], b[i][v]);
       }
     }
-    if (tile + 1 < end) {
-      rx.load(x, p.x_ld, t0 + SC_TILE, p.l, p.reverse);
-      rg.load(g, p.g_ld, t0 + SC_TILE, p.l, p.reverse);
-    }
+    if (WHOLE && tile + 1 < full) { rx.load(qx, tile + 1); rg.load(qg, tile + 1); }
 #pragma unroll
     for (int v = 0; v < V; ++v) { sa[buf][grp][cl * V + v] = A[v]; sb[buf][grp][cl * V + v] = B[v]; }
     if (p.states && grp == 0 && ok) {
@@ -183,13 +232,18 @@ __global__ __launch_bounds__(SC_THREADS) void scan_fwd_kernel(const ScanK p) {
         if (k == grp) mine[v] = s[v];
         s[v] = fmaf(sa[buf][k][cl * V + v], s[v], sb[buf][k][cl * V + v]);
       }
+    if (ok) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
+      for (int i = 0; i < R; ++i) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) mine[v] = fmaf(f[i][v], mine[v], b[i][v]);
-      if (ok && t0 + i < p.l) put<T, V>(h + (long long)(p.reverse ? p.l - 1 - t0 - i : t0 + i) * p.c, mine);
+        for (int v = 0; v < V; ++v) mine[v] = fmaf(f[i][v], mine[v], b[i][v]);
+        if (WHOLE) rh.store(tile, i, mine);
+        else rh.store_cut(t0 + i, mine);
+      }
     }
-  }
+  };
+  for (int tile = first; tile < full; ++tile) work(tile, std::true_type{});
+  if (full < end) work(full, std::false_type{});
   if (p.last && seg == p.segs - 1 && grp == 0 && ok) {
 #pragma unroll
     for (int v = 0; v < V; ++v) p.last[(long long)n * p.c + c + v] = s[v];
@@ -197,7 +251,7 @@ __global__ __launch_bounds__(SC_THREADS) void scan_fwd_kernel(const ScanK p) {
 }
 
 template <typename T, int V, int CL>
-__global__ __launch_bounds__(SC_THREADS) void scan_bwd_kernel(const ScanK p) {
+__global__ __launch_bounds__(SC_THREADS, 2) void scan_bwd_kernel(const ScanK p) {
   constexpr int G = SC_THREADS / CL, R = SC_TILE / G;
   __shared__ float sa[2][G][CL * V], sb[2][G][CL * V], sm[2][G][CL * V];
   const int cl = threadIdx.x % CL, grp = threadIdx.x / CL;
@@ -205,45 +259,49 @@ __global__ __launch_bounds__(SC_THREADS) void scan_bwd_kernel(const ScanK p) {
   const int seg = blockIdx.y;
   const bool ok = c < p.c;
   const int cc = ok ? c : 0;
-  const T* x = static_cast<const T*>(p.x) + n * p.x_ns + cc;
-  const T* g = static_cast<const T*>(p.g) + n * p.g_ns + cc;
-  const T* dh = static_cast<const T*>(p.dh) + n * p.dh_ns + cc;
-  T* dx = static_cast<T*>(p.dx) + (long long)n * p.l * p.c + cc;
-  T* dg = static_cast<T*>(p.dg) + (long long)n * p.l * p.c + cc;
-  const float* st = p.states + (long long)n * p.tiles * p.c + cc;
-
-  float mu[V];                                     // f lam of the row behind the tile
-#pragma unroll
-  for (int v = 0; v < V; ++v) mu[v] = p.dlast ? p.dlast[(long long)n * p.c + cc + v] : 0.f;
-  compose<V, -1>(p, n, cc, seg, ok, mu);
-
   const int first = seg * p.seg_tiles, end = min(p.tiles, first + p.seg_tiles);
-  Rows<T, V, R> rx, rg, rd;
+  Rows<T, V, R> rx, rg, rd, ox_, og_;
+  rx.init(static_cast<const T*>(p.x) + n * p.x_ns, p.x_ld, p.l, p.reverse, grp * R, cc);
+  rg.init(static_cast<const T*>(p.g) + n * p.g_ns, p.g_ld, p.l, p.reverse, grp * R, cc);
+  rd.init(static_cast<const T*>(p.dh) + n * p.dh_ns, p.dh_ld, p.l, p.reverse, grp * R, cc);
+  ox_.init(static_cast<const T*>(p.dx) + (long long)n * p.l * p.c, p.c, p.l, p.reverse, grp * R, cc);
+  og_.init(static_cast<const T*>(p.dg) + (long long)n * p.l * p.c, p.c, p.l, p.reverse, grp * R, cc);
+  const float* st = p.states + (long long)n * p.tiles * p.c + cc;
+  typename Rows<T, V, R>::raw qx[R], qg[R], qd[R];
   float s0[V];
   auto load = [&](int tile) {
-    const int t0 = tile * SC_TILE + grp * R;
-    rx.load(x, p.x_ld, t0, p.l, p.reverse);
-    rg.load(g, p.g_ld, t0, p.l, p.reverse);
-    rd.load(dh, p.dh_ld, t0, p.l, p.reverse);
+    rx.load(qx, tile); rg.load(qg, tile); rd.load(qd, tile);
 #pragma unroll
     for (int v = 0; v < V; ++v) s0[v] = st[(long long)tile * p.c + v];
   };
-  load(end - 1);
-  for (int tile = end - 1; tile >= first; --tile) {
-    const int t0 = tile * SC_TILE + grp * R, buf = tile & 1;
+  const bool cut = end * SC_TILE > p.l;            // the segment's last tile is not whole
+  if (!cut) load(end - 1);
+  float mu[V];                                     // f lam of the row behind the tile
+#pragma unroll
+  for (int v = 0; v < V; ++v) mu[v] = p.dlast ? p.dlast[(long long)n * p.c + cc + v] : 0.f;
+  compose<V, CL, -1>(p, n, cc, seg, grp, sa[0], sb[0], mu);
+
+  auto work = [&](int tile, auto whole) {
+    constexpr bool WHOLE = decltype(whole)::value;
+    const int buf = tile & 1, t0 = tile * SC_TILE + grp * R;
     float f[R][V], keep[R][V], xv[R][V], d[R][V], A[V], B[V], M[V], s[V];
+    if (!WHOLE) {
+      rx.load_cut(qx, t0); rg.load_cut(qg, t0); rd.load_cut(qd, t0);
+#pragma unroll
+      for (int v = 0; v < V; ++v) s0[v] = st[(long long)tile * p.c + v];
+    }
 #pragma unroll
     for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; M[v] = 0.f; s[v] = s0[v]; }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float gv[V];
-      unpack<T, V>(rx.r[i], xv[i]);
-      unpack<T, V>(rg.r[i], gv);
-      unpack<T, V>(rd.r[i], d[i]);
+      unpack<T, V>(qx[i], xv[i]);
+      unpack<T, V>(qg[i], gv);
+      unpack<T, V>(qd[i], d[i]);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         gate(gv[v], f[i][v], keep[i][v]);
-        if (t0 + i >= p.l) { f[i][v] = 1.f; keep[i][v] = 0.f; }          // (x and dh read as zero there)
+        if (!WHOLE && t0 + i >= p.l) { f[i][v] = 1.f; keep[i][v] = 0.f; }          // (x and dh read as zero there)
         A[v] *= f[i][v];
         B[v] = fmaf(f[i][v], B[v], keep[i][v] * xv[i][v]);
       }
@@ -260,14 +318,15 @@ __global__ __launch_bounds__(SC_THREADS) void scan_bwd_kernel(const ScanK p) {
       sm[buf][grp][cl * V + v] = M[v];
     }
     __syncthreads();
-    float m[V];
+    float m[V], run[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) m[v] = mu[v];
+    for (int v = 0; v < V; ++v) { m[v] = mu[v]; run[v] = s[v]; }
 #pragma unroll
-    for (int k = 0; k < G; ++k)
+    for (int k = 0; k < G - 1; ++k)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (k < grp) s[v] = fmaf(sa[buf][k][cl * V + v], s[v], sb[buf][k][cl * V + v]);
+        run[v] = fmaf(sa[buf][k][cl * V + v], run[v], sb[buf][k][cl * V + v]);
+        if (k + 1 == grp) s[v] = run[v];
       }
 #pragma unroll
     for (int k = G - 1; k >= 0; --k)
@@ -285,23 +344,30 @@ __global__ __launch_bounds__(SC_THREADS) void scan_bwd_kernel(const ScanK p) {
         s[v] = fmaf(f[i][v], s[v], keep[i][v] * xv[i][v]);
         xv[i][v] = before - xv[i][v];
       }
+    if (ok) {
 #pragma unroll
-    for (int i = R - 1; i >= 0; --i) {
-      float ox[V], og[V];
+      for (int i = R - 1; i >= 0; --i) {
+        float ox[V], og[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float lam = d[i][v] + m[v];
-        ox[v] = keep[i][v] * lam;
-        og[v] = ox[v] * f[i][v] * xv[i][v];
-        m[v] = f[i][v] * lam;
-      }
-      if (ok && t0 + i < p.l) {
-        const long long at = (long long)(p.reverse ? p.l - 1 - t0 - i : t0 + i) * p.c;
-        put<T, V>(dx + at, ox);
-        put<T, V>(dg + at, og);
+        for (int v = 0; v < V; ++v) {
+          const float lam = d[i][v] + m[v];
+          ox[v] = keep[i][v] * lam;
+          og[v] = ox[v] * f[i][v] * xv[i][v];
+          m[v] = f[i][v] * lam;
+        }
+        if (WHOLE) {
+          ox_.store(tile, i, ox);
+          og_.store(tile, i, og);
+        } else {
+          ox_.store_cut(t0 + i, ox);
+          og_.store_cut(t0 + i, og);
+        }
       }
     }
-  }
+  };
+  int tile = end - 1;
+  if (cut) work(tile--, std::false_type{});
+  for (; tile >= first; --tile) work(tile, std::true_type{});
   if (p.dh0 && seg == 0 && grp == 0 && ok) {
 #pragma unroll
     for (int v = 0; v < V; ++v) p.dh0[(long long)n * p.c + c + v] = mu[v];
@@ -328,28 +394,61 @@ __global__ __launch_bounds__(SC_THREADS) void scan_segment_kernel(const ScanK p)
   float A[V], B[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
-  for (int k = 0; k < per; k += R) {
-    const int t0 = BWD ? lo + per - R - k : lo + k;           // batches of R rows, backward from the last
-    if (t0 >= hi) continue;
-    Rows<T, V, R> ry, rg;
-    rg.load(g, p.g_ld, t0, p.l, p.reverse);
-    ry.load(y, y_ld, t0, p.l, p.reverse);
+  Walk<T, V, R> ry[2], rg[2];
+  auto take = [&](int slot, int rows, auto whole) {              // `rows` of the batch exist
+    constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       const int i = BWD ? R - 1 - j : j;
       float gv[V], yv[V];
-      unpack<T, V>(rg.r[i], gv);
-      unpack<T, V>(ry.r[i], yv);
+      unpack<T, V>(rg[slot].r[i], gv);
+      unpack<T, V>(ry[slot].r[i], yv);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         float f, keep;
         gate(gv[v], f, keep);
-        if (t0 + i < hi) {
+        if (WHOLE || i < rows) {
           A[v] *= f;
           B[v] = BWD ? f * (B[v] + yv[v]) : fmaf(f, B[v], keep * yv[v]);
         }
       }
     }
+  };
+  // batches of R rows, in walk order or (backward) from the last; the short one is the last in walk order
+  const int batches = (hi - lo) / R, rest = (hi - lo) - batches * R;
+  auto at = [&](int slot, int t0) {
+    rg[slot].start(g, p.g_ld, t0, p.l, p.reverse);
+    ry[slot].start(y, y_ld, t0, p.l, p.reverse);
+  };
+  if (BWD && rest > 0) {
+    at(0, lo + batches * R);
+    rg[0].load(rest);
+    ry[0].load(rest);
+    take(0, rest, std::false_type{});
+  }
+  if (batches > 0) {
+    at(0, BWD ? lo + (batches - 1) * R : lo);
+    rg[0].load();
+    ry[0].load();
+    for (int k = 0; k < batches; k += 2) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (k + u < batches) {
+          if (k + u + 1 < batches) {
+            at(u ^ 1, BWD ? lo + (batches - 2 - k - u) * R : lo + (k + u + 1) * R);
+            rg[u ^ 1].load();
+            ry[u ^ 1].load();
+          }
+          take(u, R, std::true_type{});
+        }
+      }
+    }
+  }
+  if (!BWD && rest > 0) {
+    at(0, lo + batches * R);
+    rg[0].load(rest);
+    ry[0].load(rest);
+    take(0, rest, std::false_type{});
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) { sa[grp][cl * V + v] = A[v]; sb[grp][cl * V + v] = B[v]; }
@@ -384,9 +483,11 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* x, long long x_
   h[i] = from_f32<T>(s);
 }
 
-// Workgroups of one segment a window; segments so that the launch has about 512 of them (two a CU), each at least
-// SC_MIN_TILES tiles long.
-constexpr int SC_FILL = 512, SC_MIN_TILES = 4;
+// Enough workgroups to fill the chip: about two a CU.  Half of that or more without segments: one launch.  Otherwise as many
+// segments as fill it, down to one tile each (against segments of at least four tiles, forward: [1, 1024, 1024] 15.6 -> 8.4 us,
+// [1, 4096, 256] 16.3 -> 9.4, [4, 4096, 512] 19.7 -> 20.0; unsplit: 28, 105 and 106 us).  Two tiles gain nothing from a second
+// launch.
+constexpr int SC_FILL = 512;
 
 struct Plan { int v, cl, ncb, tiles, segs, seg_tiles; };
 
@@ -398,10 +499,9 @@ Plan make_plan(int dtype, int n, int l, int c, bool even) {
   q.tiles = cdiv(l, SC_TILE);
   const long long wgs = (long long)n * q.ncb;
   int segs = 1;
-  if (wgs < SC_FILL / 2) {
+  if (wgs < SC_FILL / 2 && q.tiles > 2) {
     segs = (int)(SC_FILL / wgs);
-    segs = segs < q.tiles / SC_MIN_TILES ? segs : q.tiles / SC_MIN_TILES;
-    if (segs < 1) segs = 1;
+    segs = segs < q.tiles ? segs : q.tiles;
   }
   q.seg_tiles = cdiv(q.tiles, segs);
   q.segs = cdiv(q.tiles, q.seg_tiles);
@@ -410,8 +510,14 @@ Plan make_plan(int dtype, int n, int l, int c, bool even) {
 
 int check_scan(const char* what, int32_t dtype, int64_t n, int64_t l, int64_t c) {
   UNET_REQUIRE(dtype == UNET_BF16 || dtype == UNET_F32, "%s: bad dtype %d", what, dtype);
-  UNET_REQUIRE(n > 0 && l > 0 && c > 0 && l <= 0x7fffffff - 4096 && n * ((c + 63) / 64) < (1ll << 31), "%s: bad shape n=%lld l=%lld c=%lld",
+  UNET_REQUIRE(n > 0 && l > 0 && c > 0 && l <= 0x7fffffff - 4096 && n * ((c + 63) / 64) < (1ll << 31) && c <= (1 << 22), "%s: bad shape n=%lld l=%lld c=%lld",
                what, (long long)n, (long long)l, (long long)c);
+  return 0;
+}
+
+// a tile's rows lie within one buffer descriptor's 31 bits
+int check_pitch(const char* what, int64_t ld) {
+  UNET_REQUIRE(ld >= 0 && ld <= (1ll << 22), "%s: row pitch %lld, must be 0 .. 2^22 elements", what, (long long)ld);
   return 0;
 }
 
@@ -452,6 +558,7 @@ extern "C" int unet_gated_scan_fwd(int32_t dtype, const void* x, int64_t x_ns, i
                                    float* last, float* states, void* workspace, size_t ws_bytes, void* stream) {
   if (check_scan("gated_scan_fwd", dtype, n, l, c)) return -1;
   UNET_REQUIRE(x && g && h, "gated_scan_fwd: null pointer");
+  if (check_pitch("gated_scan_fwd", x_ld) || check_pitch("gated_scan_fwd", g_ld)) return -1;
   const bool even = c % 2 == 0 && even4(x, x_ns, x_ld) && even4(g, g_ns, g_ld) && even4(h, 0, 0);
   const Plan q = make_plan(dtype, n, l, c, even);
   UNET_REQUIRE(q.segs == 1 || (workspace && ws_bytes >= (size_t)n * q.segs * c * sizeof(float2)),
@@ -473,6 +580,7 @@ extern "C" int unet_gated_scan_bwd(int32_t dtype, const void* x, int64_t x_ns, i
                                    float* dh0, void* workspace, size_t ws_bytes, void* stream) {
   if (check_scan("gated_scan_bwd", dtype, n, l, c)) return -1;
   UNET_REQUIRE(x && g && states && dh && dx && dg, "gated_scan_bwd: null pointer");
+  if (check_pitch("gated_scan_bwd", x_ld) || check_pitch("gated_scan_bwd", g_ld) || check_pitch("gated_scan_bwd", dh_ld)) return -1;
   const bool even = c % 2 == 0 && even4(x, x_ns, x_ld) && even4(g, g_ns, g_ld) && even4(dh, dh_ns, dh_ld) && even4(dx, 0, 0) &&
                     even4(dg, 0, 0);
   const Plan q = make_plan(dtype, n, l, c, even);

@@ -1691,8 +1691,8 @@ def _once_differentiable(what: str):
 
 
 def _dense_channels(t: Tensor) -> Tensor:
-    """Any window and row stride will do; the channels of a row must be adjacent."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """Any window and row stride will do up to 2^22 elements a row; the channels of a row must be adjacent."""
+    return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-2) <= 1 << 22 else t.contiguous()
 
 
 def _check_scan(what: str, x: Tensor, gate: Tensor, state: Optional[Tensor], dims: int):
