@@ -22,11 +22,19 @@ namespace {
 // up to this head size two workgroups share a CU: 256 registers a lane, which also keeps the accumulators out of AGPRs
 constexpr int REL_OCC2 = 128;
 
-// the far side's constant for a tile with offsets dmin .. dmax, and whether it is one
-struct Far { bool far; float c; };
-__device__ __forceinline__ Far rel_far(int dmin, int dmax, int sat, float cneg, float cpos) {
-  return Far{dmax <= -sat || dmin >= sat, dmax <= -sat ? cneg : cpos};
+// Streamed tiles [lo, hi) of T rows against the 32 rows a wave holds from `own` on: [lo, n0) lie wholly beyond one edge of the
+// band, [n0, n1) touch it, [n1, hi) lie beyond the other edge.  The three runs are three loops (a wave's own bounds: every tile
+// has one barrier, whichever loop it is in), so the accumulators pass no branch.
+struct Runs { int n0, n1; };
+template <int T> __device__ __forceinline__ Runs rel_runs(int lo, int hi, int own, int sat) {
+  const int left = own - sat - (T - 1), right = own + 31 + sat;           // first tile that starts behind `left` / at or behind `right`
+  Runs r;
+  r.n0 = max(lo, min(hi, left >= 0 ? left / T + 1 : 0));
+  r.n1 = max(r.n0, min(hi, (right + T - 1) / T));
+  return r;
 }
+typedef std::integral_constant<bool, true> Near;
+typedef std::integral_constant<bool, false> Beyond;
 
 // TileLoader of attn_tiles.h for tiles of ROWS rows (the same LDS image)
 template <int HDP, int ROWS> struct RowLoader {
@@ -101,6 +109,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     const int nkb = (len + AT_BK - 1) / AT_BK;
     const int kb_lo = cneg == -INFINITY ? max(0, q0 - p.sat + 1) / AT_BK : 0;
     const int kb_hi = cpos == -INFINITY ? min(nkb, (q0 + AT_BQ - 2 + p.sat) / AT_BK + 1) : nkb;
+    const Runs runs = rel_runs<AT_BK>(kb_lo, kb_hi, q0 + wave * 32, p.sat);
     const unsigned tile_step = (unsigned)AT_BK * p.c * 2;
     auto issue = [&](int kb, int buf) {
       char* at = smem + buf * 2 * G::TILE;
@@ -113,14 +122,14 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     // a row that exceeds the margin sends the workgroup through a second walk with the true maxima
     int bad = 0, buf = 0;
     while (true) {
-      for (int kb = kb_lo; kb < kb_hi; ++kb) {
+      auto tile = [&](int kb, auto near, float beyond) {
+        constexpr bool NEAR = decltype(near)::value;
         __syncthreads();
         if (kb + 1 < kb_hi) issue(kb + 1, buf ^ 1);
         const char* kt = smem + buf * 2 * G::TILE;
         const char* vt = kt + G::TILE;
         buf ^= 1;
-        const int key0 = kb * AT_BK, q0w = q0 + wave * 32;
-        const Far far = rel_far(key0 - q0w - 31, key0 + AT_BK - 1 - q0w, p.sat, cneg, cpos);
+        const int key0 = kb * AT_BK;
 
         f32x16 st[2];
 #pragma unroll
@@ -157,15 +166,13 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         __builtin_amdgcn_sched_barrier(0);
 
         // score in the log2 domain = st * mul + add
-        float mul = p.scale_log2, add = far.c;
-        if (!far.far) {
+        const float mul = NEAR ? 1.f : p.scale_log2, add = NEAR ? 0.f : beyond;
+        if constexpr (NEAR) {
           const float* bl = bias + (key0 + 4 * h - qrow + p.sat + REL_PAD);
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int e = 0; e < 16; ++e) st[t][e] = fmaf(st[t][e], p.scale_log2, bl[32 * t + (e & 3) + 8 * (e >> 2)]);
-          mul = 1.f;
-          add = 0.f;
         }
         if (key0 + AT_BK > len) {
 #pragma unroll
@@ -185,7 +192,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         bad |= mx > m + 32.f;
         const float shift = add - (m == -INFINITY ? 0.f : m);
         auto exp_one = [&](int t, int e) {
-          const float pe = __builtin_amdgcn_exp2f(fmaf(st[t][e], mul, shift));
+          const float pe = __builtin_amdgcn_exp2f(NEAR ? st[t][e] + shift : fmaf(st[t][e], mul, shift));
           st[t][e] = pe;
           lsum += pe;
         };
@@ -206,7 +213,11 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
             }
           }
         }
-      }
+      };
+      int kb = kb_lo;
+      for (; kb < runs.n0; ++kb) tile(kb, Beyond{}, cneg);
+      for (; kb < runs.n1; ++kb) tile(kb, Near{}, 0.f);
+      for (; kb < kb_hi; ++kb) tile(kb, Beyond{}, cpos);
       if (!(kb_hi - kb_lo > 1 && __syncthreads_or(bad))) break;
       issue(kb_lo, buf);
       m = mtrue;
@@ -358,14 +369,14 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     rel_fill(p, head, bias, tid, AT_THREADS);
     float* const dg = diag + wave * DG_WORDS;
     int buf = 0;
-    for (int kb = kb_lo; kb < kb_hi; ++kb) {
+    auto tile = [&](int kb, auto near, float beyond, float& fsum) {
+      constexpr bool NEAR = decltype(near)::value;
       __syncthreads();
       if (kb + 1 < kb_hi) issue(kb + 1, buf ^ 1);
       const char* kt = smem + buf * 2 * TILE;
       const char* vt = kt + TILE;
       buf ^= 1;
       const int key0 = kb * BW_ROWS;
-      const Far far = rel_far(key0 - q0w - 31, key0 + BW_ROWS - 1 - q0w, p.sat, cneg, cpos);
 
       f32x16 st, dp;
 #pragma unroll
@@ -392,15 +403,12 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       load_t(0, 0);
       __builtin_amdgcn_sched_barrier(0);
       const float* bl = bias + (key0 + 4 * h - qrow + p.sat + REL_PAD);
-      float mul = p.scale_log2, add = far.c - lse;
-      if (!far.far) {
+      const float shift = beyond - lse;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) st[e] = fmaf(st[e], p.scale_log2, bl[(e & 3) + 8 * (e >> 2)]);
-        mul = 1.f;
-        add = -lse;
+      for (int e = 0; e < 16; ++e) {
+        const float off = NEAR ? bl[(e & 3) + 8 * (e >> 2)] - lse : shift;
+        st[e] = __builtin_amdgcn_exp2f(fmaf(st[e], p.scale_log2, off));
       }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) st[e] = __builtin_amdgcn_exp2f(fmaf(st[e], mul, add));
       if (key0 + BW_ROWS > len) {
 #pragma unroll
         for (int e = 0; e < 16; ++e)
@@ -409,11 +417,9 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 #pragma unroll
       for (int e = 0; e < 16; ++e) st[e] *= dp[e] - delta;
       if (p.part) {
-        if (far.far) {
-          float fsum = 0.f;
+        if constexpr (!NEAR) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) fsum += st[e];
-          if (key0 < q0w) fneg += fsum; else fpos += fsum;
         } else {
           float* row = dg + r * DG_PITCH + DG_ZERO + 4 * h;
 #pragma unroll
@@ -447,7 +453,12 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 #pragma unroll
         for (int d = 0; d < G::DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ft[g][d], db, acc[d], 0, 0, 0);
       }
-    }
+    };
+    const Runs runs = rel_runs<BW_ROWS>(kb_lo, kb_hi, q0w, p.sat);
+    int kb = kb_lo;
+    for (; kb < runs.n0; ++kb) tile(kb, Beyond{}, cneg, fneg);
+    for (; kb < runs.n1; ++kb) tile(kb, Near{}, 0.f, fneg);
+    for (; kb < kb_hi; ++kb) tile(kb, Beyond{}, cpos, fpos);
   }
 
   if (qrow < p.l) {
@@ -566,7 +577,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     rel_fill(p, head, bias, tid, AT_THREADS);
     if (tid < 2 * BW_ROWS) stats[tid] = load_stat(qb_lo);
     int buf = 0;
-    for (int qb = qb_lo; qb < qb_hi; ++qb, buf ^= 1) {
+    auto tile = [&](int qb, auto near, float beyond) {
+      constexpr bool NEAR = decltype(near)::value;
       __syncthreads();   // the tile and its stats are in LDS; every wave is done with the other buffer
       float stat_next = 0.f;
       if (qb + 1 < qb_hi) {
@@ -577,7 +589,6 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       const char* dtile = qtile + TILE;
       const float* st_in = stats + buf * 2 * BW_ROWS;
       const int row0 = qb * BW_ROWS;
-      const Far far = rel_far(key0w - row0 - 31, key0w + 31 - row0, p.sat, cneg, cpos);
       f32x16 st, dp;
 #pragma unroll
       for (int e = 0; e < 16; ++e) { st[e] = 0.f; dp[e] = 0.f; }
@@ -606,20 +617,14 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       load_tt(0, 0);
       __builtin_amdgcn_sched_barrier(0);
       const float* bl = bias + (key - row0 - 4 * h - 27 + p.sat + REL_PAD);     // bl[27 - x]: local row x + 4h
-      float mul = p.scale_log2, add = far.c;
-      if (!far.far) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) st[e] = fmaf(st[e], p.scale_log2, bl[27 - 8 * (e >> 2) - (e & 3)]);
-        mul = 1.f;
-        add = 0.f;
-      }
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
         const f32x4 ls = *reinterpret_cast<const f32x4*>(st_in + 8 * e4 + 4 * h);
         const f32x4 de = *reinterpret_cast<const f32x4*>(st_in + BW_ROWS + 8 * e4 + 4 * h);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float pe = __builtin_amdgcn_exp2f(fmaf(st[4 * e4 + e], mul, add - ls[e]));
+          const float off = NEAR ? bl[27 - 8 * e4 - e] - ls[e] : beyond - ls[e];
+          const float pe = __builtin_amdgcn_exp2f(fmaf(st[4 * e4 + e], p.scale_log2, off));
           st[4 * e4 + e] = pe;
           dp[4 * e4 + e] = pe * (dp[4 * e4 + e] - de[e]);
         }
@@ -634,7 +639,13 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         dka[d0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tq[b & 1], db, dka[d0], 0, 0, 0);
       }
       if (qb + 1 < qb_hi && tid < 2 * BW_ROWS) stats[(buf ^ 1) * 2 * BW_ROWS + tid] = stat_next;
-    }
+      buf ^= 1;
+    };
+    const Runs runs = rel_runs<BW_ROWS>(qb_lo, qb_hi, key0w, p.sat);       // rows in front of the keys: key - row > 0
+    int qb = qb_lo;
+    for (; qb < runs.n0; ++qb) tile(qb, Beyond{}, cpos);
+    for (; qb < runs.n1; ++qb) tile(qb, Near{}, 0.f);
+    for (; qb < qb_hi; ++qb) tile(qb, Beyond{}, cneg);
   }
 
   if (key < p.l) {
