@@ -69,6 +69,31 @@ def test_refusals_on_cpu():
     assert [lib.unet_adamw8_blocks(b) for b in (1, 4, 5, 16384)] == [1, 1, 2, 4096]
 
 
+def test_partly_stepped_groups_keep_their_moments_on_cpu():
+    """A loaded group of which some large tensors have codes, one fp32 moments and one nothing yet."""
+    from unet_amd.optim import ClipAdamW, dequantise_moment, quantise_moment
+    gen = torch.Generator().manual_seed(1)
+    params = [torch.nn.Parameter(torch.zeros(s)) for s in ((50, 100), (4097,), (5000,), (10,))]
+    m, v = torch.randn(50, 100, generator=gen), torch.rand(50, 100, generator=gen)
+    codes = dict(zip(("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale"),
+                     quantise_moment(m, False) + quantise_moment(v.sqrt(), True)))
+    m2, v2 = torch.randn(5000, generator=gen), torch.rand(5000, generator=gen)
+    opt = ClipAdamW(params, state_bits=8)
+    saved = opt.state_dict()
+    saved["state"] = {0: dict(codes, step=torch.tensor(3.0)), 2: dict(exp_avg=m2, exp_avg_sq=v2, step=torch.tensor(7.0))}
+    opt.load_state_dict(copy.deepcopy(saved))
+    opt.moment_buffers()
+    st = opt.state[params[0]]
+    for k, t in codes.items():
+        assert torch.equal(st[k].float(), t.float()), k
+    assert [float(opt.state[p]["step"]) for p in params] == [3, 0, 7, 0]
+    st = opt.state[params[2]]
+    want = quantise_moment(m2, False)
+    assert torch.equal(dequantise_moment(st["exp_avg"], st["exp_avg_scale"]), dequantise_moment(*want))
+    for i in (1, 3):
+        assert float(opt.state[params[i]]["exp_avg"].float().abs().max()) == 0
+
+
 # ------------------------------------------------------------------------------------------------ GPU
 SHAPES = [(256, 32, 7), (256,), (1,), (3,), (512, 256, 1), (37, 5), (1024, 130), (2, 3, 5, 7), (8193,), (4096,), (4095,), (90, 99),
           (0,), (4096, 33)]
@@ -294,3 +319,39 @@ def test_graph_replays_and_many_tensors(max_norm):
         assert torch.equal(eager.total_norm(), cap.total_norm())
     for x, y in zip(eager.moment_buffers().values(), cap.moment_buffers().values()):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_thawed_tensors_and_switched_state_bits():
+    """A frozen tensor joins after some steps; then the group goes to fp32 moments and back: nobody's moments are lost."""
+    from unet_amd.optim import ClipAdamW
+    params, gen = make(6, [(64, 80), (70, 90), (9,)])
+    lr, wd = 1e-2, 0.01
+    opt = ClipAdamW(params, lr=lr, betas=BETAS, weight_decay=wd, state_bits=8, max_grad_norm=5.0)
+    params[1].requires_grad_(False)
+    for _ in range(2):
+        set_grads(params, gen, 1.0)
+        params[1].grad = None
+        opt.step()
+    fresh = lambda p, small: (torch.zeros_like(p, dtype=torch.float64), torch.zeros_like(p, dtype=torch.float64), small, 0.0)
+    a, c = snapshot(opt, [params[0], params[2]])
+    before = [a, fresh(params[1].detach(), True), c]
+    params[1].requires_grad_(True)
+    for bits in (8, 32):
+        opt.param_groups[0]["state_bits"] = bits
+        before = [(m, v, bits == 8 and p.numel() >= 4096, t) for (m, v, _, t), p in zip(before, params)]
+        set_grads(params, gen, 1.0)
+        p0 = [p.detach().clone() for p in params]
+        opt.step()
+        after = snapshot(opt, params)
+        assert [small for _, _, small, _ in after] == [bits == 8, bits == 8, False]
+        check_step(opt, params, p0, before, [p.grad for p in params], lr, wd, 5.0)
+        before = after
+    opt.param_groups[0]["state_bits"] = 8
+    set_grads(params, gen, 0.0)
+    opt.step()
+    for (m, v, _, _), (m1, v1, small, t), p in zip(before, snapshot(opt, params), params):
+        assert small == (p.numel() >= 4096) and t == (3 if p is params[1] else 5)
+        # the moments are rounded to codes once on the way in and once when the step stores them
+        assert float((m1 - BETAS[0] * m).abs().max()) <= 2 * 2.0 ** -4 * float(m.abs().max())
+        assert float((v1.sqrt() - (BETAS[1] * v).sqrt()).abs().max()) <= 2 * 2.0 ** -4 * float(v.max().sqrt())

@@ -185,18 +185,23 @@ class _Group8:
 
     def fill(self, states) -> None:
         """Moments and step counts from the tensors' loaded states, in either form, or from an earlier table's views."""
-        for names, flat, code in ((("exp_avg", "exp_avg_sq_root"), (self.m8, self.r8), True),
-                                  (("exp_avg_scale", "exp_avg_sq_root_scale"), (self.m_scale, self.r_scale), False)):
+        coded = [(st, v) for st, v in zip(states, self.views) if "exp_avg_scale" in v]
+        if coded and all("exp_avg_scale" in st for st, _ in coded):
             # the usual case, all of the large tensors held in codes already: one gather a buffer
-            group = [(st, v) for st, v in zip(states, self.views) if "exp_avg_scale" in v]
-            if group and all("exp_avg_scale" in st for st, _ in group):
+            for names, flat, code in ((("exp_avg", "exp_avg_sq_root"), (self.m8, self.r8), True),
+                                      (("exp_avg_scale", "exp_avg_sq_root_scale"), (self.m_scale, self.r_scale), False)):
                 for name, buf in zip(names, flat):
                     parts = []
-                    for st, v in group:
+                    for st, v in coded:
                         parts.append(st[name].reshape(-1).float())
                         if code and v[name].numel() % BLOCK:
                             parts.append(parts[-1].new_zeros(-v[name].numel() % BLOCK))
                     buf[:self.end8 if code else self.end8 // BLOCK].copy_(torch.cat(parts))
+        else:                                   # some of them have not been stepped yet, or come from fp32
+            for st, v in coded:
+                if "exp_avg_scale" in st:
+                    for k in v:
+                        v[k].copy_(st[k].reshape(v[k].shape))
         for st, view in zip(states, self.views):
             if "exp_avg" in st and not ("exp_avg_scale" in view and "exp_avg_scale" in st):
                 m, v = _load_moments(st)
@@ -245,7 +250,7 @@ class ClipAdamW(torch.optim.Optimizer):
     def _tables8(self, gi: int, group) -> Optional[_Group8]:
         g = self._groups.get(gi)
         ptrs = [p.data_ptr() for p in group["params"] if p.requires_grad]
-        if g is None or g.ptrs != ptrs:
+        if not isinstance(g, _Group8) or g.ptrs != ptrs:
             params = [p for p in group["params"] if p.requires_grad]
             if not params:
                 return None
@@ -262,7 +267,7 @@ class ClipAdamW(torch.optim.Optimizer):
             return None
         g = self._groups.get(gi)
         key = tuple(p.data_ptr() for p in params)
-        if g is None or g.ptr_key != key:
+        if not isinstance(g, _Group) or g.ptr_key != key:
             old = g
             g = _Group(params)
             starts = g.start4.cpu().tolist()
