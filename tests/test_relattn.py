@@ -175,6 +175,8 @@ def test_refusals_on_cpu():
     for scale in (0.0, -1.0, float("inf"), float("nan")):
         with pytest.raises(ValueError, match="scale"):
             ops.rel_bias_attention(q, q, q, t, 2, scale=scale)
+    with pytest.raises(ValueError, match="head size"):
+        ops.rel_bias_attention(q[..., :0], q[..., :0], q[..., :0], t, 2)
     for lengths in (torch.zeros(2), torch.zeros(3, dtype=torch.int32)):
         with pytest.raises(ValueError, match="lengths"):
             ops.rel_bias_attention(q, q, q, t, 2, lengths=lengths)
@@ -186,7 +188,7 @@ def test_refusals_on_cpu():
         return lib.unet_rel_attn_fwd(dtype, q, q, q, 16, 1, buckets, starts, None, n, l, c, nh, scale, 16, None, None)
 
     for kw, msg in ((dict(q=None), b"null"), (dict(dtype=5), b"dtype"), (dict(l=0), b"shape"), (dict(c=10), b"head_dim"), (dict(q=24), b"aligned"),
-                    (dict(scale=0.0), b"scale"), (dict(buckets=3), b"buckets"), (dict(starts=(C.c_int32 * 2)(1, 1)), b"distance 0"),
+                    (dict(scale=0.0), b"scale"), (dict(scale=3e38), b"scale"), (dict(buckets=3), b"buckets"), (dict(starts=(C.c_int32 * 2)(1, 1)), b"distance 0"),
                     (dict(starts=(C.c_int32 * 2)(0, 0)), b"last bucket"), (dict(starts=(C.c_int32 * 2)(0, 600)), b"last bucket"),
                     (dict(buckets=6, starts=(C.c_int32 * 3)(0, 3, 2)), b"decrease"), (dict(l=1 << 27, c=8), b"slab")):
         assert fwd(**kw) == -1 and msg in lib.unet_last_error(), (kw, lib.unet_last_error())
@@ -384,3 +386,30 @@ def test_same_bits_side_stream_and_graph_replays(dtype):
         want = call(*fresh[:4], dout, **kw)
         for a, key in zip((out,) + grads, ("out", "dq", "dk", "dv", "dtable")):
             assert torch.equal(a, want[key]), (rep, key)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_pieces_of_flat_buffers(dtype):
+    """Contiguous tensors that start off a 16-byte boundary, the upstream gradient among them."""
+    from unet_amd import ops
+    q, k, v, table, dout = inputs(1, 70, 2, 16, 16, dtype, seed=21)
+    odd = [torch.cat([t.new_zeros(i + 1), t.reshape(-1)])[i + 1:].view(t.shape) for i, t in enumerate((q, k, v))]
+    assert all(t.data_ptr() % 16 and t.is_contiguous() for t in odd)
+    leaves = [t.requires_grad_() for t in odd] + [table.requires_grad_()]
+    out = ops.rel_bias_attention(*leaves, n_heads=2, max_distance=40)
+    flat = torch.cat([out.new_zeros(3), out.reshape(-1)])
+    grads = torch.autograd.grad(flat, leaves, torch.cat([dout.new_ones(3), dout.reshape(-1)]))
+    want = oracle(q, k, v, table, 2, 16 ** -0.5, 40, None, dout)
+    for key, t in zip(("out", "dq", "dk", "dv", "dtable"), (out,) + grads):
+        near(t, want[key], key)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    from unet_amd import ops
+    q, k, v, table, dout = inputs(1, 40, 2, 16, 16, torch.bfloat16, seed=22)
+    q.requires_grad_()
+    out = ops.rel_bias_attention(q, k, v, table, 2)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(out, q, dout, create_graph=True)

@@ -119,7 +119,14 @@ def test_refusals_on_cpu():
         ops.gated_scan_step(x, g, torch.zeros(2, 6))
     with pytest.raises(ValueError, match="state must be"):
         ops.gated_scan_step(x[0], g[0], torch.zeros(3, 6))
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.gated_scan_step(x[0], g[0].requires_grad_(), torch.zeros(4, 6))
     lib = _lib.load()
+    for ld in (-1, (1 << 22) + 1):
+        assert lib.unet_gated_scan_fwd(0, 16, 0, ld, 16, 0, 1, None, 0, 1, 2, 1, 16, None, None, None, 0, None) == -1
+        assert b"row pitch" in lib.unet_last_error()
+        assert lib.unet_gated_scan_bwd(0, 16, 0, 1, 16, 0, 1, 16, 16, 0, ld, None, 0, 1, 2, 1, 16, 16, None, None, 0, None) == -1
+        assert b"row pitch" in lib.unet_last_error()
     assert lib.unet_gated_scan_fwd(0, None, 0, 0, None, 0, 0, None, 0, 1, 1, 1, None, None, None, None, 0, None) == -1
     assert b"null" in lib.unet_last_error()
     assert lib.unet_gated_scan_fwd(7, 16, 0, 0, 16, 0, 0, None, 0, 1, 1, 1, 16, None, None, None, 0, None) == -1
@@ -298,3 +305,62 @@ def test_offsets_past_32_bits():
     want = oracle(x[2:, cut], g[2:, cut], state, None, None, False)
     near(h[2:, -100:], tuple(v[:, -100:] for v in want["h"]), "tail")
     near(last[2:], want["last"], "last")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("pitch,l", [(1 << 22, 130), ((1 << 22) + 6, 3)])
+def test_row_pitches_up_to_and_past_the_descriptor(pitch, l, dtype):
+    """2^22 elements a row is what a tile's 32-bit offsets reach; a longer pitch is copied."""
+    c = 6
+    x, g, h0, dh, dlast = inputs(1, l, c, dtype, seed=11)
+    wide = []
+    for t in (x, g, dh):
+        w = torch.empty((l - 1) * pitch + c, dtype=dtype, device="cuda").as_strided((1, l, c), (0, pitch, 1))
+        wide.append(w.copy_(t))
+    for rev in (False, True):
+        got = call(wide[0], wide[1], h0, wide[2], dlast, rev)
+        want = oracle(x, g, h0, dh, dlast, rev)
+        for k in got:
+            near(got[k], want[k], (k, rev))
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    from unet_amd import ops
+    x, g, h0, dh, _ = inputs(1, 70, 8, torch.float32, seed=12)
+    x.requires_grad_()
+    h = ops.gated_scan(x, g, h0)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(h, x, dh, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs_in_turn():
+    """Split rows (workspace) in two graphs that replay on two streams at once and in turn, with eager work between."""
+    from unet_amd import ops
+    sets = [inputs(1, 3000 + 50 * i, 40, torch.bfloat16, seed=13 + i)[:3] for i in range(2)]
+    graphs, outs = [], []
+    for x, g, h0 in sets:
+        ops.gated_scan(x, g, h0)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(ops.gated_scan(x, g, h0, return_state=True))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(4):
+        for x, g, h0 in sets:
+            g.add_(0.25)
+        torch.cuda.synchronize()
+        if rep % 2:
+            for graph, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    graph.replay()
+        else:
+            for graph in graphs:
+                graph.replay()
+        torch.cuda.synchronize()
+        for (x, g, h0), (h, last) in zip(sets, outs):
+            h2, last2 = ops.gated_scan(x, g, h0, return_state=True)
+            assert torch.equal(h, h2) and torch.equal(last, last2), rep

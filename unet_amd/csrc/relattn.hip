@@ -765,7 +765,8 @@ int make_rel(const char* what, RelK& p, int32_t dtype, int32_t n, int32_t l, int
   UNET_REQUIRE((long long)l * c * (dtype == UNET_BF16 ? 2 : 4) < (1ll << 31), "%s: one [L, C] slab of %lld bytes exceeds a buffer descriptor",
                what, (long long)l * c * (dtype == UNET_BF16 ? 2 : 4));
   UNET_REQUIRE((long long)n * nh * cdiv(l, 32) < (1ll << 31), "%s: grid too large", what);
-  UNET_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale must be positive and finite, got %g", what, (double)scale);
+  UNET_REQUIRE(scale > 0.f && scale * REL_LOG2E < INFINITY, "%s: scale must be positive and finite (also times log2 e), got %g", what,
+               (double)scale);
   UNET_REQUIRE(buckets >= 4 && buckets % 2 == 0 && buckets <= 2 * UNET_REL_MAX_SIDE, "%s: %d buckets, must be even and 4 .. %d", what,
                buckets, 2 * UNET_REL_MAX_SIDE);
   const int side = buckets / 2;

@@ -1787,6 +1787,9 @@ def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor] = None, reverse: bo
 def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
     """One row of ``gated_scan`` for every sequence: ``x``, ``gate`` ``[N, C]``; ``state`` ``[N, C]`` fp32 contiguous, moved on
     IN PLACE.  Returns the new state in ``x``'s dtype.  Inference only."""
+    if _wants_grad(x, gate, state):
+        raise RuntimeError("gated_scan_step has no backward pass (its state moves on in place): call it under torch.no_grad(), or "
+                           "gated_scan on the rows")
     _check_scan("gated_scan_step", x, gate, state, 2)
     if not state.is_contiguous():
         raise ValueError("gated_scan_step: the state is updated in place and must be contiguous")
@@ -1832,6 +1835,12 @@ def rel_bucket(offset: Tensor, n_buckets: int, max_distance: int) -> Tensor:
     return torch.bucketize(offset.abs(), starts, right=True) - 1 + (offset > 0) * (n_buckets // 2)
 
 
+def _aligned(t: Tensor) -> Tensor:
+    """Contiguous and on a 16-byte boundary (a piece of a flat buffer need not be)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 @functools.lru_cache(maxsize=None)
 def _starts_array(starts: Tuple[int, ...]):
     return (C.c_int32 * len(starts))(*starts)
@@ -1859,7 +1868,7 @@ class RelBiasAttnFn(torch.autograd.Function):
         _once_differentiable("rel_bias_attention")
         q, k, v, table, out, lse, lengths = ctx.saved_tensors
         n, l, c = q.shape
-        dout = dout.contiguous()
+        dout = _aligned(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         delta = torch.empty_like(lse)
         dtable = partials = None
@@ -1880,7 +1889,7 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
 
     ``q``, ``k``, ``v``: ``[N, L, C]``, all bf16 or all fp32; head h owns columns ``h*hd .. h*hd+hd-1``, ``hd = C / n_heads`` a
     multiple of 8 (bf16) or 4 (fp32), at most 256.  ``table``: ``[n_buckets, n_heads]`` fp32 or bf16 (``rel_bucket`` gives the
-    buckets; ``max_distance`` at most 512); an entry of -inf removes its pairs, and a far bucket of -inf also their cost.
+    buckets; ``max_distance`` at most 512); an entry of -inf removes its pairs, and in bf16 a far bucket of -inf also their cost.
     ``lengths``: ``[N]`` int32 valid positions of a padded batch (values are clamped to 0 .. L): positions behind them are
     neither keys nor queries, their outputs and gradients are zero.  A row with nothing to see gives zeros.  ``scale`` defaults
     to ``hd ** -0.5`` and must be positive.
@@ -1893,7 +1902,7 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
     if k.dtype != q.dtype or v.dtype != q.dtype or any(t.device != q.device for t in (k, v, table)):
         raise TypeError("rel_bias_attention: q, k and v must have one dtype and all tensors one device")
     n, l, c = q.shape
-    if n_heads < 1 or n_heads > 256 or c % n_heads or (c // n_heads) % unit or c // n_heads > 256 or c > 8192:
+    if n_heads < 1 or n_heads > 256 or c % n_heads or (c // n_heads) % unit or c // n_heads > 256 or not 0 < c <= 8192:
         raise ValueError(f"rel_bias_attention: {c} channels in {n_heads} heads: the head size must be a multiple of {unit} for {q.dtype} "
                          "and at most 256 (at most 256 heads and 8192 channels)")
     if table.dim() != 2 or table.shape[1] != n_heads:
@@ -1910,7 +1919,7 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
     _need_cuda(q)
     if q.numel() == 0:
         return q * k * v + 0 * table.sum().to(q.dtype)
-    q, k, v, table = q.contiguous(), k.contiguous(), v.contiguous(), table.contiguous()
+    q, k, v, table = _aligned(q), _aligned(k), _aligned(v), table.contiguous()
     if _wants_grad(q, k, v, table):
         return RelBiasAttnFn.apply(q, k, v, table, n_heads, scale, starts, lengths)
     return _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, False)[0]
