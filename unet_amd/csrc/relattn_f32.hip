@@ -20,6 +20,27 @@ __device__ __forceinline__ Place place(const RelK& p) {
   return o;
 }
 
+// load_tile of attn_f32_tiles.h in two halves: the next tile is fetched into registers while this one is worked on
+template <int HDP> struct Fetch {
+  static constexpr int CH = HDP / 4, TOTAL = A32_BK * CH, N = (TOTAL + A32_THREADS - 1) / A32_THREADS;
+  f32x4 v[N];
+  __device__ __forceinline__ void get(const float* slab, int row0, int l, int ld, int hd, int tid) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = tid + k * A32_THREADS, r = i / CH, ch = i % CH;
+      v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (i < TOTAL && row0 + r < l && ch * 4 < hd) v[k] = *reinterpret_cast<const f32x4*>(slab + (long long)(row0 + r) * ld + ch * 4);
+    }
+  }
+  __device__ __forceinline__ void put(float* tile, int tid) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int i = tid + k * A32_THREADS;
+      if (i < TOTAL) *reinterpret_cast<f32x4*>(tile + i / CH * (HDP + 4) + i % CH * 4) = v[k];
+    }
+  }
+};
+
 template <int HDP>
 __global__ __launch_bounds__(A32_THREADS, 1) void rel32_fwd_kernel(const RelK p) {
   constexpr int LD = HDP + 4, DT = HDP / 16;
@@ -41,11 +62,16 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_fwd_kernel(const RelK p)
   rel_fill(p, o.head, bias, tid, A32_THREADS);
   float m = -INFINITY, lsum = 0.f;
   const int end = o.tile * A32_ROWS < o.len ? o.len : 0;            // (uniform) nothing to do behind the window's length
+  Fetch<HDP> fk, fv;
+  fk.get(kslab, 0, end, p.c, p.hd, tid);
+  fv.get(vslab, 0, end, p.c, p.hd, tid);
   for (int key0 = 0; key0 < end; key0 += A32_BK) {
     __syncthreads();
-    load_tile<HDP, A32_BK>(kt, kslab, key0, o.len, p.c, p.hd, tid);
-    load_tile<HDP, A32_BK>(vt, vslab, key0, o.len, p.c, p.hd, tid);
+    fk.put(kt, tid);
+    fv.put(vt, tid);
     __syncthreads();
+    fk.get(kslab, key0 + A32_BK, end, p.c, p.hd, tid);
+    fv.get(vslab, key0 + A32_BK, end, p.c, p.hd, tid);
     f32x4 st[2];
     float mx = -INFINITY;
 #pragma unroll
@@ -127,12 +153,18 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dq_kernel(const RelK p) 
   auto add = [](float* at, float v) { __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); };
   const float lse = row_ok ? p.lse[o.stat + qrow] : INFINITY;          // rows past the end: p = 0
   const float delta = row_ok ? p.delta[o.stat + qrow] : 0.f;
+  float fneg = 0.f, fpos = 0.f;                          // sums beyond the band
   const int end = o.tile * A32_ROWS < o.len ? o.len : 0;
+  Fetch<HDP> fk, fv;
+  fk.get(kslab, 0, end, p.c, p.hd, tid);
+  fv.get(vslab, 0, end, p.c, p.hd, tid);
   for (int key0 = 0; key0 < end; key0 += A32_BK) {
     __syncthreads();
-    load_tile<HDP, A32_BK>(kt, kslab, key0, o.len, p.c, p.hd, tid);
-    load_tile<HDP, A32_BK>(vt, vslab, key0, o.len, p.c, p.hd, tid);
+    fk.put(kt, tid);
+    fv.put(vt, tid);
     __syncthreads();
+    fk.get(kslab, key0 + A32_BK, end, p.c, p.hd, tid);
+    fv.get(vslab, key0 + A32_BK, end, p.c, p.hd, tid);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       f32x4 st = rows_dot<HDP>(kt, 16 * s, qreg, l15, g);
@@ -147,20 +179,17 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dq_kernel(const RelK p) 
         st[i] = pe * (dp[i] - delta);
       }
       if (p.part) {
-        // inside the band the sixteen rows of a lane group have sixteen offsets; beyond it they share one: summed first
+        // inside the band the sixteen rows of a lane group have sixteen offsets; beyond it they share one: kept in a register
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int key = key0 + 16 * s + 4 * g + i;
-          const bool edge = key - qrow <= -p.sat || key - qrow >= p.sat;
+          const int off = key0 + 16 * s + 4 * g + i - qrow;
+          const bool neg = off <= -p.sat, pos = off >= p.sat;
+          fneg += neg ? st[i] : 0.f;
+          fpos += pos ? st[i] : 0.f;
+          if (__any(!neg && !pos)) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (g == q && !edge) add(sums + wave * w + at[i], st[i]);
-          float lo = edge && at[i] == 0 ? st[i] : 0.f, hi = edge && at[i] != 0 ? st[i] : 0.f;
-          lo = wave_sum(lo);
-          hi = wave_sum(hi);
-          if (lane == 0) {
-            add(sums + wave * w, lo);
-            add(sums + wave * w + w - 1, hi);
+            for (int q = 0; q < 4; ++q)
+              if (g == q && !neg && !pos) add(sums + wave * w + at[i], st[i]);
           }
         }
       }
@@ -174,6 +203,12 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dq_kernel(const RelK p) 
       if (16 * d + 4 * g < p.hd) *reinterpret_cast<f32x4*>(yp + 16 * d + 4 * g) = row_ok ? acc[d] * p.scale : f32x4{0.f, 0.f, 0.f, 0.f};
   }
   if (p.part) {
+    fneg = wave_sum(fneg);
+    fpos = wave_sum(fpos);
+    if (lane == 0) {
+      add(sums + wave * w, fneg);
+      add(sums + wave * w + w - 1, fpos);
+    }
     __syncthreads();
     const int nt = (p.l + A32_ROWS - 1) / A32_ROWS;
     float* row = p.part + ((long long)o.head * p.parts + o.n * nt + o.tile) * w;
@@ -204,15 +239,24 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dkv_kernel(const RelK p)
   for (int d = 0; d < DT; ++d) { dka[d] = f32x4{0.f, 0.f, 0.f, 0.f}; dva[d] = f32x4{0.f, 0.f, 0.f, 0.f}; }
   rel_fill(p, o.head, bias, tid, A32_THREADS);
   const int end = o.tile * A32_ROWS < o.len ? o.len : 0;
-  for (int row0 = 0; row0 < end; row0 += A32_BK) {
-    __syncthreads();
-    load_tile<HDP, A32_BK>(qtile, qslab, row0, o.len, p.c, p.hd, tid);
-    load_tile<HDP, A32_BK>(dtile, dslab, row0, o.len, p.c, p.hd, tid);
+  Fetch<HDP> fq, fd;
+  float stat = 0.f;
+  auto get = [&](int row0) {
+    fq.get(qslab, row0, end, p.c, p.hd, tid);
+    fd.get(dslab, row0, end, p.c, p.hd, tid);
     if (tid < 2 * A32_BK) {
       const int r = row0 + (tid & (A32_BK - 1));
-      stats[tid] = r < o.len ? (tid < A32_BK ? p.lse[o.stat + r] : p.delta[o.stat + r]) : (tid < A32_BK ? INFINITY : 0.f);
+      stat = r < end ? (tid < A32_BK ? p.lse[o.stat + r] : p.delta[o.stat + r]) : (tid < A32_BK ? INFINITY : 0.f);
     }
+  };
+  get(0);
+  for (int row0 = 0; row0 < end; row0 += A32_BK) {
     __syncthreads();
+    fq.put(qtile, tid);
+    fd.put(dtile, tid);
+    if (tid < 2 * A32_BK) stats[tid] = stat;
+    __syncthreads();
+    get(row0 + A32_BK);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       f32x4 st = rows_dot<HDP>(qtile, 16 * s, kreg, l15, g);
