@@ -4,8 +4,10 @@ gradients on the GPU against a plain evaluation in float64.
 Tolerances are first-order error bounds evaluated in float64 next to the values.  With u = 2^-24 and r = 2^-8 (bf16) or 0 (fp32):
   score:  an fp32 sum of hd products, then 3 more roundings in the log2 domain, and the stored maximum / lse of its size:
           ds = u ((hd + 4) scale |q| |k| + 8 (|S| + max_j |S| + 1)), so P is off by 2 ds relative
-  P V, P^T dO, dS K, dS^T Q: operands P and dS rounded to r relative, an fp32 sum of L terms (L u), the result rounded once
-  delta = <dO, O> takes O as stored: its error is |dO| . err(O) + hd u |dO| |O|
+  P V, P^T dO, dS K, dS^T Q: operands P and dS to f relative, an fp32 sum of L terms (L u), the result rounded once; f = r^2
+  (a value and the rounded rest of it) for windows of at most 128 rows, for P V where gradients follow and for dS K with heads of
+  at most 32, else r
+  delta = <dO, O> takes O to r^2: its error is |dO| . err(O) + hd u |dO| |O|
   dS = P (dP - delta): err = 2 ds |dS| + P (hd u |dO| |V| + err(delta)) + 4 u |dS|
   d table: sums of dS (before the rounding to bf16) in fp32, at most 64 terms deep inside a tile row, then one per tile and
   workgroup: 256 u relative to the sum of |dS|, and the rounding to the table's type."""
@@ -45,7 +47,9 @@ def oracle(q, k, v, table, nh, scale, maxd, lengths, dout):
     idx = row[pos[None, :] - pos[:, None] + l - 1]
     T = table.detach().double()
     z = lambda: torch.zeros((n, l, c), dtype=torch.float64, device=dev)
-    val = dict(out=z(), dq=z(), dk=z(), dv=z(), dtable=torch.zeros((B, nh), dtype=torch.float64, device=dev))
+    fine = half * half
+    rest = fine if l <= 128 else half
+    val = dict(out=z(), infer=z(), dq=z(), dk=z(), dv=z(), dtable=torch.zeros((B, nh), dtype=torch.float64, device=dev))
     err = {key: torch.zeros_like(t) for key, t in val.items()}
     picks = None
     for w in range(n):
@@ -66,21 +70,22 @@ def oracle(q, k, v, table, nh, scale, maxd, lengths, dout):
             ds = U * ((hd + 4) * scale * Q.abs() @ K.abs().T + 8 * (fin + fin.amax(1, keepdim=True) + 1))
             eP = P * (2 * ds + (2 * ds * P).sum(1, keepdim=True) + (m + 8) * U)
             O = P @ V
-            eO = eP @ V.abs() + (half + m * U) * (P @ V.abs())
+            val["infer"][w, :m, cols], err["infer"][w, :m, cols] = O, eP @ V.abs() + (rest + m * U) * (P @ V.abs())
+            eO = eP @ V.abs() + (fine + m * U) * (P @ V.abs())
             val["out"][w, :m, cols], err["out"][w, :m, cols] = O, eO
             if dout is None:
                 continue
             D = dout[w, :m, cols].double()
             dP = D @ V.T
-            eO = eO + half * O.abs()                       # as stored
+            eO = eO + fine * O.abs()                       # as stored: a value and its rest
             delta = (D * O).sum(1, keepdim=True)
             edelta = (D.abs() * eO).sum(1, keepdim=True) + hd * U * (D.abs() * O.abs()).sum(1, keepdim=True)
             dS = P * (dP - delta)
             edS = eP * (dP - delta).abs() + P * (hd * U * (D.abs() @ V.abs().T) + edelta) + 4 * U * dS.abs()
             val["dv"][w, :m, cols] = P.T @ D
-            err["dv"][w, :m, cols] = (eP + (half + m * U) * P).T @ D.abs()
-            e2 = edS + (half + m * U) * dS.abs()
-            val["dq"][w, :m, cols], err["dq"][w, :m, cols] = scale * dS @ K, scale * e2 @ K.abs()
+            err["dv"][w, :m, cols] = (eP + (rest + m * U) * P).T @ D.abs()
+            e2 = edS + (rest + m * U) * dS.abs()
+            val["dq"][w, :m, cols], err["dq"][w, :m, cols] = scale * dS @ K, scale * (e2 if hd > 32 else edS + (fine + m * U) * dS.abs()) @ K.abs()
             val["dk"][w, :m, cols], err["dk"][w, :m, cols] = scale * dS.T @ Q, scale * e2.T @ Q.abs()
             val["dtable"][:, h].index_add_(0, at.reshape(-1), dS.reshape(-1))
             err["dtable"][:, h].index_add_(0, at.reshape(-1), (edS + 256 * U * dS.abs()).reshape(-1))
@@ -184,16 +189,20 @@ def test_refusals_on_cpu():
     lib = _lib.load()
     st = (C.c_int32 * 2)(0, 1)
 
-    def fwd(dtype=1, n=1, l=4, c=8, nh=1, scale=1.0, buckets=4, starts=st, q=16):
-        return lib.unet_rel_attn_fwd(dtype, q, q, q, 16, 1, buckets, starts, None, n, l, c, nh, scale, 16, None, None)
+    def fwd(dtype=1, n=1, l=4, c=8, nh=1, scale=1.0, buckets=4, starts=st, q=16, rest=None, lse=None):
+        return lib.unet_rel_attn_fwd(dtype, q, q, q, 16, 1, buckets, starts, None, n, l, c, nh, scale, 16, rest, lse, None)
 
     for kw, msg in ((dict(q=None), b"null"), (dict(dtype=5), b"dtype"), (dict(l=0), b"shape"), (dict(c=10), b"head_dim"), (dict(q=24), b"aligned"),
                     (dict(scale=0.0), b"scale"), (dict(scale=3e38), b"scale"), (dict(buckets=3), b"buckets"), (dict(starts=(C.c_int32 * 2)(1, 1)), b"distance 0"),
                     (dict(starts=(C.c_int32 * 2)(0, 0)), b"last bucket"), (dict(starts=(C.c_int32 * 2)(0, 600)), b"last bucket"),
-                    (dict(buckets=6, starts=(C.c_int32 * 3)(0, 3, 2)), b"decrease"), (dict(l=1 << 27, c=8), b"slab")):
+                    (dict(buckets=6, starts=(C.c_int32 * 3)(0, 3, 2)), b"decrease"), (dict(l=1 << 27, c=8), b"slab"),
+                    (dict(dtype=0, lse=16), b"out_rest"), (dict(dtype=0, rest=16), b"out_rest"),
+                    (dict(dtype=0, lse=16, rest=24), b"aligned")):
         assert fwd(**kw) == -1 and msg in lib.unet_last_error(), (kw, lib.unet_last_error())
-    assert lib.unet_rel_attn_bwd(1, 16, 16, 16, 16, 1, 4, st, None, 16, 16, 16, 1, 4, 8, 1, 1.0, 16, 16, 16, 16, None, 16, None) == -1
+    assert lib.unet_rel_attn_bwd(1, 16, 16, 16, 16, 1, 4, st, None, 16, 16, 16, 16, 1, 4, 8, 1, 1.0, 16, 16, 16, 16, None, 16, None) == -1
     assert b"partial" in lib.unet_last_error()
+    assert lib.unet_rel_attn_bwd(0, 16, 16, 16, 16, 1, 4, st, None, 16, None, 16, 16, 1, 4, 8, 1, 1.0, 16, 16, 16, None, None, 16, None) == -1
+    assert b"out_rest" in lib.unet_last_error()
 
 
 # ------------------------------------------------------------------------------------------------ GPU
@@ -298,8 +307,8 @@ def test_zero_table_is_plain_attention_and_a_constant_changes_nothing():
     for t in (torch.zeros_like(table), torch.full_like(table, 2.5)):
         out = ops.rel_bias_attention(q, k, v, t, 2, scale=0.125)
         want = oracle(q, k, v, t, 2, 0.125, 128, None, None)
-        near(out, want["out"], "constant")
-        near(plain, want["out"], "band-pair kernel")
+        near(out, want["infer"], "constant")
+        near(plain, want["infer"], "band-pair kernel")
 
 
 @pytest.mark.gpu
@@ -319,7 +328,7 @@ def test_bf16_table_partial_gradients_layouts(dtype):
     near(dt, want["dtable"], "table alone")
     both = torch.cat([q, k, v], 2).transpose(0, 1).contiguous().transpose(0, 1)
     assert not both[..., :64].is_contiguous()
-    near(ops.rel_bias_attention(both[..., :64], both[..., 64:128], both[..., 128:], table, 2, max_distance=40), want["out"], "slices")
+    near(ops.rel_bias_attention(both[..., :64], both[..., 64:128], both[..., 128:], table, 2, max_distance=40), want["infer"], "slices")
     ones = torch.ones(1, 1, 64, dtype=dtype, device="cuda").expand(2, 150, 64)
     got = call(q, k, v, table, ones, n_heads=2, max_distance=40)
     want = oracle(q, k, v, table, 2, 32 ** -0.5, 40, None, ones)

@@ -5,6 +5,7 @@
 struct RelK {
   const void *q, *k, *v;       // [N][L][C], head h in columns h*hd .. h*hd+hd-1
   void* out;                   // [N][L][C]
+  void* rest;                  // [N][L][C] or null (bf16 with a backward pass): what rounding took from out
   float* lse;                  // [N][nh][L] or null; log2 domain: p = exp2(s*scale_log2 + bias - lse); +inf: nothing to see
   const void* dout;            // [N][L][C]
   float* delta;                // [N][nh][L]: <dO, O> of a row and head

@@ -15,7 +15,8 @@
 // fixed order: no atomics, the same bits every time.
 //
 // At [32, 1024, 1024], 8 heads of 128 (69 GFLOP a product; a large matrix product of this card runs at 1247 TFLOP/s):
-// forward 0.18 ms, delta 0.02, dQ 0.27, dK and dV 0.34, table 0.015: 0.75 to 0.79 PFLOP/s in each walk.  Two waves a SIMD share
+// forward 0.18 ms for inference and 0.235 in front of a backward pass, delta 0.03, dQ 0.27, dK and dV 0.34, table 0.015: 0.75 to
+// 0.88 PFLOP/s in each walk.  Two waves a SIMD share
 // the matrix pipe (busy 35 to 38 % of the cycles) and the vector pipe (42 %, exponentials and conversions first); neither
 // is full, what is left is one wave waiting for its own scores between the two products.
 #include "attn_tiles.h"
@@ -66,7 +67,15 @@ template <int HDP, int ROWS> struct RowLoader {
   }
 };
 
-template <int HDP>
+// What rounding to bf16 took from registers 8s..8s+7: x = pack8 + rest8 to 2^-16
+__device__ __forceinline__ bf16x8 rest8(const f32x16& x, int s, const bf16x8& rounded) {
+  bf16x8 o;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) o[j] = (__bf16)(x[8 * s + j] - (float)rounded[j]);
+  return o;
+}
+
+template <int HDP, bool FINE>
 __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_fwd_kernel(const RelK p) {
   typedef Cfg<HDP> G;
   extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][K tile | V tile], biases
@@ -209,6 +218,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         for (int g = 0; g < 4; ++g) {
           const int t = g >> 1, s = g & 1, tn = (g + 1) >> 1, sn = (g + 1) & 1;
           const bf16x8 pb = pack8(st[t], s);
+          bf16x8 pl;
+          if constexpr (FINE) pl = rest8(st[t], s, pb);
           if (g < 3) load_v(g + 1, (g + 1) & 1);
 #pragma unroll
           for (int d = 0; d < G::DT; ++d) {
@@ -217,6 +228,10 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 #pragma unroll
               for (int x = d * 8 / G::DT; x < (d + 1) * 8 / G::DT; ++x) exp_one(tn, 8 * sn + x);
             }
+          }
+          if constexpr (FINE) {
+#pragma unroll
+            for (int d = 0; d < G::DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv[g & 1][d], pl, acc[d], 0, 0, 0);
           }
         }
         __builtin_amdgcn_s_setprio(0);
@@ -250,10 +265,15 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       for (int e4 = 0; e4 < 4; ++e4) {
         const int dd = 32 * d + 8 * e4 + 4 * h;
         if (dd < p.hd) {
-          bf16x4 o;
+          bf16x4 o, rest;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = (__bf16)(inv == 0.f ? 0.f : acc[d][4 * e4 + e] * inv);
+          for (int e = 0; e < 4; ++e) {
+            const float x = inv == 0.f ? 0.f : acc[d][4 * e4 + e] * inv;
+            o[e] = (__bf16)x;
+            rest[e] = (__bf16)(x - (float)o[e]);
+          }
           *reinterpret_cast<bf16x4*>(op + dd) = o;
+          if (p.rest) *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.rest) + base + (long long)qrow * p.c + dd) = rest;
         }
       }
   }
@@ -274,12 +294,14 @@ __global__ __launch_bounds__(AT_THREADS) void rel_attn_rowdot_kernel(const RelK 
     if (row >= p.l) break;                         // wave-uniform
     const __bf16* dop = static_cast<const __bf16*>(p.dout) + ((long long)n * p.l + row) * p.c;
     const __bf16* op = static_cast<const __bf16*>(p.out) + ((long long)n * p.l + row) * p.c;
+    const __bf16* rp = static_cast<const __bf16*>(p.rest) + ((long long)n * p.l + row) * p.c;
     for (int ch = lane; ch < chunks; ch += 64) {
       const bf16x8 a = *reinterpret_cast<const bf16x8*>(dop + ch * 8);
       const bf16x8 b = *reinterpret_cast<const bf16x8*>(op + ch * 8);
+      const bf16x8 b2 = *reinterpret_cast<const bf16x8*>(rp + ch * 8);
       float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf((float)a[e], (float)b[e], s);
+      for (int e = 0; e < 8; ++e) s = fmaf((float)a[e], (float)b[e] + (float)b2[e], s);
       part[wave][ch] = s;
     }
     __builtin_amdgcn_wave_barrier();
@@ -306,7 +328,7 @@ __global__ __launch_bounds__(AT_THREADS) void rel_attn_rowdot_kernel(const RelK 
 constexpr int BW_ROWS = 32;                         // rows of a streamed tile
 constexpr int DG_ZERO = 36, DG_PITCH = DG_ZERO + 32, DG_WORDS = 33 * DG_PITCH;
 
-template <int HDP>
+template <int HDP, bool FINE>
 __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_dq_kernel(const RelK p) {
   typedef Cfg<HDP> G;
   constexpr int TILE = BW_ROWS * G::ROWB;
@@ -459,6 +481,11 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int d = 0; d < G::DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ft[g][d], db, acc[d], 0, 0, 0);
+        if constexpr (FINE) {
+          const bf16x8 dl = rest8(st, g, db);
+#pragma unroll
+          for (int d = 0; d < G::DT; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ft[g][d], dl, acc[d], 0, 0, 0);
+        }
       }
     };
     const Runs runs = rel_runs<BW_ROWS>(kb_lo, kb_hi, q0w, p.sat);
@@ -512,7 +539,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 // ---------------------------------------------------------------------------------------------
 constexpr int KV_KEYS = 128;
 
-template <int HDP>
+template <int HDP, bool FINE>
 __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_dkv_kernel(const RelK p) {
   typedef Cfg<HDP> G;
   constexpr int TILE = BW_ROWS * G::ROWB;
@@ -644,6 +671,10 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         __builtin_amdgcn_sched_barrier(0);
         dva[d0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(td[b & 1], pb, dva[d0], 0, 0, 0);
         dka[d0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tq[b & 1], db, dka[d0], 0, 0, 0);
+        if constexpr (FINE) {
+          dva[d0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(td[b & 1], rest8(st, s, pb), dva[d0], 0, 0, 0);
+          dka[d0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tq[b & 1], rest8(dp, s, db), dka[d0], 0, 0, 0);
+        }
       }
       if (qb + 1 < qb_hi && tid < 2 * BW_ROWS) stats[(buf ^ 1) * 2 * BW_ROWS + tid] = stat_next;
       buf ^= 1;
@@ -711,15 +742,25 @@ __global__ __launch_bounds__(AT_THREADS) void rel_attn_dtable_kernel(const RelK 
   }
 }
 
-#define REL_INSTANTIATE(HDP)                                     \
-  template __global__ void rel_attn_fwd_kernel<HDP>(const RelK); \
-  template __global__ void rel_attn_dq_kernel<HDP>(const RelK);  \
-  template __global__ void rel_attn_dkv_kernel<HDP>(const RelK);
-REL_INSTANTIATE(32)
-REL_INSTANTIATE(64)
-REL_INSTANTIATE(128)
-REL_INSTANTIATE(256)
+#define REL_INSTANTIATE(HDP, FINE)                                     \
+  template __global__ void rel_attn_fwd_kernel<HDP, FINE>(const RelK); \
+  template __global__ void rel_attn_dkv_kernel<HDP, FINE>(const RelK);
+REL_INSTANTIATE(32, false)
+REL_INSTANTIATE(64, false)
+REL_INSTANTIATE(128, false)
+REL_INSTANTIATE(256, false)
+REL_INSTANTIATE(32, true)
+REL_INSTANTIATE(64, true)
+REL_INSTANTIATE(128, true)
+REL_INSTANTIATE(256, true)
 #undef REL_INSTANTIATE
+template __global__ void rel_attn_dq_kernel<32, true>(const RelK);
+template __global__ void rel_attn_dq_kernel<64, false>(const RelK);
+template __global__ void rel_attn_dq_kernel<64, true>(const RelK);
+template __global__ void rel_attn_dq_kernel<128, false>(const RelK);
+template __global__ void rel_attn_dq_kernel<128, true>(const RelK);
+template __global__ void rel_attn_dq_kernel<256, false>(const RelK);
+template __global__ void rel_attn_dq_kernel<256, true>(const RelK);
 
 size_t bias_bytes(int sat, int copies) { return (size_t)rel_width(sat) * sizeof(float) * copies; }
 
@@ -731,26 +772,53 @@ template <typename K> int set_lds(K kernel, size_t bytes, const char* what) {
   return 0;
 }
 
-template <int HDP> int launch_fwd(const RelK& p, hipStream_t st) {
+template <int HDP, bool FINE> int launch_fwd(const RelK& p, hipStream_t st) {
   const size_t lds = 4 * (size_t)Cfg<HDP>::TILE + bias_bytes(p.sat, 1);
-  if (set_lds(&rel_attn_fwd_kernel<HDP>, lds, "rel_attn_fwd")) return -1;
-  hipLaunchKernelGGL(rel_attn_fwd_kernel<HDP>, dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ))), dim3(AT_THREADS), lds, st, p);
+  if (set_lds(&rel_attn_fwd_kernel<HDP, FINE>, lds, "rel_attn_fwd")) return -1;
+  hipLaunchKernelGGL((rel_attn_fwd_kernel<HDP, FINE>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ))), dim3(AT_THREADS), lds, st, p);
   UNET_LAUNCH_CHECK("rel_attn_fwd");
   return 0;
 }
 
-template <int HDP> int launch_bwd(const RelK& p, hipStream_t st) {
-  constexpr size_t tiles = 4 * (size_t)BW_ROWS * Cfg<HDP>::ROWB;
-  const size_t lds_q = tiles + bias_bytes(p.sat, 1) + (p.part ? bias_bytes(p.sat, 4) + 4 * DG_WORDS * sizeof(float) : 0);
-  const size_t lds_kv = tiles + KV_KEYS * Cfg<HDP>::ROWB + 4 * BW_ROWS * sizeof(float) + bias_bytes(p.sat, 1);
-  if (set_lds(&rel_attn_dq_kernel<HDP>, lds_q, "rel_attn_bwd (dq)") || set_lds(&rel_attn_dkv_kernel<HDP>, lds_kv, "rel_attn_bwd (dk, dv)"))
-    return -1;
-  hipLaunchKernelGGL(rel_attn_dq_kernel<HDP>, dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ))), dim3(AT_THREADS), lds_q, st, p);
+template <int HDP, bool FINE> int launch_dq(const RelK& p, hipStream_t st) {
+  const size_t lds = 4 * (size_t)BW_ROWS * Cfg<HDP>::ROWB + bias_bytes(p.sat, 1) +
+                     (p.part ? bias_bytes(p.sat, 4) + 4 * DG_WORDS * sizeof(float) : 0);
+  constexpr bool F = FINE || HDP <= 32;
+  if (set_lds(&rel_attn_dq_kernel<HDP, F>, lds, "rel_attn_bwd (dq)")) return -1;
+  hipLaunchKernelGGL((rel_attn_dq_kernel<HDP, F>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ))), dim3(AT_THREADS), lds, st, p);
   UNET_LAUNCH_CHECK("rel_attn_bwd (dq)");
-  hipLaunchKernelGGL(rel_attn_dkv_kernel<HDP>, dim3((unsigned)(p.n * p.nh * cdiv(p.l, KV_KEYS))), dim3(AT_THREADS), lds_kv, st, p);
+  return 0;
+}
+
+template <int HDP, bool FINE> int launch_dkv(const RelK& p, hipStream_t st) {
+  const size_t lds = (4 * (size_t)BW_ROWS + KV_KEYS) * Cfg<HDP>::ROWB + 4 * BW_ROWS * sizeof(float) + bias_bytes(p.sat, 1);
+  if (set_lds(&rel_attn_dkv_kernel<HDP, FINE>, lds, "rel_attn_bwd (dk, dv)")) return -1;
+  hipLaunchKernelGGL((rel_attn_dkv_kernel<HDP, FINE>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, KV_KEYS))), dim3(AT_THREADS), lds, st, p);
   UNET_LAUNCH_CHECK("rel_attn_bwd (dk, dv)");
   return 0;
 }
+
+// Where P and dS are carried to 16 bits (FINE: the rounded value and its rest, two matrix products).  Rounded to bf16 once, their
+// error is that of one more rounding of the result: 1.41 times the error of the final rounding alone, averaged over many rows.
+//  - Forward in front of a backward pass: delta = <dO, O> must match the fp32 P that backward recomputes, or dP - delta loses its
+//    leading digits where one key dominates (dQ, dK and the table's gradient had up to 7 times the error of a 32-bit form).
+//    [32, 1024, 1024]: forward 176 -> 235 us, of a training pass of 0.86 ms; at [32, 1024], 8 heads of 32, 66 -> 92.
+//  - Windows of one row tile, whose few rows average nothing: [32, 128], 8 heads of 128, forward 12.1 -> 12.6 us, backward 76 us
+//    either way.
+//  - dQ of heads up to 32, where the sum of dS K cancels most (1.6 times at heads of 8): backward of [32, 1024], 8 heads of 32,
+//    246 -> 265 us.  dK and dV do not need it (1.41 there too).
+bool one_tile(const RelK& p) { return p.l <= AT_BQ; }
+
+#define REL_DISPATCH(fn, fine, p, st)                                              \
+  do {                                                                             \
+    if ((p).hd <= 32) return (fine) ? fn<32, true>(p, st) : fn<32, false>(p, st);    \
+    if ((p).hd <= 64) return (fine) ? fn<64, true>(p, st) : fn<64, false>(p, st);    \
+    if ((p).hd <= 128) return (fine) ? fn<128, true>(p, st) : fn<128, false>(p, st); \
+    return (fine) ? fn<256, true>(p, st) : fn<256, false>(p, st);                    \
+  } while (0)
+int launch_fwd_bf16(const RelK& p, hipStream_t st) { REL_DISPATCH(launch_fwd, p.lse || one_tile(p), p, st); }
+int launch_dq_bf16(const RelK& p, hipStream_t st) { REL_DISPATCH(launch_dq, p.hd <= 32 || one_tile(p), p, st); }
+int launch_dkv_bf16(const RelK& p, hipStream_t st) { REL_DISPATCH(launch_dkv, one_tile(p), p, st); }
 
 // argument checks shared by the entry points; fills everything of RelK but the tensors
 int make_rel(const char* what, RelK& p, int32_t dtype, int32_t n, int32_t l, int32_t c, int32_t nh, float scale, const void* table,
@@ -792,18 +860,16 @@ int rel_parts(int dtype, int n, int l) { return n * cdiv(l, dtype == UNET_BF16 ?
 
 extern "C" int unet_rel_attn_fwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
                                  int32_t buckets, const int32_t* starts_host, const int32_t* lengths, int32_t n, int32_t l, int32_t c,
-                                 int32_t n_heads, float scale, void* out, float* lse, void* stream) {
+                                 int32_t n_heads, float scale, void* out, void* out_rest, float* lse, void* stream) {
   RelK p = {};
   UNET_REQUIRE(q && k && v && out, "rel_attn_fwd: null pointer");
+  UNET_REQUIRE(dtype != UNET_BF16 || !lse == !out_rest, "rel_attn_fwd: a bf16 backward pass needs lse and out_rest, inference neither");
   if (make_rel("rel_attn_fwd", p, dtype, n, l, c, n_heads, scale, table, table_f32, buckets, starts_host, lengths)) return -1;
-  UNET_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out), "rel_attn_fwd: pointers must be 16-byte aligned");
-  p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse;
+  UNET_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_rest), "rel_attn_fwd: pointers must be 16-byte aligned");
+  p.q = q; p.k = k; p.v = v; p.out = out; p.rest = out_rest; p.lse = lse;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == UNET_F32) return unet_rel_attn_fwd_f32(p, st);
-  if (p.hd <= 32) return launch_fwd<32>(p, st);
-  if (p.hd <= 64) return launch_fwd<64>(p, st);
-  if (p.hd <= 128) return launch_fwd<128>(p, st);
-  return launch_fwd<256>(p, st);
+  return launch_fwd_bf16(p, st);
 }
 
 extern "C" size_t unet_rel_attn_bwd_partials(int32_t dtype, int32_t n, int32_t l, int32_t n_heads, int32_t last_start) {
@@ -812,16 +878,18 @@ extern "C" size_t unet_rel_attn_bwd_partials(int32_t dtype, int32_t n, int32_t l
 }
 
 extern "C" int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
-                                 int32_t buckets, const int32_t* starts_host, const int32_t* lengths, const void* out, const float* lse,
-                                 const void* dout, int32_t n, int32_t l, int32_t c, int32_t n_heads, float scale, void* dq, void* dk,
+                                 int32_t buckets, const int32_t* starts_host, const int32_t* lengths, const void* out, const void* out_rest,
+                                 const float* lse, const void* dout, int32_t n, int32_t l, int32_t c, int32_t n_heads, float scale, void* dq, void* dk,
                                  void* dv, void* dtable, float* partials, float* delta, void* stream) {
   RelK p = {};
   UNET_REQUIRE(q && k && v && out && lse && dout && dq && dk && dv && delta, "rel_attn_bwd: null pointer");
+  UNET_REQUIRE(dtype != UNET_BF16 || out_rest, "rel_attn_bwd: null pointer (out_rest)");
   UNET_REQUIRE(!dtable || partials, "rel_attn_bwd: the table's gradient needs the partial sums");
   if (make_rel("rel_attn_bwd", p, dtype, n, l, c, n_heads, scale, table, table_f32, buckets, starts_host, lengths)) return -1;
-  UNET_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(dout) && aligned16(dq) && aligned16(dk) &&
+  UNET_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_rest) && aligned16(dout) && aligned16(dq) && aligned16(dk) &&
                    aligned16(dv), "rel_attn_bwd: pointers must be 16-byte aligned");
-  p.q = q; p.k = k; p.v = v; p.out = const_cast<void*>(out); p.lse = const_cast<float*>(lse); p.dout = dout;
+  p.q = q; p.k = k; p.v = v; p.out = const_cast<void*>(out); p.rest = const_cast<void*>(out_rest);
+  p.lse = const_cast<float*>(lse); p.dout = dout;
   p.dq = dq; p.dk = dk; p.dv = dv; p.delta = delta; p.part = dtable ? partials : nullptr; p.parts = rel_parts(dtype, n, l);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
@@ -829,8 +897,8 @@ extern "C" int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, co
   else {
     hipLaunchKernelGGL(rel_attn_rowdot_kernel, dim3(cdiv(l, RD_ROWS), n), dim3(AT_THREADS), 0, st, p);
     UNET_LAUNCH_CHECK("rel_attn_bwd (rowdot)");
-    rc = p.hd <= 32 ? launch_bwd<32>(p, st) : p.hd <= 64 ? launch_bwd<64>(p, st) : p.hd <= 128 ? launch_bwd<128>(p, st)
-                                                                                               : launch_bwd<256>(p, st);
+    rc = launch_dq_bf16(p, st);
+    if (!rc) rc = launch_dkv_bf16(p, st);
   }
   if (rc || !dtable) return rc;
   hipLaunchKernelGGL(rel_attn_dtable_kernel, dim3(buckets, n_heads), dim3(AT_THREADS), 0, st, p, dtable);

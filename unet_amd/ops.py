@@ -1850,23 +1850,24 @@ def _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, keep: bool):
     n, l, c = q.shape
     out = torch.empty_like(q)
     lse = torch.empty((n, n_heads, l), dtype=torch.float32, device=q.device) if keep else None
+    rest = torch.empty_like(q) if keep and q.dtype == torch.bfloat16 else None          # what rounding takes from out: delta needs it
     _run("unet_rel_attn_fwd", q, _dt(q), q, k, v, table, _dt(table), table.shape[0], _starts_array(starts), lengths, n, l, c, n_heads,
-         scale, out, lse)
-    return out, lse
+         scale, out, rest, lse)
+    return out, rest, lse
 
 
 class RelBiasAttnFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, table, n_heads, scale, starts, lengths):
-        out, lse = _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, True)
-        ctx.save_for_backward(q, k, v, table, out, lse, lengths)
+        out, rest, lse = _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, True)
+        ctx.save_for_backward(q, k, v, table, out, rest, lse, lengths)
         ctx.n_heads, ctx.scale, ctx.starts = n_heads, scale, starts
         return out
 
     @staticmethod
     def backward(ctx, dout):
         _once_differentiable("rel_bias_attention")
-        q, k, v, table, out, lse, lengths = ctx.saved_tensors
+        q, k, v, table, out, rest, lse, lengths = ctx.saved_tensors
         n, l, c = q.shape
         dout = _aligned(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
@@ -1876,8 +1877,8 @@ class RelBiasAttnFn(torch.autograd.Function):
             dtable = torch.empty_like(table)
             size = int(_lib.load().unet_rel_attn_bwd_partials(_dt(q), n, l, ctx.n_heads, ctx.starts[-1]))
             partials = torch.empty(size, dtype=torch.float32, device=q.device)
-        _run("unet_rel_attn_bwd", q, _dt(q), q, k, v, table, _dt(table), table.shape[0], _starts_array(ctx.starts), lengths, out, lse,
-             dout, n, l, c, ctx.n_heads, ctx.scale, dq, dk, dv, dtable, partials, delta)
+        _run("unet_rel_attn_bwd", q, _dt(q), q, k, v, table, _dt(table), table.shape[0], _starts_array(ctx.starts), lengths, out, rest,
+             lse, dout, n, l, c, ctx.n_heads, ctx.scale, dq, dk, dv, dtable, partials, delta)
         return dq, dk, dv, dtable, None, None, None, None
 
 
@@ -1894,8 +1895,8 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
     neither keys nor queries, their outputs and gradients are zero.  A row with nothing to see gives zeros.  ``scale`` defaults
     to ``hd ** -0.5`` and must be positive.
 
-    Scores, softmax statistics and all sums are fp32; in bf16 the probabilities and dS are rounded to bf16 as operands of the
-    next product.  Differentiable (once) in q, k, v and table; the table's gradient is added up in a fixed order."""
+    Scores, softmax statistics and all sums are fp32.  In bf16 the probabilities and dS are operands of the next product: with 16
+    bits for windows of at most 128 rows, for ``out`` where gradients follow and for dq of heads up to 32, otherwise with 8.  Differentiable (once) in q, k, v and table; the table's gradient is added up in a fixed order."""
     if q.dim() != 3 or k.shape != q.shape or v.shape != q.shape:
         raise ValueError(f"rel_bias_attention: q, k, v must all be [N, L, C], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     unit = 8 if _dt(q) == _lib.BF16 else 4
