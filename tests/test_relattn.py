@@ -228,6 +228,14 @@ def test_fp32_head_sizes(hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [16, 40, 128, 256])
+def test_fp32_launches_that_fill_the_chip(hd):
+    """256 workgroups of 64 rows: the waves own different rows (in small launches they share them)."""
+    q, k, v, table, dout = inputs(4, 200, 16, hd, 16, torch.float32, seed=hd)
+    verify(q, k, v, table, dout, 16, 60, lengths=torch.tensor([200, 0, 129, 64], dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("l,lens", [(130, (0, 1, 64, 65, 130, 200, -3)), (300, (0, 129, 300, 256, 1, 40, 299))])
 def test_padded_batches(l, lens, dtype):

@@ -23,6 +23,12 @@ int unet_rel_attn_bwd_f32(const RelK& p, hipStream_t st);
 
 namespace {
 
+// Rows a workgroup of the fp32 kernels owns: 16 where workgroups of 64 would take at most half of the CUs, 64 otherwise.  Forward,
+// 64 against 16, heads of 64 at [2, 512] 39.7 and 17.2 us, [4, 512] (128 workgroups) 40.5 and 23.3, [7, 512] (224) 41.1 and 41.5; heads
+// of 128 at [2, 500] 62 and 27, [7, 510] 66 and 103.  Heads of more than 128 stay at 64: the 128 rows of the other side that a
+// workgroup of 16 takes a step would not fit the LDS.
+__host__ __forceinline__ int rel32_rows(int n, int l, int nh, int hd) { return hd <= 128 && (long long)n * nh * cdiv(l, 64) <= 128 ? 16 : 64; }
+
 constexpr float REL_LOG2E = 1.4426950408889634f;
 constexpr float REL_LOWEST = -1e30f;    // finite biases stop here (log2 domain): the type's lowest value must not become -inf
 // LDS copy of a head's biases by offset: index REL_PAD + sat + offset, flat beyond +-sat for REL_PAD entries each way, so a

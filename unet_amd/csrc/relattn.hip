@@ -854,7 +854,8 @@ int make_rel(const char* what, RelK& p, int32_t dtype, int32_t n, int32_t l, int
   return 0;
 }
 
-int rel_parts(int dtype, int n, int l) { return n * cdiv(l, dtype == UNET_BF16 ? AT_BQ : 64); }
+// rows of partial sums: one a workgroup of the dQ kernel
+int rel_parts(int dtype, int n, int l, int nh, int hd) { return n * cdiv(l, dtype == UNET_BF16 ? AT_BQ : rel32_rows(n, l, nh, hd)); }
 
 }  // namespace
 
@@ -874,7 +875,7 @@ extern "C" int unet_rel_attn_fwd(int32_t dtype, const void* q, const void* k, co
 
 extern "C" size_t unet_rel_attn_bwd_partials(int32_t dtype, int32_t n, int32_t l, int32_t n_heads, int32_t last_start) {
   if (n <= 0 || l <= 0 || n_heads <= 0 || last_start < 0) return 0;
-  return (size_t)n_heads * rel_parts(dtype, n, l) * (2 * (size_t)last_start + 1);
+  return (size_t)n_heads * rel_parts(dtype, n, l, n_heads, 1) * (2 * (size_t)last_start + 1);
 }
 
 extern "C" int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
@@ -890,7 +891,7 @@ extern "C" int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, co
                    aligned16(dv), "rel_attn_bwd: pointers must be 16-byte aligned");
   p.q = q; p.k = k; p.v = v; p.out = const_cast<void*>(out); p.rest = const_cast<void*>(out_rest);
   p.lse = const_cast<float*>(lse); p.dout = dout;
-  p.dq = dq; p.dk = dk; p.dv = dv; p.delta = delta; p.part = dtable ? partials : nullptr; p.parts = rel_parts(dtype, n, l);
+  p.dq = dq; p.dk = dk; p.dv = dv; p.delta = delta; p.part = dtable ? partials : nullptr; p.parts = rel_parts(dtype, n, l, n_heads, p.hd);
   hipStream_t st = static_cast<hipStream_t>(stream);
   int rc;
   if (dtype == UNET_F32) rc = unet_rel_attn_bwd_f32(p, st);
