@@ -481,17 +481,21 @@ int unet_clip_adamw_apply(const float* const* grads_host, int32_t n_tensors, flo
  * and gradients are zero, and what they hold is not read.  A row with nothing to see gives zeros.
  * lse: [n][n_heads][l] fp32, and in bf16 out_rest [n][l][c] bf16 (what rounding took from out), for a backward pass; both NULL when
  * none follows.  Backward: dtable may be NULL; partials:
- * unet_rel_attn_bwd_partials(...) floats; delta: scratch of lse's shape. */
+ * unet_rel_attn_bwd_partials(...) floats; delta: scratch of lse's shape.  workspace: unet_rel_attn_workspace_bytes(...) bytes (0
+ * unless few rows walk a long window), 16-byte aligned, used by this call only. */
 #define UNET_REL_MAX_DISTANCE 512
 #define UNET_REL_MAX_SIDE 128
 int unet_rel_attn_fwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
                       int32_t buckets, const int32_t* starts_host, const int32_t* lengths, int32_t n, int32_t l, int32_t c,
-                      int32_t n_heads, float scale, void* out, void* out_rest, float* lse, void* stream);
+                      int32_t n_heads, float scale, void* out, void* out_rest, float* lse, void* workspace, size_t ws_bytes,
+                      void* stream);
+size_t unet_rel_attn_workspace_bytes(int32_t dtype, int32_t n, int32_t l, int32_t c, int32_t n_heads, int32_t backward);
 size_t unet_rel_attn_bwd_partials(int32_t dtype, int32_t n, int32_t l, int32_t n_heads, int32_t last_start);
 int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
                       int32_t buckets, const int32_t* starts_host, const int32_t* lengths, const void* out, const void* out_rest,
                       const float* lse, const void* dout, int32_t n, int32_t l, int32_t c, int32_t n_heads, float scale, void* dq,
-                      void* dk, void* dv, void* dtable, float* partials, float* delta, void* stream);
+                      void* dk, void* dv, void* dtable, float* partials, float* delta, void* workspace, size_t ws_bytes,
+                      void* stream);
 
 /* AdamW with both moments in 8 bits (the fp32 form is above; train.py:1553-1559 keeps fp32 moments):
  *   m <- b1 m + (1-b1) g,  r <- sqrt(b2 r^2 + (1-b2) g^2),  p <- (1 - lr wd) p - lr/(1-b1^t) m / (r / sqrt(1-b2^t) + eps)

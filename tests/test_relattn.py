@@ -190,7 +190,7 @@ def test_refusals_on_cpu():
     st = (C.c_int32 * 2)(0, 1)
 
     def fwd(dtype=1, n=1, l=4, c=8, nh=1, scale=1.0, buckets=4, starts=st, q=16, rest=None, lse=None):
-        return lib.unet_rel_attn_fwd(dtype, q, q, q, 16, 1, buckets, starts, None, n, l, c, nh, scale, 16, rest, lse, None)
+        return lib.unet_rel_attn_fwd(dtype, q, q, q, 16, 1, buckets, starts, None, n, l, c, nh, scale, 16, rest, lse, None, 0, None)
 
     for kw, msg in ((dict(q=None), b"null"), (dict(dtype=5), b"dtype"), (dict(l=0), b"shape"), (dict(c=10), b"head_dim"), (dict(q=24), b"aligned"),
                     (dict(scale=0.0), b"scale"), (dict(scale=3e38), b"scale"), (dict(buckets=3), b"buckets"), (dict(starts=(C.c_int32 * 2)(1, 1)), b"distance 0"),
@@ -199,10 +199,17 @@ def test_refusals_on_cpu():
                     (dict(dtype=0, lse=16), b"out_rest"), (dict(dtype=0, rest=16), b"out_rest"),
                     (dict(dtype=0, lse=16, rest=24), b"aligned")):
         assert fwd(**kw) == -1 and msg in lib.unet_last_error(), (kw, lib.unet_last_error())
-    assert lib.unet_rel_attn_bwd(1, 16, 16, 16, 16, 1, 4, st, None, 16, 16, 16, 16, 1, 4, 8, 1, 1.0, 16, 16, 16, 16, None, 16, None) == -1
+    assert lib.unet_rel_attn_bwd(1, 16, 16, 16, 16, 1, 4, st, None, 16, 16, 16, 16, 1, 4, 8, 1, 1.0, 16, 16, 16, 16, None, 16, None, 0, None) == -1
     assert b"partial" in lib.unet_last_error()
-    assert lib.unet_rel_attn_bwd(0, 16, 16, 16, 16, 1, 4, st, None, 16, None, 16, 16, 1, 4, 8, 1, 1.0, 16, 16, 16, None, None, 16, None) == -1
+    assert lib.unet_rel_attn_bwd(0, 16, 16, 16, 16, 1, 4, st, None, 16, None, 16, 16, 1, 4, 8, 1, 1.0, 16, 16, 16, None, None, 16, None, 0, None) == -1
     assert b"out_rest" in lib.unet_last_error()
+    # few rows of a long window: shares of the keys need their workspace
+    need = lib.unet_rel_attn_workspace_bytes(0, 1, 4096, 8, 1, 0)
+    assert need > 0 and lib.unet_rel_attn_workspace_bytes(1, 1, 4096, 8, 1, 0) == 0
+    assert fwd(dtype=0, l=4096) == -1 and b"workspace" in lib.unet_last_error()
+    assert lib.unet_rel_attn_bwd(0, 16, 16, 16, 16, 1, 4, st, None, 16, 16, 16, 16, 1, 4096, 8, 1, 1.0, 16, 16, 16, None, None, 16, 16, 8,
+                                 None) == -1
+    assert b"workspace" in lib.unet_last_error()
 
 
 # ------------------------------------------------------------------------------------------------ GPU
@@ -233,6 +240,26 @@ def test_fp32_launches_that_fill_the_chip(hd):
     """256 workgroups of 64 rows: the waves own different rows (in small launches they share them)."""
     q, k, v, table, dout = inputs(4, 200, 16, hd, 16, torch.float32, seed=hd)
     verify(q, k, v, table, dout, 16, 60, lengths=torch.tensor([200, 0, 129, 64], dtype=torch.int32, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [8, 64, 128, 256])
+@pytest.mark.parametrize("case", ["plain", "padded", "left", "band"])
+def test_few_rows_of_a_long_window(hd, case):
+    """The walked axis is cut in shares: shares behind a window's length, outside the band, with and without gradients."""
+    from unet_amd import ops
+    l, n = 1579, 3 if case == "padded" else 1
+    q, k, v, table, dout = inputs(n, l, 2, hd, 16, torch.bfloat16, seed=hd + n)
+    lengths = torch.tensor([l, 600, 0], dtype=torch.int32, device="cuda") if case == "padded" else None
+    if case in ("left", "band"):
+        table[15] = -math.inf                      # nothing far behind the query ..
+    if case == "band":
+        table[7] = -math.inf                       # .. nor far in front of it
+    got = verify(q, k, v, table, dout, 2, 50, lengths=lengths, what=case)
+    again = call(q, k, v, table, dout, n_heads=2, max_distance=50, lengths=lengths)
+    assert all(torch.equal(got[key], again[key]) for key in got)
+    near(ops.rel_bias_attention(q, k, v, table, 2, max_distance=50, lengths=lengths),
+         oracle(q, k, v, table, 2, hd ** -0.5, 50, lengths, None)["infer"], "no gradients")
 
 
 @pytest.mark.gpu

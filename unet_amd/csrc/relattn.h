@@ -13,7 +13,9 @@ struct RelK {
   const void* table;           // [buckets][nh], fp32 or bf16
   float* part;                 // [nh][parts][2*sat+1] sums of dS by offset, one row per workgroup of the dQ kernel, or null
   const int* lengths;          // [N] valid positions, or null
-  int n, l, c, nh, hd, buckets, sat, parts, table_f32;
+  float* split;                // bf16, few rows: [splits][N][L][C] sums of a workgroup's share of the walked axis (backward: three of
+                               // them, dQ | dK | dV); behind them, forward, [splits][N][nh][L] (maximum, sum)
+  int n, l, c, nh, hd, buckets, sat, parts, table_f32, splits;
   float scale, scale_log2;
   unsigned char bucket[UNET_REL_MAX_DISTANCE + 1];   // of |offset| = 0 .. sat within its side; sat: start of the last one
 };

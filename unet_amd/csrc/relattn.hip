@@ -12,13 +12,12 @@
 //   d table[b, h] = sum of dS over the pairs of bucket b
 // is taken where dS is in registers anyway, in the dQ walk: far tiles add into one register a side, the others into a wave's
 // own LDS array by offset, one diagonal of the tile a lane.  Workgroups write their sums by offset, a last launch adds them in a
-// fixed order: no atomics, the same bits every time.
+// fixed order: no atomics, the same bits every time.  A few rows in a long window split the walked axis (rel_splits).
 //
 // At [32, 1024, 1024], 8 heads of 128 (69 GFLOP a product; a large matrix product of this card runs at 1247 TFLOP/s):
 // forward 0.18 ms for inference and 0.235 in front of a backward pass, delta 0.03, dQ 0.27, dK and dV 0.34, table 0.015: 0.75 to
-// 0.88 PFLOP/s in each walk.  Two waves a SIMD share
-// the matrix pipe (busy 35 to 38 % of the cycles) and the vector pipe (42 %, exponentials and conversions first); neither
-// is full, what is left is one wave waiting for its own scores between the two products.
+// 0.88 PFLOP/s in each walk.  Two waves a SIMD share the matrix pipe (busy 35 to 38 % of the cycles) and the vector pipe (42 %,
+// exponentials and conversions first); neither is full, what is left is one wave waiting for its own scores between the products.
 #include "attn_tiles.h"
 #include "relattn.h"
 
@@ -42,6 +41,16 @@ template <int T> __device__ __forceinline__ Runs rel_runs(int lo, int hi, int ow
 }
 typedef std::integral_constant<bool, true> Near;
 typedef std::integral_constant<bool, false> Beyond;
+
+// share `split` of the walked axis, cut in p.splits pieces of whole tiles of T rows, within [lo, hi)
+__device__ __forceinline__ void rel_share(const RelK& p, int split, int T, int& lo, int& hi) {
+  const int tiles = (p.l + T - 1) / T, per = (tiles + p.splits - 1) / p.splits;
+  lo = max(lo, split * per);
+  hi = min(hi, (split + 1) * per);
+}
+__device__ __forceinline__ float2* rel_split_stats(const RelK& p) {
+  return reinterpret_cast<float2*>(p.split + (long long)p.splits * p.n * p.l * p.c);
+}
 
 // TileLoader of attn_tiles.h for tiles of ROWS rows (the same LDS image)
 template <int HDP, int ROWS> struct RowLoader {
@@ -87,6 +96,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
   int wg = xcd_remap(blockIdx.x, gridDim.x);
   const int nqt = (p.l + AT_BQ - 1) / AT_BQ;
   const int qt = wg % nqt; wg /= nqt;
+  const int split = wg % p.splits; wg /= p.splits;
   const int head = wg % p.nh;
   const int n = wg / p.nh;
   const int len = rel_length(p, n);
@@ -104,7 +114,13 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
   float m = -INFINITY, lsum = 0.f, mtrue = -INFINITY;
 
-  if (q0 < len) {                                        // (uniform over the workgroup)
+  const float cneg = rel_bias(p, head, -p.sat), cpos = rel_bias(p, head, p.sat);
+  // key tiles that any row of the workgroup can see, and of them the workgroup's share
+  const int nkb = (len + AT_BK - 1) / AT_BK;
+  int kb_lo = cneg == -INFINITY ? max(0, q0 - p.sat + 1) / AT_BK : 0;
+  int kb_hi = cpos == -INFINITY ? min(nkb, (q0 + AT_BQ - 2 + p.sat) / AT_BK + 1) : nkb;
+  rel_share(p, split, AT_BK, kb_lo, kb_hi);
+  if (q0 < len && kb_lo < kb_hi) {                       // (uniform over the workgroup)
     const __bf16* q = static_cast<const __bf16*>(p.q) + base + (long long)qrow * p.c;
     bf16x8 qf[G::KS];
 #pragma unroll
@@ -119,11 +135,6 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     ld.setup(wave, lane, p.c, p.hd);
     const int a0 = row_read_base<HDP>(lane);
     const int vb0 = tr_read_base<HDP>(lane, 0), vb1 = tr_read_base<HDP>(lane, 1);
-    const float cneg = rel_bias(p, head, -p.sat), cpos = rel_bias(p, head, p.sat);
-    // key tiles that any row of the workgroup can see
-    const int nkb = (len + AT_BK - 1) / AT_BK;
-    const int kb_lo = cneg == -INFINITY ? max(0, q0 - p.sat + 1) / AT_BK : 0;
-    const int kb_hi = cpos == -INFINITY ? min(nkb, (q0 + AT_BQ - 2 + p.sat) / AT_BK + 1) : nkb;
     const Runs runs = rel_runs<AT_BK>(kb_lo, kb_hi, q0 + wave * 32, p.sat);
     const unsigned tile_step = (unsigned)AT_BK * p.c * 2;
     auto issue = [&](int kb, int buf) {
@@ -254,6 +265,21 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 
   // rows without a single visible key, and rows behind the window's length, give zeros
   const float lt = lsum + __shfl_xor(lsum, 32, 64);
+  if (p.splits > 1) {                                    // rel_attn_join_fwd_kernel puts the shares together
+    const long long slab = (long long)split * p.n + n;
+    if (row_ok) {
+      if (h == 0) rel_split_stats(p)[(slab * p.nh + head) * p.l + qrow] = make_float2(m, lt);
+      float* sp = p.split + (slab * p.l + qrow) * p.c + hoff;
+#pragma unroll
+      for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int dd = 32 * d + 8 * e4 + 4 * h;
+          if (dd < p.hd) *reinterpret_cast<f32x4*>(sp + dd) = f32x4{acc[d][4 * e4], acc[d][4 * e4 + 1], acc[d][4 * e4 + 2], acc[d][4 * e4 + 3]};
+        }
+    }
+    return;
+  }
   const bool seen = row_ok && lt > 0.f;
   const bool spoiled = row_ok && lt != lt;
   const float inv = seen ? 1.f / lt : spoiled ? lt : 0.f;
@@ -277,6 +303,57 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         }
       }
   }
+}
+
+// The shares of a forward pass split over the keys: out = sum_s acc_s 2^(m_s - m) / sum_s l_s 2^(m_s - m).  Four channels a thread.
+__global__ __launch_bounds__(AT_THREADS) void rel_attn_join_fwd_kernel(const RelK p) {
+  const int c4 = p.c >> 2;
+  const long long i = (long long)blockIdx.x * AT_THREADS + threadIdx.x;
+  const long long at = i / c4;                           // window and row
+  if (at >= (long long)p.n * p.l) return;
+  const int n = (int)(at / p.l), row = (int)(at - (long long)n * p.l), ch = (int)(i - at * c4) * 4, head = ch / p.hd;
+  const float2* ml = rel_split_stats(p) + ((long long)n * p.nh + head) * p.l + row;
+  const long long step = (long long)p.n * p.nh * p.l;
+  const bool row_ok = row < rel_length(p, n);
+  float m = -INFINITY, lt = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (row_ok) {
+    for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ml[s * step].x);
+    for (int s = 0; s < p.splits; ++s) {
+      const float2 a = ml[s * step];
+      const float f = a.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.x - m);
+      lt = fmaf(a.y, f, lt);
+      acc += *reinterpret_cast<const f32x4*>(p.split + ((long long)s * p.n * p.l + at) * p.c + ch) * f;
+    }
+  }
+  const bool seen = lt > 0.f, spoiled = lt != lt;
+  const float inv = seen ? 1.f / lt : spoiled ? lt : 0.f;
+  if (p.lse && ch == head * p.hd) p.lse[((long long)n * p.nh + head) * p.l + row] = seen ? m + __builtin_amdgcn_logf(lt) : spoiled ? lt : INFINITY;
+  bf16x4 o, rest;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float x = inv == 0.f ? 0.f : acc[e] * inv;
+    o[e] = (__bf16)x;
+    rest[e] = (__bf16)(x - (float)o[e]);
+  }
+  *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.out) + at * p.c + ch) = o;
+  if (p.rest) *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(p.rest) + at * p.c + ch) = rest;
+}
+
+// The shares of a backward pass: dQ and dK (times scale), dV.  Four channels a thread, blockIdx.y the tensor.
+__global__ __launch_bounds__(AT_THREADS) void rel_attn_join_bwd_kernel(const RelK p) {
+  const long long total = (long long)p.n * p.l * p.c, i = ((long long)blockIdx.x * AT_THREADS + threadIdx.x) * 4;
+  if (i >= total) return;
+  const int which = blockIdx.y;
+  const float* src = p.split + (long long)which * p.splits * total + i;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < p.splits; ++s) acc += *reinterpret_cast<const f32x4*>(src + s * total);
+  if (which < 2) acc *= p.scale;
+  bf16x4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = (__bf16)acc[e];
+  void* dst = which == 0 ? p.dq : which == 1 ? p.dk : p.dv;
+  *reinterpret_cast<bf16x4*>(static_cast<__bf16*>(dst) + i) = o;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -344,6 +421,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
   int wg = xcd_remap(blockIdx.x, gridDim.x);
   const int nqt = (p.l + AT_BQ - 1) / AT_BQ;
   const int qt = wg % nqt; wg /= nqt;
+  const int split = wg % p.splits; wg /= p.splits;
   const int head = wg % p.nh;
   const int n = wg / p.nh;
   const int len = rel_length(p, n);
@@ -362,7 +440,12 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
   }
   float fneg = 0.f, fpos = 0.f;
 
-  if (q0 < len) {
+  const float cneg = rel_bias(p, head, -p.sat), cpos = rel_bias(p, head, p.sat);
+  const int nkb = (len + BW_ROWS - 1) / BW_ROWS;
+  int kb_lo = cneg == -INFINITY ? max(0, q0 - p.sat + 1) / BW_ROWS : 0;
+  int kb_hi = cpos == -INFINITY ? min(nkb, (q0 + AT_BQ - 2 + p.sat) / BW_ROWS + 1) : nkb;
+  rel_share(p, split, BW_ROWS, kb_lo, kb_hi);
+  if (q0 < len && kb_lo < kb_hi) {
     const __bf16* qp = static_cast<const __bf16*>(p.q) + base + (long long)qrow * p.c;
     const __bf16* dp_ = static_cast<const __bf16*>(p.dout) + base + (long long)qrow * p.c;
     bf16x8 qf[G::KS], dof[G::KS];
@@ -385,10 +468,6 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     const __bf16* vbase = static_cast<const __bf16*>(p.v) + base;
     const int a0 = row_read_base<HDP>(lane);
     const int vb0 = tr_read_base<HDP>(lane, 0), vb1 = tr_read_base<HDP>(lane, 1);
-    const float cneg = rel_bias(p, head, -p.sat), cpos = rel_bias(p, head, p.sat);
-    const int nkb = (len + BW_ROWS - 1) / BW_ROWS;
-    const int kb_lo = cneg == -INFINITY ? max(0, q0 - p.sat + 1) / BW_ROWS : 0;
-    const int kb_hi = cpos == -INFINITY ? min(nkb, (q0 + AT_BQ - 2 + p.sat) / BW_ROWS + 1) : nkb;
     auto issue = [&](int kb, int buf) {
       char* at = smem + buf * 2 * TILE;
       ld.issue(kbase, len, p.c, p.hd, at, (unsigned)kb * BW_ROWS, wave);
@@ -495,7 +574,19 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     for (; kb < kb_hi; ++kb) tile(kb, Beyond{}, cpos, fpos);
   }
 
-  if (qrow < p.l) {
+  if (p.splits > 1 && qrow < p.l) {
+    float* sp = p.split + (((long long)split * p.n + n) * p.l + qrow) * p.c + head * p.hd;
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int dd = 32 * d + 8 * e4 + 4 * h;
+        f32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = row_ok ? acc[d][4 * e4 + e] : 0.f;
+        if (dd < p.hd) *reinterpret_cast<f32x4*>(sp + dd) = o;
+      }
+  } else if (qrow < p.l) {
     __bf16* yp = static_cast<__bf16*>(p.dq) + base + (long long)qrow * p.c;
 #pragma unroll
     for (int d = 0; d < G::DT; ++d)
@@ -519,7 +610,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       sums[wave * w + w - 1] += fpos;
     }
     __syncthreads();
-    float* row = p.part + ((long long)head * p.parts + n * nqt + qt) * (2 * p.sat + 1);
+    float* row = p.part + ((long long)head * p.parts + (n * nqt + qt) * p.splits + split) * (2 * p.sat + 1);
     for (int i = tid; i < 2 * p.sat + 1; i += AT_THREADS) {
       float s = 0.f;
       const int lo = i == 0 ? 0 : i + REL_PAD, hi = i == 2 * p.sat ? w - 1 : i + REL_PAD;      // the flat ends belong to +-sat
@@ -554,6 +645,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
   int wg = xcd_remap(blockIdx.x, gridDim.x);
   const int nkt = (p.l + KV_KEYS - 1) / KV_KEYS;
   const int ktl = wg % nkt; wg /= nkt;
+  const int split = wg % p.splits; wg /= p.splits;
   const int head = wg % p.nh;
   const int n = wg / p.nh;
   const int len = rel_length(p, n);
@@ -567,7 +659,13 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 #pragma unroll
     for (int e = 0; e < 16; ++e) { dka[d][e] = 0.f; dva[d][e] = 0.f; }
 
-  if (key0 < len) {
+  const float cneg = rel_bias(p, head, -p.sat), cpos = rel_bias(p, head, p.sat);
+  // row tiles that can see any of the keys: row - key < sat if the left side is closed, key - row < sat if the right one is
+  const int nqb = (len + BW_ROWS - 1) / BW_ROWS;
+  int qb_lo = cpos == -INFINITY ? max(0, key0 - p.sat + 1) / BW_ROWS : 0;
+  int qb_hi = cneg == -INFINITY ? min(nqb, (key0 + KV_KEYS - 2 + p.sat) / BW_ROWS + 1) : nqb;
+  rel_share(p, split, BW_ROWS, qb_lo, qb_hi);
+  if (key0 < len && qb_lo < qb_hi) {
     const __bf16* vp = static_cast<const __bf16*>(p.v) + base + (long long)key * p.c;
     bf16x8 vf[G::KS];
 #pragma unroll
@@ -590,11 +688,6 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     const int a0 = row_read_base<HDP>(lane);
     const char* const kw = krows + wave * 32 * G::ROWB;
     const int vb0 = tr_read_base<HDP>(lane, 0), vb1 = tr_read_base<HDP>(lane, 1);
-    const float cneg = rel_bias(p, head, -p.sat), cpos = rel_bias(p, head, p.sat);
-    // row tiles that can see any of the keys: row - key < sat if the left side is closed, key - row < sat if the right one is
-    const int nqb = (len + BW_ROWS - 1) / BW_ROWS;
-    const int qb_lo = cpos == -INFINITY ? max(0, key0 - p.sat + 1) / BW_ROWS : 0;
-    const int qb_hi = cneg == -INFINITY ? min(nqb, (key0 + KV_KEYS - 2 + p.sat) / BW_ROWS + 1) : nqb;
     auto issue = [&](int qb, int buf) {
       char* at = smem + buf * 2 * TILE;
       ld.issue(qbase, len, p.c, p.hd, at, (unsigned)qb * BW_ROWS, wave);
@@ -686,7 +779,27 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     for (; qb < qb_hi; ++qb) tile(qb, Beyond{}, cneg);
   }
 
-  if (key < p.l) {
+  if (p.splits > 1 && key < p.l) {
+    const long long total = (long long)p.n * p.l * p.c;
+    float* sk = p.split + (p.splits + split) * total + base + (long long)key * p.c;
+    float* sv = sk + p.splits * total;
+#pragma unroll
+    for (int d = 0; d < G::DT; ++d)
+#pragma unroll
+      for (int e4 = 0; e4 < 4; ++e4) {
+        const int dd = 32 * d + 8 * e4 + 4 * h;
+        f32x4 ok, ov;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          ok[e] = key_ok ? dka[d][4 * e4 + e] : 0.f;
+          ov[e] = key_ok ? dva[d][4 * e4 + e] : 0.f;
+        }
+        if (dd < p.hd) {
+          *reinterpret_cast<f32x4*>(sk + dd) = ok;
+          *reinterpret_cast<f32x4*>(sv + dd) = ov;
+        }
+      }
+  } else if (key < p.l) {
     __bf16* dk = static_cast<__bf16*>(p.dk) + base + (long long)key * p.c;
     __bf16* dv = static_cast<__bf16*>(p.dv) + base + (long long)key * p.c;
 #pragma unroll
@@ -775,7 +888,7 @@ template <typename K> int set_lds(K kernel, size_t bytes, const char* what) {
 template <int HDP, bool FINE> int launch_fwd(const RelK& p, hipStream_t st) {
   const size_t lds = 4 * (size_t)Cfg<HDP>::TILE + bias_bytes(p.sat, 1);
   if (set_lds(&rel_attn_fwd_kernel<HDP, FINE>, lds, "rel_attn_fwd")) return -1;
-  hipLaunchKernelGGL((rel_attn_fwd_kernel<HDP, FINE>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ))), dim3(AT_THREADS), lds, st, p);
+  hipLaunchKernelGGL((rel_attn_fwd_kernel<HDP, FINE>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ) * p.splits)), dim3(AT_THREADS), lds, st, p);
   UNET_LAUNCH_CHECK("rel_attn_fwd");
   return 0;
 }
@@ -785,7 +898,7 @@ template <int HDP, bool FINE> int launch_dq(const RelK& p, hipStream_t st) {
                      (p.part ? bias_bytes(p.sat, 4) + 4 * DG_WORDS * sizeof(float) : 0);
   constexpr bool F = FINE || HDP <= 32;
   if (set_lds(&rel_attn_dq_kernel<HDP, F>, lds, "rel_attn_bwd (dq)")) return -1;
-  hipLaunchKernelGGL((rel_attn_dq_kernel<HDP, F>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ))), dim3(AT_THREADS), lds, st, p);
+  hipLaunchKernelGGL((rel_attn_dq_kernel<HDP, F>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, AT_BQ) * p.splits)), dim3(AT_THREADS), lds, st, p);
   UNET_LAUNCH_CHECK("rel_attn_bwd (dq)");
   return 0;
 }
@@ -793,7 +906,7 @@ template <int HDP, bool FINE> int launch_dq(const RelK& p, hipStream_t st) {
 template <int HDP, bool FINE> int launch_dkv(const RelK& p, hipStream_t st) {
   const size_t lds = (4 * (size_t)BW_ROWS + KV_KEYS) * Cfg<HDP>::ROWB + 4 * BW_ROWS * sizeof(float) + bias_bytes(p.sat, 1);
   if (set_lds(&rel_attn_dkv_kernel<HDP, FINE>, lds, "rel_attn_bwd (dk, dv)")) return -1;
-  hipLaunchKernelGGL((rel_attn_dkv_kernel<HDP, FINE>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, KV_KEYS))), dim3(AT_THREADS), lds, st, p);
+  hipLaunchKernelGGL((rel_attn_dkv_kernel<HDP, FINE>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, KV_KEYS) * p.splits)), dim3(AT_THREADS), lds, st, p);
   UNET_LAUNCH_CHECK("rel_attn_bwd (dk, dv)");
   return 0;
 }
@@ -820,6 +933,18 @@ int launch_fwd_bf16(const RelK& p, hipStream_t st) { REL_DISPATCH(launch_fwd, p.
 int launch_dq_bf16(const RelK& p, hipStream_t st) { REL_DISPATCH(launch_dq, p.hd <= 32 || one_tile(p), p, st); }
 int launch_dkv_bf16(const RelK& p, hipStream_t st) { REL_DISPATCH(launch_dkv, one_tile(p), p, st); }
 
+// Few rows in a long window: workgroups of 128 rows would leave CUs idle while each walks the whole window.  The walked axis is
+// then cut into shares of at least 512 rows, up to two workgroups a CU, and a further launch adds up their fp32 sums.  Unsplit
+// against split, one window, 2 heads, forward and backward of a training pass: [2048] heads of 128 51 and 28, 154 and 85 us; heads of
+// 256 92 and 42, 271 and 120; [8192] heads of 64 121 and 68, 444 and 186.  [1024] gains nothing (22 and 24, 82 and 88), and
+// shares of 256 are no faster.
+int rel_splits(int dtype, int n, int l, int nh) {
+  const long long wgs = (long long)n * nh * cdiv(l, AT_BQ);
+  if (dtype != UNET_BF16 || wgs > 128) return 1;
+  const int most = l / 512, want = (int)(512 / wgs);
+  return most < 3 ? 1 : want < most ? want : most;
+}
+
 // argument checks shared by the entry points; fills everything of RelK but the tensors
 int make_rel(const char* what, RelK& p, int32_t dtype, int32_t n, int32_t l, int32_t c, int32_t nh, float scale, const void* table,
              int32_t table_f32, int32_t buckets, const int32_t* starts_host, const int32_t* lengths) {
@@ -844,6 +969,7 @@ int make_rel(const char* what, RelK& p, int32_t dtype, int32_t n, int32_t l, int
   const int sat = starts_host[side - 1];
   UNET_REQUIRE(sat >= 1 && sat <= UNET_REL_MAX_DISTANCE, "%s: the last bucket must start at distance 1 .. %d, got %d", what,
                UNET_REL_MAX_DISTANCE, sat);
+  p.splits = rel_splits(dtype, n, l, nh);
   p.n = n; p.l = l; p.c = c; p.nh = nh; p.hd = c / nh; p.buckets = buckets; p.sat = sat;
   p.table = table; p.table_f32 = table_f32; p.lengths = lengths;
   p.scale = scale; p.scale_log2 = scale * REL_LOG2E;
@@ -854,14 +980,29 @@ int make_rel(const char* what, RelK& p, int32_t dtype, int32_t n, int32_t l, int
   return 0;
 }
 
+size_t workspace_bytes(int splits, int n, int l, int c, int nh, int backward) {
+  if (splits < 2) return 0;
+  const size_t rows = (size_t)splits * n * l;
+  return rows * (backward ? 3 * (size_t)c : (size_t)c + 2 * (size_t)nh) * sizeof(float);
+}
+int take_workspace(const char* what, RelK& p, void* workspace, size_t bytes, int backward) {
+  const size_t need = workspace_bytes(p.splits, p.n, p.l, p.c, p.nh, backward);
+  UNET_REQUIRE(workspace && bytes >= need && aligned16(workspace), "%s: workspace of %zu bytes, %zu needed (16-byte aligned)", what, bytes, need);
+  p.split = static_cast<float*>(workspace);
+  return 0;
+}
+
 // rows of partial sums: one a workgroup of the dQ kernel
-int rel_parts(int dtype, int n, int l, int nh, int hd) { return n * cdiv(l, dtype == UNET_BF16 ? AT_BQ : rel32_rows(n, l, nh, hd)); }
+int rel_parts(int dtype, int n, int l, int nh, int hd) {
+  return dtype == UNET_BF16 ? n * cdiv(l, AT_BQ) * rel_splits(dtype, n, l, nh) : n * cdiv(l, rel32_rows(n, l, nh, hd));
+}
 
 }  // namespace
 
 extern "C" int unet_rel_attn_fwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
                                  int32_t buckets, const int32_t* starts_host, const int32_t* lengths, int32_t n, int32_t l, int32_t c,
-                                 int32_t n_heads, float scale, void* out, void* out_rest, float* lse, void* stream) {
+                                 int32_t n_heads, float scale, void* out, void* out_rest, float* lse, void* workspace,
+                                 size_t ws_bytes, void* stream) {
   RelK p = {};
   UNET_REQUIRE(q && k && v && out, "rel_attn_fwd: null pointer");
   UNET_REQUIRE(dtype != UNET_BF16 || !lse == !out_rest, "rel_attn_fwd: a bf16 backward pass needs lse and out_rest, inference neither");
@@ -870,7 +1011,17 @@ extern "C" int unet_rel_attn_fwd(int32_t dtype, const void* q, const void* k, co
   p.q = q; p.k = k; p.v = v; p.out = out; p.rest = out_rest; p.lse = lse;
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == UNET_F32) return unet_rel_attn_fwd_f32(p, st);
-  return launch_fwd_bf16(p, st);
+  if (p.splits == 1) return launch_fwd_bf16(p, st);
+  if (take_workspace("rel_attn_fwd", p, workspace, ws_bytes, 0) || launch_fwd_bf16(p, st)) return -1;
+  hipLaunchKernelGGL(rel_attn_join_fwd_kernel, dim3((unsigned)(((long long)n * l * (c / 4) + AT_THREADS - 1) / AT_THREADS)),
+                     dim3(AT_THREADS), 0, st, p);
+  UNET_LAUNCH_CHECK("rel_attn_fwd (join)");
+  return 0;
+}
+
+extern "C" size_t unet_rel_attn_workspace_bytes(int32_t dtype, int32_t n, int32_t l, int32_t c, int32_t n_heads, int32_t backward) {
+  if (n <= 0 || l <= 0 || c <= 0 || n_heads <= 0) return 0;
+  return workspace_bytes(rel_splits(dtype, n, l, n_heads), n, l, c, n_heads, backward);
 }
 
 extern "C" size_t unet_rel_attn_bwd_partials(int32_t dtype, int32_t n, int32_t l, int32_t n_heads, int32_t last_start) {
@@ -881,7 +1032,8 @@ extern "C" size_t unet_rel_attn_bwd_partials(int32_t dtype, int32_t n, int32_t l
 extern "C" int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, const void* v, const void* table, int32_t table_f32,
                                  int32_t buckets, const int32_t* starts_host, const int32_t* lengths, const void* out, const void* out_rest,
                                  const float* lse, const void* dout, int32_t n, int32_t l, int32_t c, int32_t n_heads, float scale, void* dq, void* dk,
-                                 void* dv, void* dtable, float* partials, float* delta, void* stream) {
+                                 void* dv, void* dtable, float* partials, float* delta, void* workspace, size_t ws_bytes,
+                                 void* stream) {
   RelK p = {};
   UNET_REQUIRE(q && k && v && out && lse && dout && dq && dk && dv && delta, "rel_attn_bwd: null pointer");
   UNET_REQUIRE(dtype != UNET_BF16 || out_rest, "rel_attn_bwd: null pointer (out_rest)");
@@ -896,10 +1048,16 @@ extern "C" int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, co
   int rc;
   if (dtype == UNET_F32) rc = unet_rel_attn_bwd_f32(p, st);
   else {
+    if (p.splits > 1 && take_workspace("rel_attn_bwd", p, workspace, ws_bytes, 1)) return -1;
     hipLaunchKernelGGL(rel_attn_rowdot_kernel, dim3(cdiv(l, RD_ROWS), n), dim3(AT_THREADS), 0, st, p);
     UNET_LAUNCH_CHECK("rel_attn_bwd (rowdot)");
     rc = launch_dq_bf16(p, st);
     if (!rc) rc = launch_dkv_bf16(p, st);
+    if (!rc && p.splits > 1) {
+      hipLaunchKernelGGL(rel_attn_join_bwd_kernel, dim3((unsigned)(((long long)n * l * (c / 4) + AT_THREADS - 1) / AT_THREADS), 3),
+                         dim3(AT_THREADS), 0, st, p);
+      UNET_LAUNCH_CHECK("rel_attn_bwd (join)");
+    }
   }
   if (rc || !dtable) return rc;
   hipLaunchKernelGGL(rel_attn_dtable_kernel, dim3(buckets, n_heads), dim3(AT_THREADS), 0, st, p, dtable);

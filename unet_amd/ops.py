@@ -1846,13 +1846,23 @@ def _starts_array(starts: Tuple[int, ...]):
     return (C.c_int32 * len(starts))(*starts)
 
 
+@functools.lru_cache(maxsize=4096)
+def _rel_sizes(dt: int, n: int, l: int, c: int, n_heads: int, last_start: int):
+    """Bytes of the forward and backward workspaces, floats of the table's partial sums."""
+    lib = _lib.load()
+    return (*(int(lib.unet_rel_attn_workspace_bytes(dt, n, l, c, n_heads, b)) for b in (0, 1)),
+            int(lib.unet_rel_attn_bwd_partials(dt, n, l, n_heads, last_start)))
+
+
 def _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, keep: bool):
     n, l, c = q.shape
     out = torch.empty_like(q)
     lse = torch.empty((n, n_heads, l), dtype=torch.float32, device=q.device) if keep else None
     rest = torch.empty_like(q) if keep and q.dtype == torch.bfloat16 else None          # what rounding takes from out: delta needs it
+    size = _rel_sizes(_dt(q), n, l, c, n_heads, starts[-1])[0]
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     _run("unet_rel_attn_fwd", q, _dt(q), q, k, v, table, _dt(table), table.shape[0], _starts_array(starts), lengths, n, l, c, n_heads,
-         scale, out, rest, lse)
+         scale, out, rest, lse, ws, size)
     return out, rest, lse
 
 
@@ -1872,13 +1882,14 @@ class RelBiasAttnFn(torch.autograd.Function):
         dout = _aligned(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
         delta = torch.empty_like(lse)
+        _, size, floats = _rel_sizes(_dt(q), n, l, c, ctx.n_heads, ctx.starts[-1])
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         dtable = partials = None
         if ctx.needs_input_grad[3]:
             dtable = torch.empty_like(table)
-            size = int(_lib.load().unet_rel_attn_bwd_partials(_dt(q), n, l, ctx.n_heads, ctx.starts[-1]))
-            partials = torch.empty(size, dtype=torch.float32, device=q.device)
+            partials = torch.empty(floats, dtype=torch.float32, device=q.device)
         _run("unet_rel_attn_bwd", q, _dt(q), q, k, v, table, _dt(table), table.shape[0], _starts_array(ctx.starts), lengths, out, rest,
-             lse, dout, n, l, c, ctx.n_heads, ctx.scale, dq, dk, dv, dtable, partials, delta)
+             lse, dout, n, l, c, ctx.n_heads, ctx.scale, dq, dk, dv, dtable, partials, delta, ws, size)
         return dq, dk, dv, dtable, None, None, None, None
 
 
