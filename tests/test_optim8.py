@@ -355,3 +355,28 @@ def test_thawed_tensors_and_switched_state_bits():
         # the moments are rounded to codes once on the way in and once when the step stores them
         assert float((m1 - BETAS[0] * m).abs().max()) <= 2 * 2.0 ** -4 * float(m.abs().max())
         assert float((v1.sqrt() - (BETAS[1] * v).sqrt()).abs().max()) <= 2 * 2.0 ** -4 * float(v.max().sqrt())
+
+
+@pytest.mark.gpu
+def test_checkpoint_files(tmp_path):
+    """8-bit state through a checkpoint file, read without unpickling anything but tensors: the next step has the same bits."""
+    from unet_amd.checkpoint import load_checkpoint, save_checkpoint
+    from unet_amd.optim import ClipAdamW
+    torch.manual_seed(0)
+    nets = [torch.nn.Linear(90, 77).cuda() for _ in range(2)]
+    opts = [ClipAdamW(net.parameters(), lr=1e-2, betas=BETAS, state_bits=8, max_grad_norm=1.0) for net in nets]
+    gen = torch.Generator().manual_seed(8)
+    for _ in range(2):
+        set_grads(list(nets[0].parameters()), gen, 1.0)
+        opts[0].step()
+    save_checkpoint(nets[0], opts[0], 2, tmp_path / "c.pt")
+    load_checkpoint(tmp_path / "c.pt", nets[1], optimizer=opts[1])
+    set_grads(list(nets[0].parameters()), gen, 1.0)
+    for p, q in zip(nets[0].parameters(), nets[1].parameters()):
+        q.grad = p.grad.clone()
+    for opt in opts:
+        opt.step()
+    for p, q in zip(nets[0].parameters(), nets[1].parameters()):
+        assert torch.equal(p, q)
+        for k, t in opts[0].state[p].items():
+            assert torch.equal(t.float(), opts[1].state[q][k].float()), k

@@ -457,3 +457,26 @@ def test_second_derivatives_are_refused():
     out = ops.rel_bias_attention(q, k, v, table, 2)
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(out, q, dout, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_slabs_just_below_two_gib():
+    """[131071, 8192] bf16: byte offsets up to 2^31; a local band, so that rows at the end have an oracle of their own."""
+    from unet_amd import ops
+    l, nh, hd = 131071, 32, 256
+    gen = torch.Generator(device="cuda").manual_seed(23)
+    q, k, v, dout = (torch.randn(1, l, nh * hd, generator=gen, device="cuda", dtype=torch.bfloat16) for _ in range(4))
+    table = torch.randn(8, nh, generator=gen, device="cuda")
+    table[3] = table[7] = -math.inf                                    # nothing at distance 4 and beyond
+    got = call(q, k, v, table, dout, n_heads=nh, max_distance=4)
+    del got["dtable"]
+    cols, rows = slice(-hd, None), slice(l - 300, None)
+    part = [t[:, rows, cols].contiguous() for t in (q, k, v)]
+    want = oracle(*part, table[:, -1:], 1, hd ** -0.5, 4, None, dout[:, rows, cols].contiguous())
+    for key in got:
+        value, bound = want[key]
+        near(got[key][:, rows, cols][:, 10:], (value[:, 10:], bound[:, 10:]), key)
+    first = oracle(*(t[:, :300, :hd].contiguous() for t in (q, k, v)), table[:, :1], 1, hd ** -0.5, 4, None, dout[:, :300, :hd].contiguous())
+    for key in got:
+        value, bound = first[key]
+        near(got[key][:, :290, :hd], (value[:, :290], bound[:, :290]), key)
