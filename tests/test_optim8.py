@@ -59,6 +59,11 @@ def test_refusals_on_cpu():
     assert len(opt.param_groups) == 1
     with pytest.raises(TypeError, match="fp32"):
         ClipAdamW([torch.nn.Parameter(torch.zeros(5000, dtype=torch.bfloat16))], state_bits=8).moment_buffers()
+    from unet_amd.optim import _dense_fp32
+    dense = torch.zeros(3, 4)
+    assert _dense_fp32([dense, None]) and _dense_fp32([None]) and _dense_fp32([])
+    for bad in (dense.to_sparse(), dense.to_sparse_csr(), dense.t(), dense.bfloat16()):
+        assert not _dense_fp32([dense, bad])
     lib = _lib.load()
     assert lib.unet_adamw8_apply(None, 1, None, None, None, None, 1, None, None, None, None, None, None, None, None, None, 0.9, 0.9,
                                  1e-8, 0.0, None) == -1 and b"null" in lib.unet_last_error()
