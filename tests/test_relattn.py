@@ -480,3 +480,19 @@ def test_slabs_just_below_two_gib():
     for key in got:
         value, bound = first[key]
         near(got[key][:, :290, :hd], (value[:, :290], bound[:, :290]), key)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("l", [300, 1600])
+def test_scores_that_grow_along_the_window(hd, l):
+    """Keys whose scores rise by hundreds behind the first tile, in some rows only, and rows that see nothing for many tiles: the
+    running reference has to move, also inside a share of the keys."""
+    q, k, v, table, dout = inputs(1, l, 2, hd, 16, torch.bfloat16, seed=hd + l)
+    ramp = torch.linspace(0, 1, l, device="cuda")[None, :, None]
+    k = (k * (0.1 + 12 * ramp)).to(k.dtype)
+    q = q.clone()
+    q[:, ::3] *= 4
+    verify(q, k, v, table, dout, 2, 50, what="growing")
+    table[:8] = -math.inf                          # only keys behind the query: the last rows see nothing in front of them
+    verify(q, k, v, table, dout, 2, 50, what="growing, keys behind")
