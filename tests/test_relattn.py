@@ -496,3 +496,43 @@ def test_scores_that_grow_along_the_window(hd, l):
     verify(q, k, v, table, dout, 2, 50, what="growing")
     table[:8] = -math.inf                          # only keys behind the query: the last rows see nothing in front of them
     verify(q, k, v, table, dout, 2, 50, what="growing, keys behind")
+
+
+@pytest.mark.gpu
+def test_shared_axis_in_two_graphs_at_once():
+    """Windows long enough to be cut in shares: forward and backward captured twice, replayed in turn and on two streams."""
+    from unet_amd import ops
+    sets, graphs, outs = [], [], []
+    for i in range(2):
+        q, k, v, table, dout = inputs(1, 1600 + 70 * i, 2, 32, 16, torch.bfloat16, seed=31 + i)
+        leaves = [t.requires_grad_() for t in (q, k, v, table)]
+        sets.append((leaves, dout))
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            torch.autograd.grad(ops.rel_bias_attention(*leaves, 2, max_distance=40), leaves, dout)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.rel_bias_attention(*leaves, 2, max_distance=40)
+            outs.append((out.detach(),) + torch.autograd.grad(out, leaves, dout))
+            del out
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for rep in range(4):
+        with torch.no_grad():
+            for leaves, _ in sets:
+                leaves[0].mul_(0.9)
+                leaves[3].add_(0.1)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            if rep % 2:
+                with torch.cuda.stream(s):
+                    graph.replay()
+            else:
+                graph.replay()
+        torch.cuda.synchronize()
+        for (leaves, dout), got in zip(sets, outs):
+            out = ops.rel_bias_attention(*leaves, 2, max_distance=40)
+            want = (out.detach(),) + torch.autograd.grad(out, leaves, dout)
+            del out
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), rep
