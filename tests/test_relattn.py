@@ -235,6 +235,13 @@ def test_fp32_head_sizes(hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_most_heads_and_channels(dtype):
+    q, k, v, table, dout = inputs(1, 33, 256, 64, 16, dtype, seed=24)
+    verify(q, k, v, table, dout, 256, 60)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("hd", [16, 40, 128, 256])
 def test_fp32_launches_that_fill_the_chip(hd):
     """256 workgroups of 64 rows: the waves own different rows (in small launches they share them)."""

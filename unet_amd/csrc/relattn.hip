@@ -15,7 +15,7 @@
 // fixed order: no atomics, the same bits every time.  A few rows in a long window split the walked axis (rel_splits).
 //
 // At [32, 1024, 1024], 8 heads of 128 (69 GFLOP a product; a large matrix product of this card runs at 1247 TFLOP/s):
-// forward 0.18 ms for inference and 0.235 in front of a backward pass, delta 0.03, dQ 0.27, dK and dV 0.34, table 0.015: 0.75 to
+// forward 0.18 ms for inference and 0.235 in front of a backward pass, dQ 0.29, dK and dV 0.34, table 0.015: 0.7 to
 // 0.88 PFLOP/s in each walk.  Two waves a SIMD share the matrix pipe (busy 35 to 38 % of the cycles) and the vector pipe (42 %,
 // exponentials and conversions first); neither is full, what is left is one wave waiting for its own scores between the products.
 #include "attn_tiles.h"
@@ -41,6 +41,22 @@ template <int T> __device__ __forceinline__ Runs rel_runs(int lo, int hi, int ow
 }
 typedef std::integral_constant<bool, true> Near;
 typedef std::integral_constant<bool, false> Beyond;
+
+// A lane's fragments of its own row of a [L][C] slab, from `t` at element `row` (a row that exists; zeros unless `ok`).  No branches:
+// all loads leave at once.
+template <int HDP> __device__ __forceinline__ void own_row(bf16x8 (&f)[Cfg<HDP>::KS], const void* t, long long row, bool ok, int h, int hd) {
+#pragma unroll
+  for (int s = 0; s < Cfg<HDP>::KS; ++s) {
+    const int ch = (2 * s + h) * 8;
+    f[s] = *reinterpret_cast<const bf16x8*>(static_cast<const __bf16*>(t) + row + (ch < hd ? ch : 0));
+  }
+#pragma unroll
+  for (int s = 0; s < Cfg<HDP>::KS; ++s) {
+    const bool in = ok && (2 * s + h) * 8 < hd;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[s][e] = in ? f[s][e] : (__bf16)0.f;
+  }
+}
 
 // share `split` of the walked axis, cut in p.splits pieces of whole tiles of T rows, within [lo, hi)
 __device__ __forceinline__ void rel_share(const RelK& p, int split, int T, int& lo, int& hi) {
@@ -121,16 +137,6 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
   int kb_hi = cpos == -INFINITY ? min(nkb, (q0 + AT_BQ - 2 + p.sat) / AT_BK + 1) : nkb;
   rel_share(p, split, AT_BK, kb_lo, kb_hi);
   if (q0 < len && kb_lo < kb_hi) {                       // (uniform over the workgroup)
-    const __bf16* q = static_cast<const __bf16*>(p.q) + base + (long long)qrow * p.c;
-    bf16x8 qf[G::KS];
-#pragma unroll
-    for (int s = 0; s < G::KS; ++s) {
-      const int ch = 2 * s + h;
-      bf16x8 z;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = (__bf16)0.f;
-      qf[s] = (row_ok && ch * 8 < p.hd) ? *reinterpret_cast<const bf16x8*>(q + ch * 8) : z;
-    }
     TileLoader<HDP> ld;
     ld.setup(wave, lane, p.c, p.hd);
     const int a0 = row_read_base<HDP>(lane);
@@ -143,6 +149,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       ld.issue(static_cast<const __bf16*>(p.v), base, len, p.c, p.hd, at + G::TILE, (unsigned)kb * tile_step, wave);
     };
     issue(kb_lo, 0);
+    bf16x8 qf[G::KS];
+    own_row<HDP>(qf, p.q, base + (long long)min(qrow, len - 1) * p.c, row_ok, h, p.hd);
     rel_fill(p, head, bias, tid, AT_THREADS);
     // m: the row maximum of the first tile with anything to see, then fixed (scores up to 2^32 above it stay inside fp32);
     // a row that exceeds the margin sends the workgroup through a second walk with the true maxima
@@ -357,45 +365,8 @@ __global__ __launch_bounds__(AT_THREADS) void rel_attn_join_bwd_kernel(const Rel
 }
 
 // ---------------------------------------------------------------------------------------------
-// backward 1/4: delta = <dO, O> of every row and head.  One wave a row, HBM-bound.
-// ---------------------------------------------------------------------------------------------
-constexpr int RD_ROWS = 16, RD_CHUNKS = 1024;
-
-__global__ __launch_bounds__(AT_THREADS) void rel_attn_rowdot_kernel(const RelK p) {
-  __shared__ float part[4][RD_CHUNKS];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = blockIdx.y, len = rel_length(p, n);
-  const int chunks = p.c >> 3, cph = p.hd >> 3;
-  for (int rr = 0; rr < RD_ROWS / 4; ++rr) {
-    const int row = blockIdx.x * RD_ROWS + wave * (RD_ROWS / 4) + rr;
-    if (row >= p.l) break;                         // wave-uniform
-    const __bf16* dop = static_cast<const __bf16*>(p.dout) + ((long long)n * p.l + row) * p.c;
-    const __bf16* op = static_cast<const __bf16*>(p.out) + ((long long)n * p.l + row) * p.c;
-    const __bf16* rp = static_cast<const __bf16*>(p.rest) + ((long long)n * p.l + row) * p.c;
-    for (int ch = lane; ch < chunks; ch += 64) {
-      const bf16x8 a = *reinterpret_cast<const bf16x8*>(dop + ch * 8);
-      const bf16x8 b = *reinterpret_cast<const bf16x8*>(op + ch * 8);
-      const bf16x8 b2 = *reinterpret_cast<const bf16x8*>(rp + ch * 8);
-      float s = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) s = fmaf((float)a[e], (float)b[e] + (float)b2[e], s);
-      part[wave][ch] = s;
-    }
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_s_waitcnt(0xc07f);            // lgkmcnt(0): the wave's own LDS writes are visible to its lanes
-    for (int head = lane; head < p.nh; head += 64) {
-      float s = 0.f;
-      for (int k = 0; k < cph; ++k) s += part[wave][head * cph + k];
-      p.delta[((long long)n * p.nh + head) * p.l + row] = row < len ? s : 0.f;
-    }
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_s_waitcnt(0xc07f);
-  }
-}
-
-// ---------------------------------------------------------------------------------------------
-// backward 2/4: dQ = scale dS K, and the sums of dS by offset.  Steps of 32 keys: 16 scores and 16 dP a lane, so that everything
-// fits the 256 registers of two workgroups a CU.
+// backward 1/3: delta = <dO, O> (dO is in registers here; dK and dV read it), dQ = scale dS K, and the sums of dS by offset.  Steps of
+// 32 keys: 16 scores and 16 dP a lane, so that everything fits the 256 registers of two workgroups a CU.
 //
 // Sums by offset inside the band: a wave's [32 rows][32 keys] of dS go to its own LDS array with a row pitch of 68 words, 36 of
 // them zero; lane d then adds the 32 words of diagonal d (stride 69) and keeps the sum with one read and one write.  Words outside
@@ -445,23 +416,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
   int kb_lo = cneg == -INFINITY ? max(0, q0 - p.sat + 1) / BW_ROWS : 0;
   int kb_hi = cpos == -INFINITY ? min(nkb, (q0 + AT_BQ - 2 + p.sat) / BW_ROWS + 1) : nkb;
   rel_share(p, split, BW_ROWS, kb_lo, kb_hi);
-  if (q0 < len && kb_lo < kb_hi) {
-    const __bf16* qp = static_cast<const __bf16*>(p.q) + base + (long long)qrow * p.c;
-    const __bf16* dp_ = static_cast<const __bf16*>(p.dout) + base + (long long)qrow * p.c;
-    bf16x8 qf[G::KS], dof[G::KS];
-#pragma unroll
-    for (int s = 0; s < G::KS; ++s) {
-      const int ch = 2 * s + h;
-      bf16x8 z;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = (__bf16)0.f;
-      const bool ok = row_ok && ch * 8 < p.hd;
-      qf[s] = ok ? *reinterpret_cast<const bf16x8*>(qp + ch * 8) : z;
-      dof[s] = ok ? *reinterpret_cast<const bf16x8*>(dp_ + ch * 8) : z;
-    }
-    const long long si = ((long long)n * p.nh + head) * p.l + qrow;
-    const float lse = row_ok ? p.lse[si] : INFINITY;
-    const float delta = row_ok ? p.delta[si] : 0.f;
+  const bool walks = kb_lo < kb_hi;
+  if (q0 < len && (walks || split == 0)) {
     RowLoader<HDP, BW_ROWS> ld;
     ld.setup(wave, lane, p.c, p.hd);
     const __bf16* kbase = static_cast<const __bf16*>(p.k) + base;
@@ -473,7 +429,21 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       ld.issue(kbase, len, p.c, p.hd, at, (unsigned)kb * BW_ROWS, wave);
       ld.issue(vbase, len, p.c, p.hd, at + TILE, (unsigned)kb * BW_ROWS, wave);
     };
-    issue(kb_lo, 0);
+    if (walks) issue(kb_lo, 0);
+    bf16x8 qf[G::KS], dof[G::KS], of[G::KS], rest[G::KS];
+    const long long at = base + (long long)min(qrow, len - 1) * p.c, si = ((long long)n * p.nh + head) * p.l + min(qrow, len - 1);
+    own_row<HDP>(dof, p.dout, at, row_ok, h, p.hd);
+    own_row<HDP>(of, p.out, at, row_ok, h, p.hd);
+    own_row<HDP>(rest, p.rest, at, row_ok, h, p.hd);
+    own_row<HDP>(qf, p.q, at, row_ok, h, p.hd);
+    const float stat = p.lse[si], lse = row_ok ? stat : INFINITY;
+    float delta = 0.f;
+#pragma unroll
+    for (int s = 0; s < G::KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) delta = fmaf((float)dof[s][e], (float)of[s][e] + (float)rest[s][e], delta);
+    delta += __shfl_xor(delta, 32, 64);
+    if (split == 0 && h == 0 && row_ok) p.delta[si] = delta;
     rel_fill(p, head, bias, tid, AT_THREADS);
     float* const dg = diag + wave * DG_WORDS;
     int buf = 0;
@@ -623,7 +593,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 }
 
 // ---------------------------------------------------------------------------------------------
-// backward 3/4: dK = scale dS^T Q, dV = P^T dO.  A workgroup owns 128 keys, 32 a wave, and walks the query rows 32 at a time (Q and
+// backward 2/3: dK = scale dS^T Q, dV = P^T dO.  A workgroup owns 128 keys, 32 a wave, and walks the query rows 32 at a time (Q and
 // dO tiles, double-buffered).  X = Q K^T has the key on the lane and the rows in the registers, so P and dS are the next products'
 // B operands as they stand: dV^T += dO^T P, dK^T += Q^T dS (transposed reads of the tiles).  The accumulators take 128 registers
 // at head size 128; the keys' K rows are read from LDS, their V rows stay in registers, and two workgroups fit a CU.
@@ -666,16 +636,6 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
   int qb_hi = cneg == -INFINITY ? min(nqb, (key0 + KV_KEYS - 2 + p.sat) / BW_ROWS + 1) : nqb;
   rel_share(p, split, BW_ROWS, qb_lo, qb_hi);
   if (key0 < len && qb_lo < qb_hi) {
-    const __bf16* vp = static_cast<const __bf16*>(p.v) + base + (long long)key * p.c;
-    bf16x8 vf[G::KS];
-#pragma unroll
-    for (int s = 0; s < G::KS; ++s) {
-      const int ch = 2 * s + h;
-      bf16x8 z;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = (__bf16)0.f;
-      vf[s] = key_ok && ch * 8 < p.hd ? *reinterpret_cast<const bf16x8*>(vp + ch * 8) : z;
-    }
     {
       RowLoader<HDP, KV_KEYS> lk;
       lk.setup(wave, lane, p.c, p.hd);
@@ -701,6 +661,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       return v;
     };
     issue(qb_lo, 0);
+    bf16x8 vf[G::KS];
+    own_row<HDP>(vf, p.v, base + (long long)min(key, len - 1) * p.c, key_ok, h, p.hd);
     rel_fill(p, head, bias, tid, AT_THREADS);
     if (tid < 2 * BW_ROWS) stats[tid] = load_stat(qb_lo);
     int buf = 0;
@@ -822,7 +784,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 }
 
 // ---------------------------------------------------------------------------------------------
-// backward 4/4: d table[b][head] = the sums of dS over the offsets of bucket b, added up over the dQ kernel's workgroups
+// backward 3/3: d table[b][head] = the sums of dS over the offsets of bucket b, added up over the dQ kernel's workgroups
 // ---------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(AT_THREADS) void rel_attn_dtable_kernel(const RelK p, void* dtable) {
   __shared__ int range[2];
@@ -952,9 +914,8 @@ int make_rel(const char* what, RelK& p, int32_t dtype, int32_t n, int32_t l, int
   UNET_REQUIRE(table && starts_host, "%s: null pointer", what);
   UNET_REQUIRE(n > 0 && l > 0 && c > 0 && nh > 0 && nh <= 256 && n <= 65535, "%s: bad shape n=%d l=%d c=%d heads=%d", what, n, l, c, nh);
   const int unit = dtype == UNET_BF16 ? 8 : 4;
-  UNET_REQUIRE(c % nh == 0 && (c / nh) % unit == 0 && c / nh <= 256 && c <= 8 * RD_CHUNKS,
-               "%s: head_dim %d must be a multiple of %d and at most 256, channels at most %d (c=%d heads=%d)", what, c / nh, unit,
-               8 * RD_CHUNKS, c, nh);
+  UNET_REQUIRE(c % nh == 0 && (c / nh) % unit == 0 && c / nh <= 256,
+               "%s: head_dim %d must be a multiple of %d and at most 256 (c=%d heads=%d)", what, c / nh, unit, c, nh);
   UNET_REQUIRE((long long)l * c * (dtype == UNET_BF16 ? 2 : 4) < (1ll << 31), "%s: one [L, C] slab of %lld bytes exceeds a buffer descriptor",
                what, (long long)l * c * (dtype == UNET_BF16 ? 2 : 4));
   UNET_REQUIRE((long long)n * nh * cdiv(l, 32) < (1ll << 31), "%s: grid too large", what);
@@ -1049,8 +1010,6 @@ extern "C" int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, co
   if (dtype == UNET_F32) rc = unet_rel_attn_bwd_f32(p, st);
   else {
     if (p.splits > 1 && take_workspace("rel_attn_bwd", p, workspace, ws_bytes, 1)) return -1;
-    hipLaunchKernelGGL(rel_attn_rowdot_kernel, dim3(cdiv(l, RD_ROWS), n), dim3(AT_THREADS), 0, st, p);
-    UNET_LAUNCH_CHECK("rel_attn_bwd (rowdot)");
     rc = launch_dq_bf16(p, st);
     if (!rc) rc = launch_dkv_bf16(p, st);
     if (!rc && p.splits > 1) {

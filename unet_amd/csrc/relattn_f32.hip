@@ -155,21 +155,6 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_fwd_kernel(const RelK p)
   }
 }
 
-__global__ __launch_bounds__(A32_THREADS) void rel32_rowdot_kernel(const RelK p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = blockIdx.y, len = rel_length(p, n), row = blockIdx.x * 4 + wave;
-  if (row >= p.l) return;
-  const float* dop = static_cast<const float*>(p.dout) + ((long long)n * p.l + row) * p.c;
-  const float* op = static_cast<const float*>(p.out) + ((long long)n * p.l + row) * p.c;
-  for (int head = 0; head < p.nh; ++head) {
-    float acc = 0.f;
-    if (row < len)
-      for (int d = lane; d < p.hd; d += 64) acc = fmaf(dop[head * p.hd + d], op[head * p.hd + d], acc);
-    acc = wave_sum(acc);
-    if (lane == 0) p.delta[((long long)n * p.nh + head) * p.l + row] = acc;
-  }
-}
-
 template <int HDP, bool SPLIT>
 __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dq_kernel(const RelK p) {
   constexpr int LD = HDP + 4, DT = HDP / 16, ROWS = Shape<SPLIT>::ROWS, STEP = Shape<SPLIT>::STEP;
@@ -196,7 +181,17 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dq_kernel(const RelK p) 
     for (int i = tid; i < 4 * w; i += A32_THREADS) sums[i] = 0.f;
   auto add = [](float* at, float v) { __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); };
   const float lse = row_ok ? p.lse[o.stat + qrow] : INFINITY;          // rows past the end: p = 0
-  const float delta = row_ok ? p.delta[o.stat + qrow] : 0.f;
+  float delta = 0.f;                                                   // <dO, O>, kept for dK and dV
+  {
+    f32x4 oreg[DT];
+    load_rows<HDP>(oreg, static_cast<const float*>(p.out) + o.base + (long long)qrow * p.c, row_ok, g, p.hd);
+#pragma unroll
+    for (int u = 0; u < DT; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) delta = fmaf(doreg[u][e], oreg[u][e], delta);
+    delta = group_sum(delta);
+    if (g == 0 && row_ok && (!SPLIT || wave == 0)) p.delta[o.stat + qrow] = delta;
+  }
   float fneg = 0.f, fpos = 0.f;                          // sums beyond the band
   const int end = o.tile * ROWS < o.len ? o.len : 0;
   Fetch<HDP, STEP> fk, fv;
@@ -396,7 +391,5 @@ template <int HDP, bool SPLIT> int launch_bwd32(const RelK& p, hipStream_t st) {
 int unet_rel_attn_fwd_f32(const RelK& p, hipStream_t st) { REL32_DISPATCH(launch_fwd32, p, st); }
 
 int unet_rel_attn_bwd_f32(const RelK& p, hipStream_t st) {
-  hipLaunchKernelGGL(rel32_rowdot_kernel, dim3(cdiv(p.l, 4), p.n), dim3(A32_THREADS), 0, st, p);
-  UNET_LAUNCH_CHECK("rel_attn_bwd (fp32 rowdot)");
   REL32_DISPATCH(launch_bwd32, p, st);
 }

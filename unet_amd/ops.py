@@ -1914,9 +1914,9 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
     if k.dtype != q.dtype or v.dtype != q.dtype or any(t.device != q.device for t in (k, v, table)):
         raise TypeError("rel_bias_attention: q, k and v must have one dtype and all tensors one device")
     n, l, c = q.shape
-    if n_heads < 1 or n_heads > 256 or c % n_heads or (c // n_heads) % unit or c // n_heads > 256 or not 0 < c <= 8192:
+    if n_heads < 1 or n_heads > 256 or c % n_heads or (c // n_heads) % unit or c // n_heads > 256 or c < 1:
         raise ValueError(f"rel_bias_attention: {c} channels in {n_heads} heads: the head size must be a multiple of {unit} for {q.dtype} "
-                         "and at most 256 (at most 256 heads and 8192 channels)")
+                         "and at most 256 (at most 256 heads)")
     if table.dim() != 2 or table.shape[1] != n_heads:
         raise ValueError(f"rel_bias_attention: the table must be [n_buckets, {n_heads}], got {tuple(table.shape)}")
     _dt(table)
