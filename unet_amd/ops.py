@@ -1666,12 +1666,10 @@ def band_project(bands: Tensor, wq, bq, wk, bk, wv, bv):
 # ---------------------------------------------------------------------------------------------
 # gated linear recurrence along the rows (csrc/scan.hip)
 # ---------------------------------------------------------------------------------------------
-def _run(what: str, t: Tensor, *args):
-    """Library call ``what`` on ``t``'s device and that device's current stream (its last argument).  Tensors go in as their
-    pointers; a call of a few microseconds notices every Python object made on the way."""
-    dev = t.device.index
+def _run(what: str, dev: int, *args):
+    """Library call ``what`` on device ``dev`` and its current stream (the call's last argument).  Tensors go in as their pointers:
+    a call of a few microseconds notices every Python object made on the way."""
     fn = getattr(_lib.load(), what)
-    args = [a.data_ptr() if isinstance(a, Tensor) else a for a in args]
     if dev == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
@@ -1679,6 +1677,10 @@ def _run(what: str, t: Tensor, *args):
             rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         check(rc, what)
+
+
+def _ptr(t: Optional[Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
 
 
 def _wants_grad(*tensors: Optional[Tensor]) -> bool:
@@ -1711,9 +1713,11 @@ def _check_scan(what: str, x: Tensor, gate: Tensor, state: Optional[Tensor], dim
     _need_cuda(x)
 
 
-def _scan_workspace(x: Tensor, n: int, l: int, c: int):
-    size = int(_lib.load().unet_gated_scan_workspace_bytes(_dt(x), n, l, c))
-    return (torch.empty(size, dtype=torch.uint8, device=x.device) if size else None), size
+@functools.lru_cache(maxsize=4096)
+def _scan_sizes(dt: int, n: int, l: int, c: int):
+    """Bytes of a call's workspace, and how many states the forward pass keeps for backward."""
+    lib = _lib.load()
+    return int(lib.unet_gated_scan_workspace_bytes(dt, n, l, c)), -(-l // lib.unet_gated_scan_tile())
 
 
 def _scan_forward(x: Tensor, gate: Tensor, h0: Optional[Tensor], reverse: bool, keep: bool):
@@ -1721,12 +1725,11 @@ def _scan_forward(x: Tensor, gate: Tensor, h0: Optional[Tensor], reverse: bool, 
     n, l, c = x.shape
     h = torch.empty((n, l, c), dtype=x.dtype, device=x.device)
     last = torch.empty((n, c), dtype=torch.float32, device=x.device)
-    states = None
-    if keep:
-        states = torch.empty((n, -(-l // _lib.load().unet_gated_scan_tile()), c), dtype=torch.float32, device=x.device)
-    ws, size = _scan_workspace(x, n, l, c)
-    _run("unet_gated_scan_fwd", x, _dt(x), x, x.stride(0), x.stride(1), gate, gate.stride(0), gate.stride(1), h0, reverse, n, l, c, h,
-         last, states, ws, size)
+    size, kept = _scan_sizes(_dt(x), n, l, c)
+    states = torch.empty((n, kept, c), dtype=torch.float32, device=x.device) if keep else None
+    ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    _run("unet_gated_scan_fwd", x.device.index, _dt(x), x.data_ptr(), x.stride(0), x.stride(1), gate.data_ptr(), gate.stride(0),
+         gate.stride(1), _ptr(h0), reverse, n, l, c, h.data_ptr(), last.data_ptr(), _ptr(states), _ptr(ws), size)
     return h, last, states
 
 
@@ -1754,9 +1757,11 @@ class GatedScanFn(torch.autograd.Function):
         dx = torch.empty((n, l, c), dtype=x.dtype, device=x.device)
         dg = torch.empty_like(dx)
         dh0 = torch.empty((n, c), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
-        ws, size = _scan_workspace(x, n, l, c)
-        _run("unet_gated_scan_bwd", x, _dt(x), x, x.stride(0), x.stride(1), gate, gate.stride(0), gate.stride(1), states, dh,
-             dh.stride(0), dh.stride(1), dlast, ctx.reverse, n, l, c, dx, dg, dh0, ws, size)
+        size, _ = _scan_sizes(_dt(x), n, l, c)
+        ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        _run("unet_gated_scan_bwd", x.device.index, _dt(x), x.data_ptr(), x.stride(0), x.stride(1), gate.data_ptr(), gate.stride(0),
+             gate.stride(1), states.data_ptr(), dh.data_ptr(), dh.stride(0), dh.stride(1), _ptr(dlast), ctx.reverse, n, l, c,
+             dx.data_ptr(), dg.data_ptr(), _ptr(dh0), _ptr(ws), size)
         return dx, dg, dh0, None
 
 
@@ -1797,7 +1802,8 @@ def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
     h = torch.empty((n, c), dtype=x.dtype, device=x.device)
     if h.numel():
         x, gate = _dense_channels(x), _dense_channels(gate)
-        _run("unet_gated_scan_step", x, _dt(x), x, x.stride(0), gate, gate.stride(0), state, h, n, c)
+        _run("unet_gated_scan_step", x.device.index, _dt(x), x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0),
+             state.data_ptr(), h.data_ptr(), n, c)
     return h
 
 
@@ -1861,8 +1867,9 @@ def _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, keep: bool):
     rest = torch.empty_like(q) if keep and q.dtype == torch.bfloat16 else None          # what rounding takes from out: delta needs it
     size = _rel_sizes(_dt(q), n, l, c, n_heads, starts[-1])[0]
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    _run("unet_rel_attn_fwd", q, _dt(q), q, k, v, table, _dt(table), table.shape[0], _starts_array(starts), lengths, n, l, c, n_heads,
-         scale, out, rest, lse, ws, size)
+    _run("unet_rel_attn_fwd", q.device.index, _dt(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), _dt(table),
+         table.shape[0], _starts_array(starts), _ptr(lengths), n, l, c, n_heads, scale, out.data_ptr(), _ptr(rest), _ptr(lse), _ptr(ws),
+         size)
     return out, rest, lse
 
 
@@ -1888,8 +1895,10 @@ class RelBiasAttnFn(torch.autograd.Function):
         if ctx.needs_input_grad[3]:
             dtable = torch.empty_like(table)
             partials = torch.empty(floats, dtype=torch.float32, device=q.device)
-        _run("unet_rel_attn_bwd", q, _dt(q), q, k, v, table, _dt(table), table.shape[0], _starts_array(ctx.starts), lengths, out, rest,
-             lse, dout, n, l, c, ctx.n_heads, ctx.scale, dq, dk, dv, dtable, partials, delta, ws, size)
+        _run("unet_rel_attn_bwd", q.device.index, _dt(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr(), _dt(table),
+             table.shape[0], _starts_array(ctx.starts), _ptr(lengths), out.data_ptr(), _ptr(rest), lse.data_ptr(), dout.data_ptr(), n,
+             l, c, ctx.n_heads, ctx.scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(dtable), _ptr(partials),
+             delta.data_ptr(), _ptr(ws), size)
         return dq, dk, dv, dtable, None, None, None, None
 
 
