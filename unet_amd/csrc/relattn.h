@@ -7,6 +7,7 @@ struct RelK {
   void* out;                   // [N][L][C]
   void* rest;                  // [N][L][C] or null (bf16 with a backward pass): what rounding took from out
   float* lse;                  // [N][nh][L] or null; log2 domain: p = exp2(s*scale_log2 + bias - lse); +inf: nothing to see
+                               // (fp32: [2][N][nh][L], maximum in the natural domain and log2 of the sum)
   const void* dout;            // [N][L][C]
   float* delta;                // [N][nh][L]: <dO, O> of a row and head
   void *dq, *dk, *dv;          // [N][L][C]
@@ -38,25 +39,26 @@ constexpr float REL_LOWEST = -1e30f;    // finite biases stop here (log2 domain)
 constexpr int REL_PAD = 96;
 __device__ __host__ __forceinline__ int rel_width(int sat) { return (2 * sat + 1 + 2 * REL_PAD + 3) & ~3; }      // 16-byte multiple
 
-// bias of key j seen from query i, off = j - i, in the log2 domain.  A NaN entry stays NaN; a finite one is held above
-// REL_LOWEST (the type's lowest value times log2(e) would be -inf, which means "never").
-__device__ __forceinline__ float rel_bias(const RelK& p, int head, int off) {
+// Bias of key j seen from query i, off = j - i, times `unit`: log2(e) for scores in the log2 domain (bf16), 1 for natural ones
+// (fp32).  A NaN entry stays NaN; a finite one is held above REL_LOWEST (the type's lowest value times log2(e), or with a score
+// added, would be -inf, which means "never").
+__device__ __forceinline__ float rel_bias(const RelK& p, int head, int off, float unit = REL_LOG2E) {
   const int a = min(abs(off), p.sat);
   const int b = p.bucket[a] + (off > 0 ? p.buckets >> 1 : 0);
   const float v = p.table_f32 ? static_cast<const float*>(p.table)[b * p.nh + head]
                               : (float)static_cast<const __bf16*>(p.table)[b * p.nh + head];
-  return v == -INFINITY || v != v ? v : fmaxf(v * REL_LOG2E, REL_LOWEST);
+  return v == -INFINITY || v != v ? v : fmaxf(v * unit, REL_LOWEST);
 }
 
 __device__ __forceinline__ int rel_length(const RelK& p, int n) {
   return p.lengths ? max(0, min(p.lengths[n], p.l)) : p.l;
 }
 
-__device__ __forceinline__ void rel_fill(const RelK& p, int head, float* bias, int tid, int threads) {
+__device__ __forceinline__ void rel_fill(const RelK& p, int head, float* bias, int tid, int threads, float unit = REL_LOG2E) {
   const int w = rel_width(p.sat);
   for (int i = tid; i < w; i += threads) {
     const int off = i - REL_PAD - p.sat;
-    bias[i] = rel_bias(p, head, max(-p.sat, min(off, p.sat)));
+    bias[i] = rel_bias(p, head, max(-p.sat, min(off, p.sat)), unit);
   }
 }
 

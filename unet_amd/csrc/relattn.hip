@@ -788,7 +788,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 // ---------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(AT_THREADS) void rel_attn_dtable_kernel(const RelK p, void* dtable) {
   __shared__ int range[2];
-  __shared__ float wsum[4];
+  __shared__ double wsum[4];
   const int b = blockIdx.x, head = blockIdx.y, side = p.buckets >> 1, tid = threadIdx.x;
   const int local = b < side ? b : b - side;
   if (tid == 0) { range[0] = p.sat + 1; range[1] = -1; }
@@ -797,23 +797,23 @@ __global__ __launch_bounds__(AT_THREADS) void rel_attn_dtable_kernel(const RelK 
     if (p.bucket[a] == local && !(a == 0 && b >= side)) { atomicMin(&range[0], a); atomicMax(&range[1], a); }
   __syncthreads();
   const int a0 = range[0], cnt = range[1] - range[0] + 1;      // distances a0 .. a0+cnt-1; none: cnt <= 0
-  float s = 0.f;
+  double s = 0.0;                                 // (the sums of a bucket cancel)
   if (cnt > 0) {
     const float* src = p.part + (long long)head * p.parts * (2 * p.sat + 1);
     const int first = b < side ? p.sat - (a0 + cnt - 1) : p.sat + a0;
     const long long total = (long long)p.parts * cnt;
     for (long long i = tid; i < total; i += AT_THREADS) {
       const long long row = i / cnt;
-      s += src[row * (2 * p.sat + 1) + first + (int)(i - row * cnt)];
+      s += (double)src[row * (2 * p.sat + 1) + first + (int)(i - row * cnt)];
     }
   }
-  s = wave_sum(s);
+  for (int m = 32; m; m >>= 1) s += __shfl_xor(s, m, 64);
   if ((tid & 63) == 0) wsum[tid >> 6] = s;
   __syncthreads();
   if (tid == 0) {
-    s = wsum[0] + wsum[1] + wsum[2] + wsum[3];
-    if (p.table_f32) static_cast<float*>(dtable)[b * p.nh + head] = s;
-    else static_cast<__bf16*>(dtable)[b * p.nh + head] = (__bf16)s;
+    const float t = (float)((wsum[0] + wsum[1]) + (wsum[2] + wsum[3]));
+    if (p.table_f32) static_cast<float*>(dtable)[b * p.nh + head] = t;
+    else static_cast<__bf16*>(dtable)[b * p.nh + head] = (__bf16)t;
   }
 }
 

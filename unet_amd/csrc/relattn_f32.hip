@@ -11,6 +11,12 @@
 
 namespace {
 
+// Scores stay in the natural domain and lse is kept as two planes, the maximum and log2 of the sum: in P = exp(s - m) / l the
+// difference of two scores is exact where one key dominates, so that P is as good there as an exp of 32 bits, and dP - delta keeps its
+// digits (one rounded sum m + log2 l, in the log2 domain, cost up to 4 times the error of dQ and the table's gradient).
+__device__ __forceinline__ long long rel32_logs(const RelK& p) { return (long long)p.n * p.nh * p.l; }
+__device__ __forceinline__ float rel32_exp(float diff, float lg = 0.f) { return __builtin_amdgcn_exp2f(fmaf(diff, REL_LOG2E, -lg)); }
+
 template <bool SPLIT> struct Shape {
   static constexpr int ROWS = SPLIT ? 16 : A32_ROWS;          // rows a workgroup owns
   static constexpr int STEP = SPLIT ? 4 * A32_BK : A32_BK;    // rows of the other side a step
@@ -84,7 +90,7 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_fwd_kernel(const RelK p)
   load_rows<HDP>(qreg, static_cast<const float*>(p.q) + o.base + (long long)qrow * p.c, row_ok, g, p.hd);
 #pragma unroll
   for (int d = 0; d < DT; ++d) oacc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  rel_fill(p, o.head, bias, tid, A32_THREADS);
+  rel_fill(p, o.head, bias, tid, A32_THREADS, 1.f);
   float m = -INFINITY, lsum = 0.f;
   const int end = o.tile * ROWS < o.len ? o.len : 0;            // (uniform) nothing to do behind the window's length
   Fetch<HDP, STEP> fk, fv;
@@ -107,18 +113,18 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_fwd_kernel(const RelK p)
       for (int i = 0; i < 4; ++i) {
         const int key = key0 + 16 * s + 4 * g + i;
         const float b = bias[max(-p.sat, min(key - qrow, p.sat)) + p.sat + REL_PAD];
-        st[s][i] = key < o.len ? fmaf(st[s][i], p.scale_log2, b) : -INFINITY;
+        st[s][i] = key < o.len ? fmaf(st[s][i], p.scale, b) : -INFINITY;
         mx = fmaxf(mx, st[s][i]);
       }
     }
     mx = group_max(mx);
     const float m_new = fmaxf(m, mx), ref = m_new == -INFINITY ? 0.f : m_new;       // a row with nothing to see yet
-    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+    const float alpha = m == -INFINITY ? 0.f : rel32_exp(m - m_new);
     float ps = 0.f;
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { st[s][i] = __builtin_amdgcn_exp2f(st[s][i] - ref); ps += st[s][i]; }
+      for (int i = 0; i < 4; ++i) { st[s][i] = rel32_exp(st[s][i] - ref); ps += st[s][i]; }
     lsum = lsum * alpha + group_sum(ps);
     m = m_new;
 #pragma unroll
@@ -137,14 +143,17 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_fwd_kernel(const RelK p)
     lsum = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      f[w] = vt[w * 32 + l15] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(vt[w * 32 + l15] - m);
+      f[w] = vt[w * 32 + l15] == -INFINITY ? 0.f : rel32_exp(vt[w * 32 + l15] - m);
       lsum = fmaf(vt[w * 32 + 16 + l15], f[w], lsum);
     }
   }
   if (qrow < p.l) {
     const bool seen = row_ok && lsum > 0.f, spoiled = row_ok && lsum != lsum;
     const float inv = seen ? 1.f / lsum : spoiled ? lsum : 0.f;
-    if (p.lse && g == 0 && (!SPLIT || wave == 0)) p.lse[o.stat + qrow] = seen ? m + __builtin_amdgcn_logf(lsum) : spoiled ? lsum : INFINITY;
+    if (p.lse && g == 0 && (!SPLIT || wave == 0)) {
+      p.lse[o.stat + qrow] = seen ? m : spoiled ? lsum : INFINITY;
+      p.lse[rel32_logs(p) + o.stat + qrow] = seen ? __builtin_amdgcn_logf(lsum) : 0.f;
+    }
     float* yp = static_cast<float*>(p.out) + o.base + (long long)qrow * p.c;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -176,20 +185,23 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dq_kernel(const RelK p) 
   load_rows<HDP>(doreg, static_cast<const float*>(p.dout) + o.base + (long long)qrow * p.c, row_ok, g, p.hd);
 #pragma unroll
   for (int d = 0; d < DT; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  rel_fill(p, o.head, bias, tid, A32_THREADS);
+  rel_fill(p, o.head, bias, tid, A32_THREADS, 1.f);
   if (p.part)
     for (int i = tid; i < 4 * w; i += A32_THREADS) sums[i] = 0.f;
   auto add = [](float* at, float v) { __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); };
-  const float lse = row_ok ? p.lse[o.stat + qrow] : INFINITY;          // rows past the end: p = 0
-  float delta = 0.f;                                                   // <dO, O>, kept for dK and dV
+  const float m = row_ok ? p.lse[o.stat + qrow] : INFINITY;            // rows past the end: p = 0
+  const float lg = row_ok ? p.lse[rel32_logs(p) + o.stat + qrow] : 0.f;
+  float delta;                                                         // <dO, O>, kept for dK and dV
   {
     f32x4 oreg[DT];
     load_rows<HDP>(oreg, static_cast<const float*>(p.out) + o.base + (long long)qrow * p.c, row_ok, g, p.hd);
+    double d = 0.0;                          // (its error stays in every dS of the row, where the sums of a bucket cancel)
 #pragma unroll
     for (int u = 0; u < DT; ++u)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) delta = fmaf(doreg[u][e], oreg[u][e], delta);
-    delta = group_sum(delta);
+      for (int e = 0; e < 4; ++e) d = fma((double)doreg[u][e], (double)oreg[u][e], d);
+    d += __shfl_xor(d, 16, 64);
+    delta = (float)(d + __shfl_xor(d, 32, 64));
     if (g == 0 && row_ok && (!SPLIT || wave == 0)) p.delta[o.stat + qrow] = delta;
   }
   float fneg = 0.f, fpos = 0.f;                          // sums beyond the band
@@ -215,7 +227,7 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dq_kernel(const RelK p) 
         const int key = key0 + 16 * s + 4 * g + i;
         at[i] = max(-p.sat, min(key - qrow, p.sat)) + p.sat;
         const float b = bias[at[i] + REL_PAD];
-        const float pe = key < o.len ? __builtin_amdgcn_exp2f(fmaf(st[i], p.scale_log2, b - lse)) : 0.f;
+        const float pe = key < o.len ? rel32_exp(fmaf(st[i], p.scale, b) - m, lg) : 0.f;
         st[i] = pe * (dp[i] - delta);
       }
       if (p.part) {
@@ -272,8 +284,8 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dkv_kernel(const RelK p)
   extern __shared__ __attribute__((aligned(16))) char smem_raw[];
   float* qtile = reinterpret_cast<float*>(smem_raw);
   float* dtile = qtile + STEP * LD;
-  float* stats = dtile + STEP * LD;                     // [STEP] lse, [STEP] delta of the step's rows
-  float* bias = stats + 2 * STEP;
+  float* stats = dtile + STEP * LD;                     // [STEP] maxima, [STEP] log2 of the sums, [STEP] delta of the step's rows
+  float* bias = stats + 3 * STEP;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, g = lane >> 4;
   const Place o = place<ROWS>(p);
   const int key = o.tile * ROWS + (SPLIT ? 0 : wave * 16) + l15, mine = SPLIT ? wave * A32_BK : 0;
@@ -287,16 +299,19 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dkv_kernel(const RelK p)
   load_rows<HDP>(vreg, static_cast<const float*>(p.v) + kvo, key_ok, g, p.hd);
 #pragma unroll
   for (int d = 0; d < DT; ++d) { dka[d] = f32x4{0.f, 0.f, 0.f, 0.f}; dva[d] = f32x4{0.f, 0.f, 0.f, 0.f}; }
-  rel_fill(p, o.head, bias, tid, A32_THREADS);
+  rel_fill(p, o.head, bias, tid, A32_THREADS, 1.f);
   const int end = o.tile * ROWS < o.len ? o.len : 0;
   Fetch<HDP, STEP> fq, fd;
-  float stat = 0.f;
+  constexpr int NS = (3 * STEP + A32_THREADS - 1) / A32_THREADS;
+  float stat[NS];
   auto get = [&](int row0) {
     fq.get(qslab, row0, end, p.c, p.hd, tid);
     fd.get(dslab, row0, end, p.c, p.hd, tid);
-    if (tid < 2 * STEP) {
-      const int r = row0 + (tid & (STEP - 1));
-      stat = r < end ? (tid < STEP ? p.lse[o.stat + r] : p.delta[o.stat + r]) : (tid < STEP ? INFINITY : 0.f);
+#pragma unroll
+    for (int k = 0; k < NS; ++k) {
+      const int i = tid + k * A32_THREADS, which = i / STEP, r = row0 + i % STEP;
+      stat[k] = which == 0 ? INFINITY : 0.f;
+      if (which < 3 && r < end) stat[k] = which == 0 ? p.lse[o.stat + r] : which == 1 ? p.lse[rel32_logs(p) + o.stat + r] : p.delta[o.stat + r];
     }
   };
   get(0);
@@ -304,7 +319,9 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dkv_kernel(const RelK p)
     __syncthreads();
     fq.put(qtile, tid);
     fd.put(dtile, tid);
-    if (tid < 2 * STEP) stats[tid] = stat;
+#pragma unroll
+    for (int k = 0; k < NS; ++k)
+      if (tid + k * A32_THREADS < 3 * STEP) stats[tid + k * A32_THREADS] = stat[k];
     __syncthreads();
     get(step + STEP);
     const int row0 = step + mine;
@@ -316,9 +333,9 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dkv_kernel(const RelK p)
       for (int r = 0; r < 4; ++r) {
         const int rl = 16 * s + 4 * g + r;
         const float b = bias[max(-p.sat, min(key - row0 - rl, p.sat)) + p.sat + REL_PAD];
-        const float pe = __builtin_amdgcn_exp2f(fmaf(st[r], p.scale_log2, b - stats[mine + rl]));   // rows past the end: lse = inf
+        const float pe = rel32_exp(fmaf(st[r], p.scale, b) - stats[mine + rl], stats[STEP + mine + rl]);   // rows past the end: inf
         st[r] = pe;
-        dp[r] = pe * (dp[r] - stats[STEP + mine + rl]);
+        dp[r] = pe * (dp[r] - stats[2 * STEP + mine + rl]);
       }
       rows_acc<HDP>(dva, dtile, mine + 16 * s, st, l15, g);
       rows_acc<HDP>(dka, qtile, mine + 16 * s, dp, l15, g);
@@ -365,7 +382,7 @@ template <int HDP, bool SPLIT> int launch_fwd32(const RelK& p, hipStream_t st) {
 template <int HDP, bool SPLIT> int launch_bwd32(const RelK& p, hipStream_t st) {
   typedef Shape<SPLIT> S;
   const size_t tiles = (size_t)2 * S::STEP * (HDP + 4) + rel_width(p.sat);
-  const size_t lds_q = sizeof(float) * (tiles + (p.part ? 4 * (2 * (size_t)p.sat + 1) : 0)), lds_kv = sizeof(float) * (tiles + 2 * S::STEP);
+  const size_t lds_q = sizeof(float) * (tiles + (p.part ? 4 * (2 * (size_t)p.sat + 1) : 0)), lds_kv = sizeof(float) * (tiles + 3 * S::STEP);
   if (set_lds(&rel32_dq_kernel<HDP, SPLIT>, lds_q, "rel_attn_bwd (fp32 dq)")) return -1;
   if (set_lds(&rel32_dkv_kernel<HDP, SPLIT>, lds_kv, "rel_attn_bwd (fp32 dk, dv)")) return -1;
   const dim3 grid((unsigned)(p.n * p.nh * cdiv(p.l, S::ROWS)));

@@ -1863,7 +1863,8 @@ def _rel_sizes(dt: int, n: int, l: int, c: int, n_heads: int, last_start: int):
 def _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, keep: bool):
     n, l, c = q.shape
     out = torch.empty_like(q)
-    lse = torch.empty((n, n_heads, l), dtype=torch.float32, device=q.device) if keep else None
+    planes = 1 if q.dtype == torch.bfloat16 else 2
+    lse = torch.empty((planes, n, n_heads, l), dtype=torch.float32, device=q.device) if keep else None
     rest = torch.empty_like(q) if keep and q.dtype == torch.bfloat16 else None          # what rounding takes from out: delta needs it
     size = _rel_sizes(_dt(q), n, l, c, n_heads, starts[-1])[0]
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
@@ -1888,7 +1889,7 @@ class RelBiasAttnFn(torch.autograd.Function):
         n, l, c = q.shape
         dout = _aligned(dout)
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-        delta = torch.empty_like(lse)
+        delta = torch.empty((n, ctx.n_heads, l), dtype=torch.float32, device=q.device)
         _, size, floats = _rel_sizes(_dt(q), n, l, c, ctx.n_heads, ctx.starts[-1])
         ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
         dtable = partials = None
