@@ -503,13 +503,16 @@ int unet_rel_attn_bwd(int32_t dtype, const void* q, const void* k, const void* v
  * UNET_OPT_MAX_TENSORS tensors (device): start256 [n+1] first block of each (absolute; the batch covers blocks start256[0]
  * .. start256[n]-1 = blocks256 of them), numel [n] < 2^31, slot [n] first block in m8 / r8 and the scale arrays, or
  * 0x80000000 | first float4 in m32 / v32 for a tensor whose moments stay fp32.  A NULL gradient skips its tensor.
- * Order of a step with a clip: unet_grad_sqnorm (advances step_t), unet_adamw8_prepare (norm from the partial sums, clip,
- * bias corrections into bc [n][2]), unet_adamw8_apply.  Without one: prepare with advance = 1 and n_partial = 0, apply with
- * `partial` (unet_adamw8_blocks(blocks256) floats of g^2 sums), prepare with n_tensors = 0 and those sums for the norm.
- * coef [8]: [0] clip, [3] norm, [4] lr. */
+ * Order of a step with a clip: unet_adamw8_sqnorm (partial: unet_adamw8_norm_blocks(blocks256) doubles), unet_adamw8_prepare with
+ * sums64 = 1 (norm from the partial sums, clip, step counts, bias corrections into bc [n][2]), unet_adamw8_apply.  Without one:
+ * prepare with n_partial = 0, apply with `partial` (unet_adamw8_blocks(blocks256) floats of g^2 sums), prepare with n_tensors = 0,
+ * sums64 = 0 and those sums for the norm.  coef [8]: [0] clip, [3] norm, [4] lr. */
 int32_t unet_adamw8_blocks(int64_t blocks256);
-int unet_adamw8_prepare(const float* const* grads_host, int32_t n_tensors, const float* partial, int32_t n_partial,
-                        int32_t advance, float max_norm, const float* lr, float* coef, float* step_t, double beta1, double beta2,
+int32_t unet_adamw8_norm_blocks(int64_t blocks256);
+int unet_adamw8_sqnorm(const float* const* grads_host, int32_t n_tensors, const uint32_t* start256, const uint32_t* numel,
+                       int64_t blocks256, double* partial, void* stream);
+int unet_adamw8_prepare(const float* const* grads_host, int32_t n_tensors, const void* partial, int32_t n_partial,
+                        int32_t sums64, float max_norm, const float* lr, float* coef, float* step_t, double beta1, double beta2,
                         float* bc, void* stream);
 int unet_adamw8_apply(const float* const* grads_host, int32_t n_tensors, float* const* p_ptrs, const uint32_t* start256,
                       const uint32_t* numel, const uint32_t* slot, int64_t blocks256, void* m8, void* r8, float* m_scale,

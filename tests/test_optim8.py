@@ -71,6 +71,8 @@ def test_refusals_on_cpu():
     assert b"clip" in lib.unet_last_error()
     assert lib.unet_adamw8_prepare(None, 300, None, 0, 0, 0.0, 16, 16, 16, 0.9, 0.9, 16, None) == -1
     assert b"at most" in lib.unet_last_error()
+    assert lib.unet_adamw8_sqnorm(None, 1, 16, 16, 1, 16, None) == -1 and b"null" in lib.unet_last_error()
+    assert [lib.unet_adamw8_norm_blocks(b) for b in (1, 32, 33, 16384)] == [1, 1, 2, 512]
     assert [lib.unet_adamw8_blocks(b) for b in (1, 4, 5, 16384)] == [1, 1, 2, 4096]
 
 

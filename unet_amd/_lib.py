@@ -150,6 +150,8 @@ _SIGNATURES = {
     "unet_rel_attn_bwd": (C.c_int, [_i32, _vp, _vp, _vp, _vp, _i32, _i32, C.POINTER(_i32), _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32,
                                     _i32, _f32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _vp]),
     "unet_adamw8_blocks": (_i32, [_i64]),
+    "unet_adamw8_norm_blocks": (_i32, [_i64]),
+    "unet_adamw8_sqnorm": (C.c_int, [C.POINTER(C.c_void_p), _i32, _vp, _vp, _i64, _vp, _vp]),
     "unet_adamw8_prepare": (C.c_int, [C.POINTER(C.c_void_p), _i32, _vp, _i32, _i32, _f32, _vp, _vp, _vp, C.c_double, C.c_double,
                                       _vp, _vp]),
     "unet_adamw8_apply": (C.c_int, [C.POINTER(C.c_void_p), _i32, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,

@@ -91,6 +91,49 @@ __device__ __forceinline__ int find_tensor(const unsigned* start, int n, unsigne
   return lo;
 }
 
+// Sums of g^2 in 64 bits, one a workgroup: with 32-bit sums the clip was now and then an ulp off the rounding of the exact norm's, which
+// moves a hundred of 42 M codes across a border.  HBM-bound: NORM_BLOCKS loads of 16 bytes a lane in flight; 42 M elements 31 us.
+constexpr int NORM_BLOCKS = 8;                                     // blocks of 256 elements a wave
+__global__ __launch_bounds__(A8_THREADS) void adamw8_sqnorm_kernel(const GradPtrs gp, const unsigned* start, const unsigned* numel, int n,
+                                                                   double* partial) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned first = start[0] + (blockIdx.x * A8_WAVES + wave) * NORM_BLOCKS;
+  const unsigned end = min(first + NORM_BLOCKS, start[n]);
+  double s = 0.0;
+  if (first < end) {
+    int t = find_tensor(start, n, first);
+    const float* g0 = gp.g[t];
+    // the usual case: whole blocks of one aligned tensor
+    if (end == first + NORM_BLOCKS && end <= start[t + 1] && (end - start[t]) * 256u <= numel[t] && !(reinterpret_cast<uintptr_t>(g0) & 15)) {
+      if (g0) {
+        f32x4 v[NORM_BLOCKS];
+#pragma unroll
+        for (int u = 0; u < NORM_BLOCKS; ++u) v[u] = *reinterpret_cast<const f32x4*>(g0 + (first - start[t] + u) * 256u + lane * 4);
+#pragma unroll
+        for (int u = 0; u < NORM_BLOCKS; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s = fma((double)v[u][e], (double)v[u][e], s);
+      }
+    } else {
+      for (unsigned b = first; b < end; ++b) {
+        while (b >= start[t + 1]) ++t;
+        const float* g = gp.g[t];
+        if (!g) continue;
+        const unsigned i = (b - start[t]) * 256u + lane * 4, ne = numel[t];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (i + e < ne) s = fma((double)g[i + e], (double)g[i + e], s);
+      }
+    }
+  }
+  __shared__ double red[A8_WAVES];
+#pragma unroll
+  for (int m = 32; m; m >>= 1) s += __shfl_xor(s, m, 64);
+  if (lane == 0) red[wave] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
 __global__ __launch_bounds__(A8_THREADS) void adamw8_apply_kernel(const Adam8 k, const GradPtrs gp) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned b = k.start[0] + blockIdx.x * A8_WAVES + wave;
@@ -173,29 +216,29 @@ __global__ __launch_bounds__(A8_THREADS) void adamw8_apply_kernel(const Adam8 k,
   }
 }
 
-// One workgroup.  norm != 0: ||g|| from the partial sums into coef[3], and the clip min(1, max_norm / (||g|| + 1e-6)) into
-// coef[0]; otherwise coef[0] = 1.  Then lr into coef[4] and each tensor's bias corrections.  advance != 0: the tensors with a
-// gradient count this step (unet_grad_sqnorm has done it otherwise).
+// One workgroup.  blocks > 0: ||g|| from the partial sums into coef[3], and the clip min(1, max_norm / (||g|| + 1e-6)) into
+// coef[0]; otherwise coef[0] = 1.  Then lr into coef[4], and the tensors with a gradient count this step and get their bias corrections.
 constexpr int PREP_THREADS = 1024;
-__global__ __launch_bounds__(PREP_THREADS) void adamw8_prepare_kernel(const GradPtrs gp, const float* partial, int blocks, int norm,
-                                                                      int advance, float max_norm, const float* lr, float* coef,
-                                                                      float* step_t, int n, double beta1, double beta2, float2* bc) {
+template <typename T> __device__ __forceinline__ double prepare_sum(const T* partial, int blocks) {
+  double a = 0.0;
+  int i = threadIdx.x;
+  for (; i + 3 * PREP_THREADS < blocks; i += 4 * PREP_THREADS)
+    a += ((double)partial[i] + (double)partial[i + PREP_THREADS]) +
+         ((double)partial[i + 2 * PREP_THREADS] + (double)partial[i + 3 * PREP_THREADS]);
+  for (; i < blocks; i += PREP_THREADS) a += (double)partial[i];
+  return a;
+}
+__global__ __launch_bounds__(PREP_THREADS) void adamw8_prepare_kernel(const GradPtrs gp, const void* partial, int blocks, int sums64,
+                                                                      float max_norm, const float* lr, float* coef, float* step_t, int n,
+                                                                      double beta1, double beta2, float2* bc) {
   const int t = threadIdx.x;
   if (bc && t < n) {
-    if (advance && gp.g[t]) step_t[t] += 1.f;
+    if (gp.g[t]) step_t[t] += 1.f;
     const double st = (double)step_t[t];
     bc[t] = make_float2((float)((double)*lr / (1.0 - pow(beta1, st))), (float)(1.0 / sqrt(1.0 - pow(beta2, st))));
   }
-  double a = 0.0;
-  if (norm) {
-    int i = t;
-    for (; i + 3 * PREP_THREADS < blocks; i += 4 * PREP_THREADS)
-      a += ((double)partial[i] + (double)partial[i + PREP_THREADS]) +
-           ((double)partial[i + 2 * PREP_THREADS] + (double)partial[i + 3 * PREP_THREADS]);
-    for (; i < blocks; i += PREP_THREADS) a += (double)partial[i];
-  }
   __shared__ double red[PREP_THREADS];
-  red[t] = a;
+  red[t] = sums64 ? prepare_sum(static_cast<const double*>(partial), blocks) : prepare_sum(static_cast<const float*>(partial), blocks);
   __syncthreads();
   for (int s = PREP_THREADS / 2; s > 0; s >>= 1) {
     if (t < s) red[t] += red[t + s];
@@ -203,7 +246,7 @@ __global__ __launch_bounds__(PREP_THREADS) void adamw8_prepare_kernel(const Grad
   }
   if (t == 0) {
     float clip = 1.f;
-    if (norm) {
+    if (blocks > 0) {
       const float total = (float)sqrt(red[0]);
       coef[3] = total;
       if (max_norm > 0.f) {
@@ -220,8 +263,26 @@ __global__ __launch_bounds__(PREP_THREADS) void adamw8_prepare_kernel(const Grad
 
 extern "C" int32_t unet_adamw8_blocks(int64_t blocks256) { return (int32_t)((blocks256 + A8_WAVES - 1) / A8_WAVES); }
 
-extern "C" int unet_adamw8_prepare(const float* const* grads_host, int32_t n_tensors, const float* partial, int32_t n_partial,
-                                   int32_t advance, float max_norm, const float* lr, float* coef, float* step_t, double beta1,
+extern "C" int32_t unet_adamw8_norm_blocks(int64_t blocks256) {
+  return (int32_t)((blocks256 + A8_WAVES * NORM_BLOCKS - 1) / (A8_WAVES * NORM_BLOCKS));
+}
+
+extern "C" int unet_adamw8_sqnorm(const float* const* grads_host, int32_t n_tensors, const uint32_t* start256, const uint32_t* numel,
+                                  int64_t blocks256, double* partial, void* stream) {
+  UNET_REQUIRE(grads_host && start256 && numel && partial, "adamw8_sqnorm: null pointer");
+  UNET_REQUIRE(n_tensors >= 1 && n_tensors <= UNET_OPT_MAX_TENSORS, "adamw8_sqnorm: 1..%d tensors per call, got %d",
+               UNET_OPT_MAX_TENSORS, n_tensors);
+  UNET_REQUIRE(blocks256 > 0 && blocks256 < (1ll << 31), "adamw8_sqnorm: %lld blocks", (long long)blocks256);
+  GradPtrs gp;
+  for (int i = 0; i < UNET_OPT_MAX_TENSORS; ++i) gp.g[i] = i < n_tensors ? grads_host[i] : nullptr;
+  hipLaunchKernelGGL(adamw8_sqnorm_kernel, dim3(unet_adamw8_norm_blocks(blocks256)), dim3(A8_THREADS), 0, static_cast<hipStream_t>(stream),
+                     gp, start256, numel, n_tensors, partial);
+  UNET_LAUNCH_CHECK("adamw8_sqnorm");
+  return 0;
+}
+
+extern "C" int unet_adamw8_prepare(const float* const* grads_host, int32_t n_tensors, const void* partial, int32_t n_partial,
+                                   int32_t sums64, float max_norm, const float* lr, float* coef, float* step_t, double beta1,
                                    double beta2, float* bc, void* stream) {
   UNET_REQUIRE(lr && coef, "adamw8_prepare: null pointer");
   UNET_REQUIRE(n_tensors >= 0 && n_tensors <= UNET_OPT_MAX_TENSORS, "adamw8_prepare: at most %d tensors per call, got %d",
@@ -231,8 +292,8 @@ extern "C" int unet_adamw8_prepare(const float* const* grads_host, int32_t n_ten
   UNET_REQUIRE(n_partial > 0 || !(max_norm > 0.f), "adamw8_prepare: a clip needs the partial sums");
   GradPtrs gp;
   for (int i = 0; i < UNET_OPT_MAX_TENSORS; ++i) gp.g[i] = i < n_tensors ? grads_host[i] : nullptr;
-  hipLaunchKernelGGL(adamw8_prepare_kernel, dim3(1), dim3(PREP_THREADS), 0, static_cast<hipStream_t>(stream), gp, partial, n_partial,
-                     (int)(n_partial > 0), advance, max_norm, lr, coef, step_t, n_tensors, beta1, beta2,
+  hipLaunchKernelGGL(adamw8_prepare_kernel, dim3(1), dim3(PREP_THREADS), 0, static_cast<hipStream_t>(stream), gp, partial, n_partial, sums64,
+                     max_norm, lr, coef, step_t, n_tensors, beta1, beta2,
                      n_tensors ? reinterpret_cast<float2*>(bc) : nullptr);
   UNET_LAUNCH_CHECK("adamw8_prepare");
   return 0;

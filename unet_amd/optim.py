@@ -145,7 +145,6 @@ class _Group8:
             raise ValueError("ClipAdamW: more than 2^33 parameters in one group")
         as_u32 = lambda v: torch.tensor(v, dtype=torch.int64).to(torch.int32).to(dev)        # the low 32 bits
         self.start256, self.slot = as_u32(start), as_u32(slot)
-        self.start4 = as_u32([b * (BLOCK // 4) for b in start])
         self.numel = as_u32([p.numel() for p in params])
         self.p_ptrs = torch.tensor([p.data_ptr() for p in params], dtype=torch.int64, device=dev)
         self.ptrs = [p.data_ptr() for p in params]
@@ -168,14 +167,15 @@ class _Group8:
             if nb == 0:
                 continue
             batches.append((a, b - a, nb, n1, n2))
-            n1 += int(lib.unet_opt_blocks(nb * BLOCK))
+            n1 += int(lib.unet_adamw8_norm_blocks(nb))
             n2 += int(lib.unet_adamw8_blocks(nb))
         self.n_norm, self.n_step = n1, n2
-        self.partial = torch.zeros(max(n1, n2, 1), dtype=torch.float32, device=dev)
+        self.partial = torch.zeros(max(n2, 1), dtype=torch.float32, device=dev)
+        self.partial64 = torch.zeros(max(n1, 1), dtype=torch.float64, device=dev)
         # the fixed arguments of a batch's three calls (tables of 4-byte entries, but 8 bytes a pointer and a bias correction)
         part, at = self.partial.data_ptr(), lambda t, a: t.data_ptr() + a * t.element_size()
         self.calls = [(a, n,
-                       (at(self.start4, a), at(self.numel, a), nb * BLOCK, part + 4 * p1, at(self.step, a)),
+                       (at(self.start256, a), at(self.numel, a), nb, at(self.partial64, p1)),
                        (at(self.step, a), at(self.bc, 2 * a)),
                        (at(self.p_ptrs, a), at(self.start256, a), at(self.numel, a), at(self.slot, a), nb, self.m8.data_ptr(),
                         self.r8.data_ptr(), self.m_scale.data_ptr(), self.r_scale.data_ptr(), self.m.data_ptr(), self.v.data_ptr(),
@@ -340,18 +340,18 @@ class ClipAdamW(torch.optim.Optimizer):
         st = torch._C._cuda_getCurrentRawStream(g.device)
         b1, b2 = (float(b) for b in group["betas"])
         eps, decay = float(group["eps"]), float(group["weight_decay"])
-        clips, part, coef = max_norm > 0.0, g.partial.data_ptr(), g.coef.data_ptr()
+        clips, coef = max_norm > 0.0, g.coef.data_ptr()
         arrs = [(C.c_void_p * c[1])(*grads[c[0]:c[0] + c[1]]) for c in g.calls]
+        sums = (g.partial64.data_ptr(), g.n_norm, 1) if clips else (None, 0, 0)
         if clips:
             for (_, n, norm, _, _, _), arr in zip(g.calls, arrs):
-                check(lib.unet_grad_sqnorm(arr, n, *norm, st), "unet_grad_sqnorm")
+                check(lib.unet_adamw8_sqnorm(arr, n, *norm, st), "unet_adamw8_sqnorm")
         for (_, n, _, prep, _, _), arr in zip(g.calls, arrs):
-            check(lib.unet_adamw8_prepare(arr, n, part, g.n_norm if clips else 0, int(not clips), max_norm, lr_ptr, coef, prep[0], b1,
-                                          b2, prep[1], st), "unet_adamw8_prepare")
+            check(lib.unet_adamw8_prepare(arr, n, *sums, max_norm, lr_ptr, coef, prep[0], b1, b2, prep[1], st), "unet_adamw8_prepare")
         for (_, n, _, _, table, p2), arr in zip(g.calls, arrs):
             check(lib.unet_adamw8_apply(arr, n, *table, None if clips else p2, b1, b2, eps, decay, st), "unet_adamw8_apply")
         if not clips:
-            check(lib.unet_adamw8_prepare(None, 0, part, g.n_step, 0, 0.0, lr_ptr, coef, None, b1, b2, None, st),
+            check(lib.unet_adamw8_prepare(None, 0, g.partial.data_ptr(), g.n_step, 0, 0.0, lr_ptr, coef, None, b1, b2, None, st),
                   "unet_adamw8_prepare")
 
     @torch.no_grad()
