@@ -91,8 +91,8 @@ __device__ __forceinline__ int find_tensor(const unsigned* start, int n, unsigne
   return lo;
 }
 
-// Sums of g^2 in 64 bits, one a workgroup: with 32-bit sums the clip was now and then an ulp off the rounding of the exact norm's, which
-// moves a hundred of 42 M codes across a border.  HBM-bound: NORM_BLOCKS loads of 16 bytes a lane in flight; 42 M elements 31 us.
+// Sums of g^2 in 64 bits, one a workgroup: with 32-bit sums the clip was now and then an ulp off the one of the exact norm, which
+// moves some of 42 M codes across a border.  HBM-bound: NORM_BLOCKS loads of 16 bytes a lane in flight; 42 M elements 31 us.
 constexpr int NORM_BLOCKS = 8;                                     // blocks of 256 elements a wave
 __global__ __launch_bounds__(A8_THREADS) void adamw8_sqnorm_kernel(const GradPtrs gp, const unsigned* start, const unsigned* numel, int n,
                                                                    double* partial) {
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(PREP_THREADS) void adamw8_prepare_kernel(const Grad
       const float total = (float)sqrt(red[0]);
       coef[3] = total;
       if (max_norm > 0.f) {
-        clip = max_norm / (total + 1e-6f);
+        clip = max_norm * (1.f / (total + 1e-6f));      // rounded as clip_grad_norm_ does: an ulp of it moves codes
         clip = clip < 1.f ? clip : 1.f;
       }
     }
