@@ -479,8 +479,8 @@ int unet_clip_adamw_apply(const float* const* grads_host, int32_t n_tensors, flo
  * (starts_host[0] = 0, not decreasing, the last one in 1 .. UNET_REL_MAX_DISTANCE).  A bias of -inf removes its pairs.
  * lengths: NULL or [n] int32 on the device; positions at or past a window's length are neither keys nor queries: their outputs
  * and gradients are zero, and what they hold is not read.  A row with nothing to see gives zeros.
- * For a backward pass, otherwise NULL: lse, fp32, [n][n_heads][l] in bf16 and [2][n][n_heads][l] in fp32; in bf16 also out_rest
- * [n][l][c] bf16 (what rounding took from out).  Backward: dtable may be NULL; partials:
+ * For a backward pass, otherwise NULL: lse, fp32, [2][n][n_heads][l]; in bf16 also out_rest [n][l][c] bf16 (what rounding took
+ * from out).  Backward: dtable may be NULL; partials:
  * unet_rel_attn_bwd_partials(...) floats; delta: scratch, [n][n_heads][l] floats.  workspace: unet_rel_attn_workspace_bytes(...) bytes (0
  * unless few rows walk a long window), 16-byte aligned, used by this call only. */
 #define UNET_REL_MAX_DISTANCE 512

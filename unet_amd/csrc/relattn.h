@@ -6,8 +6,9 @@ struct RelK {
   const void *q, *k, *v;       // [N][L][C], head h in columns h*hd .. h*hd+hd-1
   void* out;                   // [N][L][C]
   void* rest;                  // [N][L][C] or null (bf16 with a backward pass): what rounding took from out
-  float* lse;                  // [N][nh][L] or null; log2 domain: p = exp2(s*scale_log2 + bias - lse); +inf: nothing to see
-                               // (fp32: [2][N][nh][L], maximum in the natural domain and log2 of the sum)
+  float* lse;                  // [2][N][nh][L] or null: a reference m of the row's scores (bf16: in the log2 domain; +inf: nothing to
+                               // see) and the log2 of the sum over m.  Two planes, p = exp2((s - m) - log): a score that a large finite bias
+                               // absorbed differs from m by nothing, and log2 of the sum is not lost beside such an m
   const void* dout;            // [N][L][C]
   float* delta;                // [N][nh][L]: <dO, O> of a row and head
   void *dq, *dk, *dv;          // [N][L][C]
@@ -49,6 +50,8 @@ __device__ __forceinline__ float rel_bias(const RelK& p, int head, int off, floa
                               : (float)static_cast<const __bf16*>(p.table)[b * p.nh + head];
   return v == -INFINITY || v != v ? v : fmaxf(v * unit, REL_LOWEST);
 }
+
+__device__ __forceinline__ long long rel_logs(const RelK& p) { return (long long)p.n * p.nh * p.l; }      // lse: start of the logs
 
 __device__ __forceinline__ int rel_length(const RelK& p, int n) {
   return p.lengths ? max(0, min(p.lengths[n], p.l)) : p.l;

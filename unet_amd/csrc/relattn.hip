@@ -28,19 +28,34 @@ namespace {
 // [32, 1024, 1024], heads of 128.  Heads of 256 need the registers of a whole CU.
 constexpr int REL_OCC2 = 128;
 
+// What a tile adds to its scores: biases by offset (NEAR), or one constant (BEYOND, FLAT).  A constant is folded into the exponential's
+// fma (BEYOND) while it is small.  A large one (a mask of the type's lowest value, -1e9) absorbs the scores it is added to; the
+// difference of two such constants would bring them back, so the complete score is formed first and the row's maximum and the log2 of
+// its sum are taken off one after the other, as in NEAR tiles: forward and backward then see the same P (FLAT).
+enum Kind { NEAR, BEYOND, FLAT };
+typedef std::integral_constant<Kind, NEAR> Near;
+typedef std::integral_constant<Kind, BEYOND> Beyond;
+typedef std::integral_constant<Kind, FLAT> Flat;
+constexpr float REL_FOLD = 1024.f;      // folded up to here (log2 domain): its rounding, 2^-14, is below those of a P in bf16
+
+__device__ __forceinline__ bool rel_folds(float beyond) {
+  return __builtin_amdgcn_readfirstlane(!(fabsf(beyond) > REL_FOLD) || beyond == -INFINITY);
+}
+
 // Streamed tiles [lo, hi) of T rows against the 32 rows a wave holds from `own` on: [lo, n0) lie wholly beyond one edge of the
-// band, [n0, n1) touch it, [n1, hi) lie beyond the other edge.  The three runs are three loops (a wave's own bounds: every tile
-// has one barrier, whichever loop it is in), so the accumulators pass no branch.
-struct Runs { int n0, n1; };
-template <int T> __device__ __forceinline__ Runs rel_runs(int lo, int hi, int own, int sat) {
+// band ([lo, f0) of them fold their constant, all or none), [n0, n1) touch it, [n1, hi) lie beyond the other edge ([n1, f1) fold).
+// The runs are loops of their own (a wave's own bounds: every tile has one barrier, whichever loop it is in), so the accumulators
+// pass no branch.
+struct Runs { int f0, n0, n1, f1; };
+template <int T> __device__ __forceinline__ Runs rel_runs(int lo, int hi, int own, int sat, float before, float behind) {
   const int left = own - sat - (T - 1), right = own + 31 + sat;           // first tile that starts behind `left` / at or behind `right`
   Runs r;
   r.n0 = max(lo, min(hi, left >= 0 ? left / T + 1 : 0));
   r.n1 = max(r.n0, min(hi, (right + T - 1) / T));
+  r.f0 = rel_folds(before) ? r.n0 : lo;
+  r.f1 = rel_folds(behind) ? hi : r.n1;
   return r;
 }
-typedef std::integral_constant<bool, true> Near;
-typedef std::integral_constant<bool, false> Beyond;
 
 // A lane's fragments of its own row of a [L][C] slab, from `t` at element `row` (a row that exists; zeros unless `ok`).  No branches:
 // all loads leave at once.
@@ -141,7 +156,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     ld.setup(wave, lane, p.c, p.hd);
     const int a0 = row_read_base<HDP>(lane);
     const int vb0 = tr_read_base<HDP>(lane, 0), vb1 = tr_read_base<HDP>(lane, 1);
-    const Runs runs = rel_runs<AT_BK>(kb_lo, kb_hi, q0 + wave * 32, p.sat);
+    const Runs runs = rel_runs<AT_BK>(kb_lo, kb_hi, q0 + wave * 32, p.sat, cneg, cpos);
     const unsigned tile_step = (unsigned)AT_BK * p.c * 2;
     auto issue = [&](int kb, int buf) {
       char* at = smem + buf * 2 * G::TILE;
@@ -156,8 +171,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     // a row that exceeds the margin sends the workgroup through a second walk with the true maxima
     int bad = 0, buf = 0;
     while (true) {
-      auto tile = [&](int kb, auto near, float beyond) {
-        constexpr bool NEAR = decltype(near)::value;
+      auto tile = [&](int kb, auto kind, float beyond) {
+        constexpr Kind KIND = decltype(kind)::value;
         __syncthreads();
         if (kb + 1 < kb_hi) issue(kb + 1, buf ^ 1);
         const char* kt = smem + buf * 2 * G::TILE;
@@ -200,13 +215,14 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         __builtin_amdgcn_s_setprio(0);
 
         // score in the log2 domain = st * mul + add
-        const float mul = NEAR ? 1.f : p.scale_log2, add = NEAR ? 0.f : beyond;
-        if constexpr (NEAR) {
+        const float mul = KIND == BEYOND ? p.scale_log2 : 1.f, add = KIND == BEYOND ? beyond : 0.f;
+        if constexpr (KIND != BEYOND) {
           const float* bl = bias + (key0 + 4 * h - qrow + p.sat + REL_PAD);
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) st[t][e] = fmaf(st[t][e], p.scale_log2, bl[32 * t + (e & 3) + 8 * (e >> 2)]);
+            for (int e = 0; e < 16; ++e)
+              st[t][e] = fmaf(st[t][e], p.scale_log2, KIND == NEAR ? bl[32 * t + (e & 3) + 8 * (e >> 2)] : beyond);
         }
         if (key0 + AT_BK > len) {
 #pragma unroll
@@ -226,7 +242,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         bad |= mx > m + 32.f;
         const float shift = add - (m == -INFINITY ? 0.f : m);
         auto exp_one = [&](int t, int e) {
-          const float pe = __builtin_amdgcn_exp2f(NEAR ? st[t][e] + shift : fmaf(st[t][e], mul, shift));
+          const float pe = __builtin_amdgcn_exp2f(KIND == BEYOND ? fmaf(st[t][e], mul, shift) : st[t][e] + shift);
           st[t][e] = pe;
           lsum += pe;
         };
@@ -256,9 +272,11 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         __builtin_amdgcn_s_setprio(0);
       };
       int kb = kb_lo;
-      for (; kb < runs.n0; ++kb) tile(kb, Beyond{}, cneg);
+      for (; kb < runs.f0; ++kb) tile(kb, Beyond{}, cneg);
+      for (; kb < runs.n0; ++kb) tile(kb, Flat{}, cneg);
       for (; kb < runs.n1; ++kb) tile(kb, Near{}, 0.f);
-      for (; kb < kb_hi; ++kb) tile(kb, Beyond{}, cpos);
+      for (; kb < runs.f1; ++kb) tile(kb, Beyond{}, cpos);
+      for (; kb < kb_hi; ++kb) tile(kb, Flat{}, cpos);
       if (!(kb_hi - kb_lo > 1 && __syncthreads_or(bad))) break;
       issue(kb_lo, buf);
       m = mtrue;
@@ -292,7 +310,10 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
   const bool spoiled = row_ok && lt != lt;
   const float inv = seen ? 1.f / lt : spoiled ? lt : 0.f;
   if (qrow < p.l) {
-    if (lse && h == 0) *lse = seen ? m + __builtin_amdgcn_logf(lt) : spoiled ? lt : INFINITY;
+    if (lse && h == 0) {
+      lse[0] = seen ? m : spoiled ? lt : INFINITY;
+      lse[rel_logs(p)] = seen ? __builtin_amdgcn_logf(lt) : 0.f;
+    }
 #pragma unroll
     for (int d = 0; d < G::DT; ++d)
 #pragma unroll
@@ -336,7 +357,11 @@ __global__ __launch_bounds__(AT_THREADS) void rel_attn_join_fwd_kernel(const Rel
   }
   const bool seen = lt > 0.f, spoiled = lt != lt;
   const float inv = seen ? 1.f / lt : spoiled ? lt : 0.f;
-  if (p.lse && ch == head * p.hd) p.lse[((long long)n * p.nh + head) * p.l + row] = seen ? m + __builtin_amdgcn_logf(lt) : spoiled ? lt : INFINITY;
+  if (p.lse && ch == head * p.hd) {
+    float* lse = p.lse + ((long long)n * p.nh + head) * p.l + row;
+    lse[0] = seen ? m : spoiled ? lt : INFINITY;
+    lse[rel_logs(p)] = seen ? __builtin_amdgcn_logf(lt) : 0.f;
+  }
   bf16x4 o, rest;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -436,7 +461,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     own_row<HDP>(of, p.out, at, row_ok, h, p.hd);
     own_row<HDP>(rest, p.rest, at, row_ok, h, p.hd);
     own_row<HDP>(qf, p.q, at, row_ok, h, p.hd);
-    const float stat = p.lse[si], lse = row_ok ? stat : INFINITY;
+    const float stat = p.lse[si], logs = p.lse[rel_logs(p) + si];
+    const float m = row_ok ? stat : INFINITY, lg = row_ok ? logs : 0.f, lse = m + lg;       // rows past the end: p = 0
     float delta = 0.f;
 #pragma unroll
     for (int s = 0; s < G::KS; ++s)
@@ -447,8 +473,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
     rel_fill(p, head, bias, tid, AT_THREADS);
     float* const dg = diag + wave * DG_WORDS;
     int buf = 0;
-    auto tile = [&](int kb, auto near, float beyond, float& fsum) {
-      constexpr bool NEAR = decltype(near)::value;
+    auto tile = [&](int kb, auto kind, float beyond, float& fsum) {
+      constexpr Kind KIND = decltype(kind)::value;
       __syncthreads();
       if (kb + 1 < kb_hi) issue(kb + 1, buf ^ 1);
       const char* kt = smem + buf * 2 * TILE;
@@ -484,8 +510,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       const float shift = beyond - lse;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float off = NEAR ? bl[(e & 3) + 8 * (e >> 2)] - lse : shift;
-        st[e] = __builtin_amdgcn_exp2f(fmaf(st[e], p.scale_log2, off));
+        if constexpr (KIND == BEYOND) st[e] = __builtin_amdgcn_exp2f(fmaf(st[e], p.scale_log2, shift));
+        else st[e] = __builtin_amdgcn_exp2f((fmaf(st[e], p.scale_log2, KIND == NEAR ? bl[(e & 3) + 8 * (e >> 2)] : beyond) - m) - lg);
       }
       if (key0 + BW_ROWS > len) {
 #pragma unroll
@@ -495,7 +521,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 #pragma unroll
       for (int e = 0; e < 16; ++e) st[e] *= dp[e] - delta;
       if (p.part) {
-        if constexpr (!NEAR) {
+        if constexpr (KIND != NEAR) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) fsum += st[e];
         } else {
@@ -537,11 +563,13 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
         }
       }
     };
-    const Runs runs = rel_runs<BW_ROWS>(kb_lo, kb_hi, q0w, p.sat);
+    const Runs runs = rel_runs<BW_ROWS>(kb_lo, kb_hi, q0w, p.sat, cneg, cpos);
     int kb = kb_lo;
-    for (; kb < runs.n0; ++kb) tile(kb, Beyond{}, cneg, fneg);
+    for (; kb < runs.f0; ++kb) tile(kb, Beyond{}, cneg, fneg);
+    for (; kb < runs.n0; ++kb) tile(kb, Flat{}, cneg, fneg);
     for (; kb < runs.n1; ++kb) tile(kb, Near{}, 0.f, fneg);
-    for (; kb < kb_hi; ++kb) tile(kb, Beyond{}, cpos, fpos);
+    for (; kb < runs.f1; ++kb) tile(kb, Beyond{}, cpos, fpos);
+    for (; kb < kb_hi; ++kb) tile(kb, Flat{}, cpos, fpos);
   }
 
   if (p.splits > 1 && qrow < p.l) {
@@ -599,15 +627,16 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 // at head size 128; the keys' K rows are read from LDS, their V rows stay in registers, and two workgroups fit a CU.
 // ---------------------------------------------------------------------------------------------
 constexpr int KV_KEYS = 128;
+constexpr int KV_STATS = 4 * BW_ROWS;               // of a tile's rows: maximum, log2 of the sum, delta, and the first two added up
 
 template <int HDP, bool FINE>
 __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_dkv_kernel(const RelK p) {
   typedef Cfg<HDP> G;
   constexpr int TILE = BW_ROWS * G::ROWB;
-  extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][Q tile | dO tile], K rows, [2][64] row stats, biases
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // [2 buffers][Q tile | dO tile], K rows, [2][4][32] row stats, biases
   char* const krows = smem + 4 * TILE;
   float* const stats = reinterpret_cast<float*>(krows + KV_KEYS * G::ROWB);
-  float* const bias = stats + 4 * BW_ROWS;
+  float* const bias = stats + 2 * KV_STATS;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
@@ -654,20 +683,23 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       ld.issue(dbase, len, p.c, p.hd, at + TILE, (unsigned)qb * BW_ROWS, wave);
     };
     const long long sbase = ((long long)n * p.nh + head) * p.l;
-    auto load_stat = [&](int qb) {                   // threads 0..31: lse, 32..63: delta of the tile's rows
-      float v = tid < BW_ROWS ? INFINITY : 0.f;      // rows past the end: p = 0, delta = 0
-      const int row = qb * BW_ROWS + (tid & (BW_ROWS - 1));
-      if (tid < 2 * BW_ROWS && row < len) v = tid < BW_ROWS ? p.lse[sbase + row] : p.delta[sbase + row];
+    auto load_stat = [&](int qb) {                   // 32 threads a kind
+      const int which = tid / BW_ROWS, row = qb * BW_ROWS + (tid & (BW_ROWS - 1));
+      float v = which == 0 || which == 3 ? INFINITY : 0.f;      // rows past the end: p = 0, delta = 0
+      if (which < 4 && row < len) {
+        v = which == 2 ? p.delta[sbase + row] : p.lse[(which == 1 ? rel_logs(p) : 0) + sbase + row];
+        if (which == 3) v += p.lse[rel_logs(p) + sbase + row];
+      }
       return v;
     };
     issue(qb_lo, 0);
     bf16x8 vf[G::KS];
     own_row<HDP>(vf, p.v, base + (long long)min(key, len - 1) * p.c, key_ok, h, p.hd);
     rel_fill(p, head, bias, tid, AT_THREADS);
-    if (tid < 2 * BW_ROWS) stats[tid] = load_stat(qb_lo);
+    if (tid < KV_STATS) stats[tid] = load_stat(qb_lo);
     int buf = 0;
-    auto tile = [&](int qb, auto near, float beyond) {
-      constexpr bool NEAR = decltype(near)::value;
+    auto tile = [&](int qb, auto kind, float beyond) {
+      constexpr Kind KIND = decltype(kind)::value;
       __syncthreads();   // the tile and its stats are in LDS; every wave is done with the other buffer
       float stat_next = 0.f;
       if (qb + 1 < qb_hi) {
@@ -676,7 +708,7 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       }
       const char* qtile = smem + buf * 2 * TILE;
       const char* dtile = qtile + TILE;
-      const float* st_in = stats + buf * 2 * BW_ROWS;
+      const float* st_in = stats + buf * KV_STATS;
       const int row0 = qb * BW_ROWS;
       f32x16 st, dp;
 #pragma unroll
@@ -708,12 +740,15 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
       const float* bl = bias + (key - row0 - 4 * h - 27 + p.sat + REL_PAD);     // bl[27 - x]: local row x + 4h
 #pragma unroll
       for (int e4 = 0; e4 < 4; ++e4) {
-        const f32x4 ls = *reinterpret_cast<const f32x4*>(st_in + 8 * e4 + 4 * h);
-        const f32x4 de = *reinterpret_cast<const f32x4*>(st_in + BW_ROWS + 8 * e4 + 4 * h);
+        auto stat = [&](int which) { return *reinterpret_cast<const f32x4*>(st_in + which * BW_ROWS + 8 * e4 + 4 * h); };
+        const f32x4 ls = stat(KIND == BEYOND ? 3 : 0), de = stat(2);
+        f32x4 lg;
+        if constexpr (KIND != BEYOND) lg = stat(1);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float off = NEAR ? bl[27 - 8 * e4 - e] - ls[e] : beyond - ls[e];
-          const float pe = __builtin_amdgcn_exp2f(fmaf(st[4 * e4 + e], p.scale_log2, off));
+          float pe;
+          if constexpr (KIND == BEYOND) pe = __builtin_amdgcn_exp2f(fmaf(st[4 * e4 + e], p.scale_log2, beyond - ls[e]));
+          else pe = __builtin_amdgcn_exp2f((fmaf(st[4 * e4 + e], p.scale_log2, KIND == NEAR ? bl[27 - 8 * e4 - e] : beyond) - ls[e]) - lg[e]);
           st[4 * e4 + e] = pe;
           dp[4 * e4 + e] = pe * (dp[4 * e4 + e] - de[e]);
         }
@@ -731,14 +766,16 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
           dka[d0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(tq[b & 1], rest8(dp, s, db), dka[d0], 0, 0, 0);
         }
       }
-      if (qb + 1 < qb_hi && tid < 2 * BW_ROWS) stats[(buf ^ 1) * 2 * BW_ROWS + tid] = stat_next;
+      if (qb + 1 < qb_hi && tid < KV_STATS) stats[(buf ^ 1) * KV_STATS + tid] = stat_next;
       buf ^= 1;
     };
-    const Runs runs = rel_runs<BW_ROWS>(qb_lo, qb_hi, key0w, p.sat);       // rows in front of the keys: key - row > 0
+    const Runs runs = rel_runs<BW_ROWS>(qb_lo, qb_hi, key0w, p.sat, cpos, cneg);       // rows in front of the keys: key - row > 0
     int qb = qb_lo;
-    for (; qb < runs.n0; ++qb) tile(qb, Beyond{}, cpos);
+    for (; qb < runs.f0; ++qb) tile(qb, Beyond{}, cpos);
+    for (; qb < runs.n0; ++qb) tile(qb, Flat{}, cpos);
     for (; qb < runs.n1; ++qb) tile(qb, Near{}, 0.f);
-    for (; qb < qb_hi; ++qb) tile(qb, Beyond{}, cneg);
+    for (; qb < runs.f1; ++qb) tile(qb, Beyond{}, cneg);
+    for (; qb < qb_hi; ++qb) tile(qb, Flat{}, cneg);
   }
 
   if (p.splits > 1 && key < p.l) {
@@ -866,7 +903,7 @@ template <int HDP, bool FINE> int launch_dq(const RelK& p, hipStream_t st) {
 }
 
 template <int HDP, bool FINE> int launch_dkv(const RelK& p, hipStream_t st) {
-  const size_t lds = (4 * (size_t)BW_ROWS + KV_KEYS) * Cfg<HDP>::ROWB + 4 * BW_ROWS * sizeof(float) + bias_bytes(p.sat, 1);
+  const size_t lds = (4 * (size_t)BW_ROWS + KV_KEYS) * Cfg<HDP>::ROWB + 2 * KV_STATS * sizeof(float) + bias_bytes(p.sat, 1);
   if (set_lds(&rel_attn_dkv_kernel<HDP, FINE>, lds, "rel_attn_bwd (dk, dv)")) return -1;
   hipLaunchKernelGGL((rel_attn_dkv_kernel<HDP, FINE>), dim3((unsigned)(p.n * p.nh * cdiv(p.l, KV_KEYS) * p.splits)), dim3(AT_THREADS), lds, st, p);
   UNET_LAUNCH_CHECK("rel_attn_bwd (dk, dv)");

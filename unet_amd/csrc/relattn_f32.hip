@@ -14,7 +14,6 @@ namespace {
 // Scores stay in the natural domain and lse is kept as two planes, the maximum and log2 of the sum: in P = exp(s - m) / l the
 // difference of two scores is exact where one key dominates, so that P is as good there as an exp of 32 bits, and dP - delta keeps its
 // digits (one rounded sum m + log2 l, in the log2 domain, cost up to 4 times the error of dQ and the table's gradient).
-__device__ __forceinline__ long long rel32_logs(const RelK& p) { return (long long)p.n * p.nh * p.l; }
 __device__ __forceinline__ float rel32_exp(float diff, float lg = 0.f) { return __builtin_amdgcn_exp2f(fmaf(diff, REL_LOG2E, -lg)); }
 
 template <bool SPLIT> struct Shape {
@@ -152,7 +151,7 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_fwd_kernel(const RelK p)
     const float inv = seen ? 1.f / lsum : spoiled ? lsum : 0.f;
     if (p.lse && g == 0 && (!SPLIT || wave == 0)) {
       p.lse[o.stat + qrow] = seen ? m : spoiled ? lsum : INFINITY;
-      p.lse[rel32_logs(p) + o.stat + qrow] = seen ? __builtin_amdgcn_logf(lsum) : 0.f;
+      p.lse[rel_logs(p) + o.stat + qrow] = seen ? __builtin_amdgcn_logf(lsum) : 0.f;
     }
     float* yp = static_cast<float*>(p.out) + o.base + (long long)qrow * p.c;
 #pragma unroll
@@ -190,7 +189,7 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dq_kernel(const RelK p) 
     for (int i = tid; i < 4 * w; i += A32_THREADS) sums[i] = 0.f;
   auto add = [](float* at, float v) { __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); };
   const float m = row_ok ? p.lse[o.stat + qrow] : INFINITY;            // rows past the end: p = 0
-  const float lg = row_ok ? p.lse[rel32_logs(p) + o.stat + qrow] : 0.f;
+  const float lg = row_ok ? p.lse[rel_logs(p) + o.stat + qrow] : 0.f;
   float delta;                                                         // <dO, O>, kept for dK and dV
   {
     f32x4 oreg[DT];
@@ -311,7 +310,7 @@ __global__ __launch_bounds__(A32_THREADS, 1) void rel32_dkv_kernel(const RelK p)
     for (int k = 0; k < NS; ++k) {
       const int i = tid + k * A32_THREADS, which = i / STEP, r = row0 + i % STEP;
       stat[k] = which == 0 ? INFINITY : 0.f;
-      if (which < 3 && r < end) stat[k] = which == 0 ? p.lse[o.stat + r] : which == 1 ? p.lse[rel32_logs(p) + o.stat + r] : p.delta[o.stat + r];
+      if (which < 3 && r < end) stat[k] = which == 0 ? p.lse[o.stat + r] : which == 1 ? p.lse[rel_logs(p) + o.stat + r] : p.delta[o.stat + r];
     }
   };
   get(0);
