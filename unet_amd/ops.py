@@ -16,6 +16,7 @@ from dataclasses import dataclass
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import ACT_IDS, ConvDesc, check
@@ -1679,12 +1680,23 @@ def _run(what: str, dev: int, *args):
         check(rc, what)
 
 
+def _dims(t: Tensor) -> Tuple[int, ...]:
+    """Plain ints, also under ``torch.jit.trace``, which hands out sizes as tensors."""
+    return tuple(map(int, t.shape))
+
+
 def _ptr(t: Optional[Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
 
 def _wants_grad(*tensors: Optional[Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _watched() -> bool:
+    """A forward-mode level is open or ``torch.jit.trace`` runs: both see what an autograd function does, not what a library call
+    writes into an empty tensor."""
+    return forward_ad._current_level >= 0 or torch.jit.is_tracing()
 
 
 def _once_differentiable(what: str):
@@ -1722,7 +1734,7 @@ def _scan_sizes(dt: int, n: int, l: int, c: int):
 
 def _scan_forward(x: Tensor, gate: Tensor, h0: Optional[Tensor], reverse: bool, keep: bool):
     """(h, last, states): ``states`` is what backward starts from, the fp32 state in front of every tile of rows."""
-    n, l, c = x.shape
+    n, l, c = _dims(x)
     h = torch.empty((n, l, c), dtype=x.dtype, device=x.device)
     last = torch.empty((n, c), dtype=torch.float32, device=x.device)
     size, kept = _scan_sizes(_dt(x), n, l, c)
@@ -1782,7 +1794,7 @@ def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor] = None, reverse: bo
     else:
         x, gate = _dense_channels(x), _dense_channels(gate)
         h0 = None if h0 is None else h0.contiguous()
-        if _wants_grad(x, gate, h0):
+        if _wants_grad(x, gate, h0) or _watched():
             h, last = GatedScanFn.apply(x, gate, h0, bool(reverse))
         else:
             h, last, _ = _scan_forward(x, gate, h0, bool(reverse), False)
@@ -1795,6 +1807,9 @@ def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
     if _wants_grad(x, gate, state):
         raise RuntimeError("gated_scan_step has no backward pass (its state moves on in place): call it under torch.no_grad(), or "
                            "gated_scan on the rows")
+    if _watched() and (torch.jit.is_tracing() or any(forward_ad.unpack_dual(t).tangent is not None for t in (x, gate, state))):
+        raise RuntimeError("gated_scan_step carries no tangents and cannot be traced (its state moves on in place): call gated_scan on "
+                           "the rows")
     _check_scan("gated_scan_step", x, gate, state, 2)
     if not state.is_contiguous():
         raise ValueError("gated_scan_step: the state is updated in place and must be contiguous")
@@ -1861,7 +1876,7 @@ def _rel_sizes(dt: int, n: int, l: int, c: int, n_heads: int, last_start: int):
 
 
 def _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, keep: bool):
-    n, l, c = q.shape
+    n, l, c = _dims(q)
     out = torch.empty_like(q)
     lse = torch.empty((2, n, n_heads, l), dtype=torch.float32, device=q.device) if keep else None
     rest = torch.empty_like(q) if keep and q.dtype == torch.bfloat16 else None          # what rounding takes from out: delta needs it
@@ -1924,14 +1939,14 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
     unit = 8 if _dt(q) == _lib.BF16 else 4
     if k.dtype != q.dtype or v.dtype != q.dtype or any(t.device != q.device for t in (k, v, table)):
         raise TypeError("rel_bias_attention: q, k and v must have one dtype and all tensors one device")
-    n, l, c = q.shape
+    n, l, c = _dims(q)
     if n_heads < 1 or n_heads > 256 or c % n_heads or (c // n_heads) % unit or c // n_heads > 256 or c < 1:
         raise ValueError(f"rel_bias_attention: {c} channels in {n_heads} heads: the head size must be a multiple of {unit} for {q.dtype} "
                          "and at most 256 (at most 256 heads)")
     if table.dim() != 2 or table.shape[1] != n_heads:
         raise ValueError(f"rel_bias_attention: the table must be [n_buckets, {n_heads}], got {tuple(table.shape)}")
     _dt(table)
-    starts = rel_bucket_starts(table.shape[0], int(max_distance))
+    starts = rel_bucket_starts(int(table.shape[0]), int(max_distance))
     scale = (c // n_heads) ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError(f"rel_bias_attention: scale must be positive and finite, got {scale}")
@@ -1943,6 +1958,6 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
     if q.numel() == 0:
         return q * k * v + 0 * table.sum().to(q.dtype)
     q, k, v, table = _aligned(q), _aligned(k), _aligned(v), table.contiguous()
-    if _wants_grad(q, k, v, table):
+    if _wants_grad(q, k, v, table) or _watched():
         return RelBiasAttnFn.apply(q, k, v, table, n_heads, scale, starts, lengths)
     return _rel_forward(q, k, v, table, n_heads, scale, starts, lengths, False)[0]
