@@ -364,3 +364,27 @@ def test_two_captured_graphs_in_turn():
         for (x, g, h0), (h, last) in zip(sets, outs):
             h2, last2 = ops.gated_scan(x, g, h0, return_state=True)
             assert torch.equal(h, h2) and torch.equal(last, last2), rep
+
+
+def check_moved_state(dev):
+    from unet_amd import ops
+    w, state = torch.ones(2, 8, device=dev, requires_grad=True), torch.full((2, 8), 2.0, device=dev)
+    loss = (w * state[:]).sum()                 # saves the state (a view of it) for backward
+    version = state._version
+    with torch.no_grad():
+        ops.gated_scan_step(torch.ones(2, 8, device=dev), torch.zeros(2, 8, device=dev), state)
+    assert state._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_a_moved_state_is_seen_by_autograd_on_cpu(monkeypatch):
+    from unet_amd import ops
+    monkeypatch.setattr(ops, "_run", lambda *a: None)
+    monkeypatch.setattr(ops, "_need_cuda", lambda *a: None)
+    check_moved_state("cpu")
+
+
+@pytest.mark.gpu
+def test_a_moved_state_is_seen_by_autograd():
+    check_moved_state("cuda")

@@ -1819,6 +1819,7 @@ def gated_scan_step(x: Tensor, gate: Tensor, state: Tensor) -> Tensor:
         x, gate = _dense_channels(x), _dense_channels(gate)
         _run("unet_gated_scan_step", x.device.index, _dt(x), x.data_ptr(), x.stride(0), gate.data_ptr(), gate.stride(0),
              state.data_ptr(), h.data_ptr(), n, c)
+        torch.autograd.graph.increment_version(state)        # whoever saved the state for backward is told
     return h
 
 
