@@ -387,3 +387,37 @@ def test_checkpoint_files(tmp_path):
         assert torch.equal(p, q)
         for k, t in opts[0].state[p].items():
             assert torch.equal(t.float(), opts[1].state[q][k].float()), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_gradient_norms_that_are_not_finite(bad):
+    """With a clip the norm carries a NaN to every tensor, and an infinite norm takes the other gradients to zero, as
+    clip_grad_norm_ in front of torch's AdamW does; the fp32 tensors of the group likewise."""
+    from unet_amd.optim import ClipAdamW
+    shapes = [(40, 130), (77,), (5000,), (3,)]
+    params, gen = make(9, shapes)
+    other = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    kw = dict(lr=1e-3, betas=BETAS, weight_decay=0.0)
+    opt, ref = ClipAdamW(params, max_grad_norm=1.0, state_bits=8, **kw), torch.optim.AdamW(other, **kw)
+    for it in range(2):
+        set_grads(params, gen, 1.0)
+        if it == 1:
+            params[2].grad[1234] = bad
+        for p, q in zip(params, other):
+            q.grad = p.grad.clone()
+        before = [p.detach().clone() for p in params]
+        opt.step()
+        torch.nn.utils.clip_grad_norm_(other, 1.0)
+        ref.step()
+    block = torch.zeros(5000, dtype=torch.bool, device="cuda")
+    block[1234 // 256 * 256:1234 // 256 * 256 + 256] = True      # shares the spoilt element's scale
+    for i, (p, q, p0) in enumerate(zip(params, other, before)):
+        stray = torch.isnan(p) != torch.isnan(q)
+        assert not bool((stray & ~block if i == 2 else stray).any()), i
+        if math.isinf(bad):       # the first step's momentum alone: lr m / sqrt(v) changes, by less than a few steps of lr
+            keep = torch.isfinite(p)
+            assert int((~keep).sum()) == (1 if i == 2 else 0)
+            assert 0 < float((p - p0)[keep].abs().max()) < 4e-3
+        else:
+            assert bool(torch.isnan(p).all())

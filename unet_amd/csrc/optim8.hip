@@ -4,7 +4,8 @@
 // ROOT of v is kept because codes with a 4-bit exponent cover 2^-15 of a block's largest root, that is 2^-30 of its largest v.
 // A positive root never becomes zero (it is raised to the smallest code, 2^-9): a stored m over a vanished root would be
 // divided by eps alone at the next step.  A block whose largest value is below 2^-100 is stored as zeros: 448 / max would
-// overflow, and such moments are far below any eps.  An infinite or NaN gradient makes its block of 256 NaN.
+// overflow, and such moments are far below any eps.  An infinite or NaN gradient makes its block of 256 NaN; with a clip a NaN
+// reaches every element through the norm, and an infinite norm takes all other gradients to zero.
 // Stored values are rounded to nearest even; the step itself uses m and r before that rounding.
 // Tensors the caller keeps in 32 bits (small ones: norms, biases) go through the same launches.
 //
@@ -251,7 +252,7 @@ __global__ __launch_bounds__(PREP_THREADS) void adamw8_prepare_kernel(const Grad
       coef[3] = total;
       if (max_norm > 0.f) {
         clip = max_norm * (1.f / (total + 1e-6f));      // rounded as clip_grad_norm_ does: an ulp of it moves codes
-        clip = clip < 1.f ? clip : 1.f;
+        clip = clip > 1.f ? 1.f : clip;                 // (a NaN norm reaches every tensor, as it does there)
       }
     }
     coef[0] = clip;
