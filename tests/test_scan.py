@@ -388,3 +388,98 @@ def test_a_moved_state_is_seen_by_autograd_on_cpu(monkeypatch):
 @pytest.mark.gpu
 def test_a_moved_state_is_seen_by_autograd():
     check_moved_state("cuda")
+
+
+# ---------------------------------------------------------------------------------------- long memories
+def long_gates(c):
+    """Gates from 9 to 18.6, a constant per channel; half of them put 1 - sigmoid halfway between two multiples of 2^-24, where
+    rounding the gate itself to 32 bits would be furthest off."""
+    k = torch.logspace(0, 3.2, c // 2, dtype=torch.float64).floor()
+    keep = (k + 0.5) * U
+    return torch.cat([torch.linspace(9.0, 18.6, c - c // 2, dtype=torch.float64), torch.log((1 - keep) / keep)]).float()
+
+
+def long_oracle(x, g, h0, dh, dlast):
+    """As ``oracle``, for a kernel whose states keep 1 - f: a row's gate costs keep times a relative error (400 u: 40 u of the gate, and
+    the chains of up to 200 pairs that span a long sequence), and the state itself is rounded once per 8 rows (a span of 8 rows is
+    one step of the state's chain) and 16 units more on the way to a row (8 rows, each a rounding and half a unit of the rounded
+    gate, and the last step).  The adjoint likewise; sums of dh over a span of up to
+    12288 rows round in steps of at least 192 rows: 100 u |dh| a row."""
+    x, g, d = (t.double().cpu() for t in (x, g, dh))
+    s, mu = h0.double().cpu(), dlast.double().cpu()
+    e, em = torch.zeros_like(s), torch.zeros_like(s)
+    f, keep = torch.sigmoid(g), torch.sigmoid(-g)
+    l, top = x.shape[1], d.abs().amax(1)
+    h, eh, before, eb, dx, ex, dg, eg = (torch.empty_like(x) for _ in range(8))
+    for t in range(l):
+        before[:, t], eb[:, t] = s, e + 16 * U * s.abs()
+        e = f[:, t] * e + 400 * U * keep[:, t] * (s.abs() + x[:, t].abs())
+        s = f[:, t] * s + keep[:, t] * x[:, t]
+        e += U / 8 * s.abs()
+        h[:, t], eh[:, t] = s, e + 16 * U * s.abs()
+    last = (s, e + 16 * U * s.abs())
+    for t in range(l - 1, -1, -1):
+        lam = d[:, t] + mu
+        el = em + 16 * U * lam.abs()
+        diff, ed = before[:, t] - x[:, t], eb[:, t] + U * (before[:, t].abs() + x[:, t].abs())
+        fk = f[:, t] * keep[:, t]
+        dx[:, t], ex[:, t] = keep[:, t] * lam, keep[:, t] * (el + 2 * K * U * lam.abs())
+        dg[:, t], eg[:, t] = lam * diff * fk, fk * (el * diff.abs() + lam.abs() * ed + 3 * K * U * (lam * diff).abs())
+        mu = f[:, t] * lam
+        em = f[:, t] * em + 400 * U * keep[:, t] * lam.abs() + U / 8 * mu.abs() + 100 * U * top
+    return dict(h=(h, eh), last=last, dx=(dx, ex), dg=(dg, eg), dh0=(mu, em + 16 * U * mu.abs()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,l", [(1, 20000), (300, 3000)])
+def test_long_memories(n, l, dtype):
+    """Split sequences and whole ones, with gates whose memory is 8 thousand to 120 million rows."""
+    c = 64
+    gen = torch.Generator().manual_seed(l)
+    r = lambda *s: 1.0 + 0.3 * torch.randn(*s, generator=gen)
+    x, dh, h0, dlast = r(n, l, c).to(dtype).cuda(), r(n, l, c).to(dtype).cuda(), r(n, c).cuda(), r(n, c).cuda()
+    g = long_gates(c).to(dtype).cuda().expand(n, l, c)
+    got, want = call(x, g, h0, dh, dlast, False), long_oracle(x, g, h0, dh, dlast)
+    for k in got:
+        near(got[k], want[k], k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_constant_input_holds_its_state(dtype):
+    """x = h0 is the recurrence's fixed point, whatever the gate.  A span's A + B / x differs from 1 by the roundings of its sums, at most
+    2.5 R + 5 units of C for a chain of R, and a state leaves a fixed point only where that exceeds half an ulp (C above 1 / 40), to
+    come back at a rate of C: 2.5 R + 5 + 100 units, R at most 200.  A single row's f + rest + keep is 1 to one rounding."""
+    from unet_amd import ops
+    v = torch.linspace(1.0, 1.9375, 64).to(dtype).float().cuda()
+    v[::2] *= -1
+    for n, l in ((1, 75000), (300, 3000)):
+        g = long_gates(64).to(dtype).cuda().expand(n, l, 64)
+        for reverse in (False, True):
+            h, last = ops.gated_scan(v.to(dtype).expand(n, l, 64), g, v.expand(n, 64), reverse=reverse, return_state=True)
+            assert float((last.double() / v.double() - 1).abs().max()) <= 605 * U, (n, l, reverse)
+    state, x = v.repeat(3, 1), v.to(dtype).repeat(3, 1)
+    g = torch.stack([long_gates(64), -long_gates(64), torch.linspace(-9, 9, 64)]).to(dtype).cuda()
+    for _ in range(3000):
+        ops.gated_scan_step(x, g, state)
+    assert float((state.double() / v.double() - 1).abs().max()) <= 2 * U
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinite_inputs_stay_infinite(dtype):
+    """An infinite input makes its state infinite for the rest of the sequence, of one sign, without a NaN where gates are open."""
+    from unet_amd import ops
+    for n, l in ((1, 5000), (300, 130)):
+        x, g, h0, _, _ = inputs(n, l, 64, dtype, seed=40)
+        g = g.abs() + 0.5
+        g[:, :, 32:] += 12.0
+        x[0, 70, 3], x[0, 70, 40] = float("inf"), -float("inf")
+        h, last = ops.gated_scan(x, g, h0, return_state=True)
+        assert not bool(torch.isnan(h).any())
+        assert bool((h[0, 70:, 3] == float("inf")).all()) and bool((h[0, 70:, 40] == -float("inf")).all())
+        assert int(torch.isinf(h).sum()) == 2 * (l - 70) and int(torch.isinf(last).sum()) == 2
+        state = last.clone()
+        ops.gated_scan_step(x[:, 0], g[:, 0], state)
+        assert torch.equal(torch.isinf(state), torch.isinf(last)) and not bool(torch.isnan(state).any())

@@ -20,9 +20,13 @@
 // there: forward 71 us (403 MB, 5.7 TB/s), backward 123 us (671 MB, 5.5 TB/s); [1, 75000, 1024] forward 134 us, of which the
 // segment launch takes 55 (461 + 307 MB).
 //
-// Everything between loads and stores is fp32.  sigmoid: with t = exp(-|g|), small = t / (1 + t), big = 1 - small; both sides
-// keep full relative precision where 1 - f would cancel.
+// Everything between loads and stores is fp32.  sigmoid: with t = exp(-|g|), small = t / (1 + t), big = 1 - small; keep = 1 - f
+// has full relative precision on both sides.  A long memory lives in 1 - f, which fp32 rounds to multiples of 2^-24 next to 1: 1 - f
+// would be 0.07 % off at g = 10 and nothing at g = 17.4, so that a state would settle beside its input or never forget.  So the
+// complement C = 1 - A of a span is summed beside A, C + A keep a row; where it is below a half, A is 1 - C and the rest that this
+// rounding left, and h = A h + (rest h + B) rounds once.  Within eight rows, whose errors end with their span, f is used as it is.
 #include "common.h"
+#include <cfloat>
 
 namespace {
 
@@ -31,13 +35,15 @@ constexpr int SC_TILE = 64;      // rows of a tile, and the distance of the kept
 constexpr int NT = 2;            // buffer accesses: non-temporal
 constexpr float LOG2E = 1.4426950408889634f;
 
+struct Pair;
+
 struct ScanK {
   const void *x, *g, *dh;        // [n][l][ld]
   void *h, *dx, *dg;             // [n][l][c]
   const float *h0, *dlast;       // [n][c] or null
   float *last, *dh0;             // [n][c] or null
   float* states;                 // [n][tiles][c] or null: state in front of every tile
-  float2* agg;                   // [n][segs][c] pairs, or null (one segment)
+  Pair* agg;                     // [n][segs][c], or null (one segment)
   long long x_ns, x_ld, g_ns, g_ld, dh_ns, dh_ld;
   int n, l, c, tiles, segs, seg_tiles, ncb, reverse;
 };
@@ -70,6 +76,36 @@ __device__ __forceinline__ void gate(float g, float& f, float& keep) {     // f 
   f = g >= 0.f ? big : small;
   keep = g >= 0.f ? small : big;
 }
+
+// h -> (a + rest) h + b.  a is rounded down, so that an infinite h meets a positive rest and stays as it is.
+struct Pair { float a, rest, b; };
+__device__ __forceinline__ float apply(const Pair& p, float h) { return fmaf(p.a, h, fmaf(p.rest, h, p.b)); }
+// 1 - c (c at most a half) as a + rest
+__device__ __forceinline__ void complement(float c, float& a, float& rest) {
+  a = 1.f - (c + 0x1p-25f);
+  rest = fmaxf((1.f - a) - c, FLT_MIN);
+}
+// A span as it grows in walk order: A, its complement, B
+template <int V> struct Span {
+  float a[V], c[V], b[V];
+  __device__ __forceinline__ Span() {
+#pragma unroll
+    for (int v = 0; v < V; ++v) { a[v] = 1.f; c[v] = 0.f; b[v] = 0.f; }
+  }
+  __device__ __forceinline__ void grow(int v, float f, float keep) {
+    c[v] = fmaf(keep, a[v], c[v]);
+    a[v] *= f;
+  }
+  __device__ __forceinline__ void then(int v, const Pair& q) {          // a span behind this one
+    grow(v, q.a, (1.f - q.a) - q.rest);
+    b[v] = apply(q, b[v]);
+  }
+  __device__ __forceinline__ Pair pair(int v) const {
+    Pair q = {a[v], FLT_MIN, b[v]};
+    if (c[v] < 0.5f) complement(c[v], q.a, q.rest);
+    return q;
+  }
+};
 
 // One tensor [l][ld] of a window, as a thread walks it: R rows at `row` (a multiple of R inside the tile) of V channels.  Whole
 // tiles go through buffer instructions: the tile's base and the rows' offsets are scalars, a lane holds one 32-bit offset.
@@ -140,39 +176,33 @@ template <typename T, int V, int R> struct Walk {
 };
 
 // Start value of segment `seg`: the pairs of the segments before it (walk order DIR) applied to `s`.  Each group composes a
-// contiguous share of them, the groups' pairs meet in LDS (`a`, `b`, free again after the call).
+// contiguous share of them, the groups' pairs meet in LDS (`sp`, free again after the call).
 template <int V, int CL, int DIR>
-__device__ __forceinline__ void compose(const ScanK& p, int n, int c, int seg, int grp, float (*a)[CL * V], float (*b)[CL * V], float (&s)[V]) {
+__device__ __forceinline__ void compose(const ScanK& p, int n, int c, int seg, int grp, Pair (*sp)[CL * V], float (&s)[V]) {
   constexpr int G = SC_THREADS / CL;
   if (!p.agg) return;                              // uniform
   const int cl = threadIdx.x % CL, before = DIR > 0 ? seg : p.segs - 1 - seg, share = (before + G - 1) / G;
   const int lo = min(before, grp * share), hi = min(before, lo + share);
-  const float2* q = p.agg + ((long long)n * p.segs + (DIR > 0 ? 0 : p.segs - 1)) * p.c + c;       // k-th pair in walk order: q[DIR * k * c]
-  float A[V], B[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
+  const Pair* q = p.agg + ((long long)n * p.segs + (DIR > 0 ? 0 : p.segs - 1)) * p.c + c;       // k-th pair in walk order: q[DIR * k * c]
+  Span<V> span;
 #pragma unroll 4
   for (int k = lo; k < hi; ++k)
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float2 ab = q[(long long)DIR * k * p.c + v];
-      A[v] *= ab.x;
-      B[v] = fmaf(ab.x, B[v], ab.y);
-    }
+    for (int v = 0; v < V; ++v) span.then(v, q[(long long)DIR * k * p.c + v]);
 #pragma unroll
-  for (int v = 0; v < V; ++v) { a[grp][cl * V + v] = A[v]; b[grp][cl * V + v] = B[v]; }
+  for (int v = 0; v < V; ++v) sp[grp][cl * V + v] = span.pair(v);
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < G; ++k)
 #pragma unroll
-    for (int v = 0; v < V; ++v) s[v] = fmaf(a[k][cl * V + v], s[v], b[k][cl * V + v]);
+    for (int v = 0; v < V; ++v) s[v] = apply(sp[k][cl * V + v], s[v]);
   __syncthreads();
 }
 
 template <typename T, int V, int CL>
 __global__ __launch_bounds__(SC_THREADS) void scan_fwd_kernel(const ScanK p) {
   constexpr int G = SC_THREADS / CL, R = SC_TILE / G;
-  __shared__ float sa[2][G][CL * V], sb[2][G][CL * V];
+  __shared__ Pair sp[2][G][CL * V];
   const int cl = threadIdx.x % CL, grp = threadIdx.x / CL;
   const int n = blockIdx.x / p.ncb, c = (blockIdx.x % p.ncb) * CL * V + cl * V;
   const int seg = blockIdx.y;
@@ -189,15 +219,14 @@ __global__ __launch_bounds__(SC_THREADS) void scan_fwd_kernel(const ScanK p) {
   float s[V];                                      // state in front of the tile (the same in every group)
 #pragma unroll
   for (int v = 0; v < V; ++v) s[v] = p.h0 ? p.h0[(long long)n * p.c + cc + v] : 0.f;
-  compose<V, CL, 1>(p, n, cc, seg, grp, sa[0], sb[0], s);
+  compose<V, CL, 1>(p, n, cc, seg, grp, sp[0], s);
 
   auto work = [&](int tile, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
     const int buf = tile & 1, t0 = tile * SC_TILE + grp * R;
-    float f[R][V], b[R][V], A[V], B[V];
+    float f[R][V], b[R][V];
+    Span<V> span;
     if (!WHOLE) { rx.load_cut(qx, t0); rg.load_cut(qg, t0); }
-#pragma unroll
-    for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float xv[V], gv[V];
@@ -208,14 +237,14 @@ __global__ __launch_bounds__(SC_THREADS) void scan_fwd_kernel(const ScanK p) {
         float keep;
         gate(gv[v], f[i][v], keep);
         b[i][v] = keep * xv[v];
-        if (!WHOLE && t0 + i >= p.l) { f[i][v] = 1.f; b[i][v] = 0.f; }
-        A[v] *= f[i][v];
-        B[v] = fmaf(f[i][v], B[v], b[i][v]);
+        if (!WHOLE && t0 + i >= p.l) { f[i][v] = 1.f; keep = b[i][v] = 0.f; }
+        span.grow(v, f[i][v], keep);
+        span.b[v] = fmaf(f[i][v], span.b[v], b[i][v]);
       }
     }
     if (WHOLE && tile + 1 < full) { rx.load(qx, tile + 1); rg.load(qg, tile + 1); }
 #pragma unroll
-    for (int v = 0; v < V; ++v) { sa[buf][grp][cl * V + v] = A[v]; sb[buf][grp][cl * V + v] = B[v]; }
+    for (int v = 0; v < V; ++v) sp[buf][grp][cl * V + v] = span.pair(v);
     if (p.states && grp == 0 && ok) {
       float* st = p.states + ((long long)n * p.tiles + tile) * p.c + c;
 #pragma unroll
@@ -230,7 +259,7 @@ __global__ __launch_bounds__(SC_THREADS) void scan_fwd_kernel(const ScanK p) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (k == grp) mine[v] = s[v];
-        s[v] = fmaf(sa[buf][k][cl * V + v], s[v], sb[buf][k][cl * V + v]);
+        s[v] = apply(sp[buf][k][cl * V + v], s[v]);
       }
     if (ok) {
 #pragma unroll
@@ -253,7 +282,8 @@ __global__ __launch_bounds__(SC_THREADS) void scan_fwd_kernel(const ScanK p) {
 template <typename T, int V, int CL>
 __global__ __launch_bounds__(SC_THREADS, 2) void scan_bwd_kernel(const ScanK p) {
   constexpr int G = SC_THREADS / CL, R = SC_TILE / G;
-  __shared__ float sa[2][G][CL * V], sb[2][G][CL * V], sm[2][G][CL * V];
+  __shared__ Pair sp[2][G][CL * V];
+  __shared__ float sm[2][G][CL * V];
   const int cl = threadIdx.x % CL, grp = threadIdx.x / CL;
   const int n = blockIdx.x / p.ncb, c = (blockIdx.x % p.ncb) * CL * V + cl * V;
   const int seg = blockIdx.y;
@@ -279,19 +309,20 @@ __global__ __launch_bounds__(SC_THREADS, 2) void scan_bwd_kernel(const ScanK p) 
   float mu[V];                                     // f lam of the row behind the tile
 #pragma unroll
   for (int v = 0; v < V; ++v) mu[v] = p.dlast ? p.dlast[(long long)n * p.c + cc + v] : 0.f;
-  compose<V, CL, -1>(p, n, cc, seg, grp, sa[0], sb[0], mu);
+  compose<V, CL, -1>(p, n, cc, seg, grp, sp[0], mu);
 
   auto work = [&](int tile, auto whole) {
     constexpr bool WHOLE = decltype(whole)::value;
     const int buf = tile & 1, t0 = tile * SC_TILE + grp * R;
-    float f[R][V], keep[R][V], xv[R][V], d[R][V], A[V], B[V], M[V], s[V];
+    float f[R][V], keep[R][V], xv[R][V], d[R][V], M[V], s[V];
+    Span<V> span;
     if (!WHOLE) {
       rx.load_cut(qx, t0); rg.load_cut(qg, t0); rd.load_cut(qd, t0);
 #pragma unroll
       for (int v = 0; v < V; ++v) s0[v] = st[(long long)tile * p.c + v];
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; M[v] = 0.f; s[v] = s0[v]; }
+    for (int v = 0; v < V; ++v) { M[v] = 0.f; s[v] = s0[v]; }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float gv[V];
@@ -302,8 +333,8 @@ __global__ __launch_bounds__(SC_THREADS, 2) void scan_bwd_kernel(const ScanK p) 
       for (int v = 0; v < V; ++v) {
         gate(gv[v], f[i][v], keep[i][v]);
         if (!WHOLE && t0 + i >= p.l) { f[i][v] = 1.f; keep[i][v] = 0.f; }          // (x and dh read as zero there)
-        A[v] *= f[i][v];
-        B[v] = fmaf(f[i][v], B[v], keep[i][v] * xv[i][v]);
+        span.grow(v, f[i][v], keep[i][v]);
+        span.b[v] = fmaf(f[i][v], span.b[v], keep[i][v] * xv[i][v]);
       }
     }
 #pragma unroll
@@ -313,8 +344,7 @@ __global__ __launch_bounds__(SC_THREADS, 2) void scan_bwd_kernel(const ScanK p) 
     if (tile > first) load(tile - 1);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      sa[buf][grp][cl * V + v] = A[v];
-      sb[buf][grp][cl * V + v] = B[v];
+      sp[buf][grp][cl * V + v] = span.pair(v);
       sm[buf][grp][cl * V + v] = M[v];
     }
     __syncthreads();
@@ -325,7 +355,7 @@ __global__ __launch_bounds__(SC_THREADS, 2) void scan_bwd_kernel(const ScanK p) 
     for (int k = 0; k < G - 1; ++k)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        run[v] = fmaf(sa[buf][k][cl * V + v], run[v], sb[buf][k][cl * V + v]);
+        run[v] = apply(sp[buf][k][cl * V + v], run[v]);
         if (k + 1 == grp) s[v] = run[v];
       }
 #pragma unroll
@@ -333,7 +363,8 @@ __global__ __launch_bounds__(SC_THREADS, 2) void scan_bwd_kernel(const ScanK p) 
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if (k == grp) m[v] = mu[v];
-        mu[v] = fmaf(sa[buf][k][cl * V + v], mu[v], sm[buf][k][cl * V + v]);
+        const Pair q = sp[buf][k][cl * V + v];
+        mu[v] = apply({q.a, q.rest, sm[buf][k][cl * V + v]}, mu[v]);
       }
     // forward through the rows: h_{t-1} - x_t takes the place of x_t
 #pragma unroll
@@ -379,7 +410,7 @@ __global__ __launch_bounds__(SC_THREADS, 2) void scan_bwd_kernel(const ScanK p) 
 template <typename T, int V, int CL, bool BWD>
 __global__ __launch_bounds__(SC_THREADS) void scan_segment_kernel(const ScanK p) {
   constexpr int G = SC_THREADS / CL, R = 8;
-  __shared__ float sa[G][CL * V], sb[G][CL * V];
+  __shared__ Pair sp[G][CL * V];
   const int cl = threadIdx.x % CL, grp = threadIdx.x / CL;
   const int n = blockIdx.x / p.ncb, c = (blockIdx.x % p.ncb) * CL * V + cl * V;
   const int seg = blockIdx.y;
@@ -391,12 +422,11 @@ __global__ __launch_bounds__(SC_THREADS) void scan_segment_kernel(const ScanK p)
   const int row0 = seg * p.seg_tiles * SC_TILE, row1 = min(p.l, row0 + p.seg_tiles * SC_TILE);
   const int per = ((row1 - row0 + G - 1) / G + R - 1) / R * R;
   const int lo = min(row1, row0 + grp * per), hi = min(row1, lo + per);
-  float A[V], B[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) { A[v] = 1.f; B[v] = 0.f; }
+  Span<V> span;
   Walk<T, V, R> ry[2], rg[2];
   auto take = [&](int slot, int rows, auto whole) {              // `rows` of the batch exist
     constexpr bool WHOLE = decltype(whole)::value;
+    Span<V> batch;                                               // R rows, then part of the span
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       const int i = BWD ? R - 1 - j : j;
@@ -408,11 +438,13 @@ __global__ __launch_bounds__(SC_THREADS) void scan_segment_kernel(const ScanK p)
         float f, keep;
         gate(gv[v], f, keep);
         if (WHOLE || i < rows) {
-          A[v] *= f;
-          B[v] = BWD ? f * (B[v] + yv[v]) : fmaf(f, B[v], keep * yv[v]);
+          batch.grow(v, f, keep);
+          batch.b[v] = BWD ? f * (batch.b[v] + yv[v]) : fmaf(f, batch.b[v], keep * yv[v]);
         }
       }
     }
+#pragma unroll
+    for (int v = 0; v < V; ++v) span.then(v, batch.pair(v));
   };
   // batches of R rows, in walk order or (backward) from the last; the short one is the last in walk order
   const int batches = (hi - lo) / R, rest = (hi - lo) - batches * R;
@@ -451,19 +483,15 @@ __global__ __launch_bounds__(SC_THREADS) void scan_segment_kernel(const ScanK p)
     take(0, rest, std::false_type{});
   }
 #pragma unroll
-  for (int v = 0; v < V; ++v) { sa[grp][cl * V + v] = A[v]; sb[grp][cl * V + v] = B[v]; }
+  for (int v = 0; v < V; ++v) sp[grp][cl * V + v] = span.pair(v);
   __syncthreads();
   if (grp == 0 && ok) {
-    float2* out = p.agg + ((long long)n * p.segs + seg) * p.c + c;
+    Pair* out = p.agg + ((long long)n * p.segs + seg) * p.c + c;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      float a = 1.f, b = 0.f;
-      for (int k = 0; k < G; ++k) {
-        const int q = BWD ? G - 1 - k : k;
-        a *= sa[q][cl * V + v];
-        b = fmaf(sa[q][cl * V + v], b, sb[q][cl * V + v]);
-      }
-      out[v] = make_float2(a, b);
+      Span<1> all;
+      for (int k = 0; k < G; ++k) all.then(0, sp[BWD ? G - 1 - k : k][cl * V + v]);
+      out[v] = all.pair(0);
     }
   }
 }
@@ -476,9 +504,12 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const T* x, long long x_
   if (i >= total) return;
   const long long n = i / c;
   const int ch = (int)(i - n * c);
-  float f, keep;
-  gate(to_f32(g[n * g_ld + ch]), f, keep);
-  const float s = fmaf(f, state[i], keep * to_f32(x[n * x_ld + ch]));
+  float keep;
+  Pair row = {0.f, FLT_MIN, 0.f};
+  gate(to_f32(g[n * g_ld + ch]), row.a, keep);
+  if (keep < 0.5f) complement(keep, row.a, row.rest);
+  row.b = keep * to_f32(x[n * x_ld + ch]);
+  const float s = apply(row, state[i]);
   state[i] = s;
   h[i] = from_f32<T>(s);
 }
@@ -547,7 +578,7 @@ extern "C" size_t unet_gated_scan_workspace_bytes(int32_t dtype, int32_t n, int3
   size_t most = 0;
   for (int even = 0; even < 2; ++even) {
     const Plan q = make_plan(dtype, n, l, c, even != 0);
-    const size_t b = q.segs > 1 ? (size_t)n * q.segs * c * sizeof(float2) : 0;
+    const size_t b = q.segs > 1 ? (size_t)n * q.segs * c * sizeof(Pair) : 0;
     most = b > most ? b : most;
   }
   return most;
@@ -561,11 +592,11 @@ extern "C" int unet_gated_scan_fwd(int32_t dtype, const void* x, int64_t x_ns, i
   if (check_pitch("gated_scan_fwd", x_ld) || check_pitch("gated_scan_fwd", g_ld)) return -1;
   const bool even = c % 2 == 0 && even4(x, x_ns, x_ld) && even4(g, g_ns, g_ld) && even4(h, 0, 0);
   const Plan q = make_plan(dtype, n, l, c, even);
-  UNET_REQUIRE(q.segs == 1 || (workspace && ws_bytes >= (size_t)n * q.segs * c * sizeof(float2)),
-               "gated_scan_fwd: workspace of %zu bytes, %zu needed", ws_bytes, (size_t)n * q.segs * c * sizeof(float2));
+  UNET_REQUIRE(q.segs == 1 || (workspace && ws_bytes >= (size_t)n * q.segs * c * sizeof(Pair)),
+               "gated_scan_fwd: workspace of %zu bytes, %zu needed", ws_bytes, (size_t)n * q.segs * c * sizeof(Pair));
   ScanK p = {};
   p.x = x; p.g = g; p.h = h; p.h0 = h0; p.last = last; p.states = states;
-  p.agg = q.segs > 1 ? static_cast<float2*>(workspace) : nullptr;
+  p.agg = q.segs > 1 ? static_cast<Pair*>(workspace) : nullptr;
   p.x_ns = x_ns; p.x_ld = x_ld; p.g_ns = g_ns; p.g_ld = g_ld;
   p.n = n; p.l = l; p.c = c; p.reverse = reverse != 0;
   p.tiles = q.tiles; p.segs = q.segs; p.seg_tiles = q.seg_tiles; p.ncb = q.ncb;
@@ -584,11 +615,11 @@ extern "C" int unet_gated_scan_bwd(int32_t dtype, const void* x, int64_t x_ns, i
   const bool even = c % 2 == 0 && even4(x, x_ns, x_ld) && even4(g, g_ns, g_ld) && even4(dh, dh_ns, dh_ld) && even4(dx, 0, 0) &&
                     even4(dg, 0, 0);
   const Plan q = make_plan(dtype, n, l, c, even);
-  UNET_REQUIRE(q.segs == 1 || (workspace && ws_bytes >= (size_t)n * q.segs * c * sizeof(float2)),
-               "gated_scan_bwd: workspace of %zu bytes, %zu needed", ws_bytes, (size_t)n * q.segs * c * sizeof(float2));
+  UNET_REQUIRE(q.segs == 1 || (workspace && ws_bytes >= (size_t)n * q.segs * c * sizeof(Pair)),
+               "gated_scan_bwd: workspace of %zu bytes, %zu needed", ws_bytes, (size_t)n * q.segs * c * sizeof(Pair));
   ScanK p = {};
   p.x = x; p.g = g; p.dh = dh; p.dx = dx; p.dg = dg; p.dlast = dlast; p.dh0 = dh0; p.states = const_cast<float*>(states);
-  p.agg = q.segs > 1 ? static_cast<float2*>(workspace) : nullptr;
+  p.agg = q.segs > 1 ? static_cast<Pair*>(workspace) : nullptr;
   p.x_ns = x_ns; p.x_ld = x_ld; p.g_ns = g_ns; p.g_ld = g_ld; p.dh_ns = dh_ns; p.dh_ld = dh_ld;
   p.n = n; p.l = l; p.c = c; p.reverse = reverse != 0;
   p.tiles = q.tiles; p.segs = q.segs; p.seg_tiles = q.seg_tiles; p.ncb = q.ncb;

@@ -1785,8 +1785,9 @@ def gated_scan(x: Tensor, gate: Tensor, h0: Optional[Tensor] = None, reverse: bo
     ``x`` and ``gate``: bf16 or fp32, both of one dtype; windows and rows may be strided (column ranges of one projection).
     ``h0`` ``[N, C]`` fp32: the state in front of the first row (default zeros).  ``reverse``: walk from the last row to the
     first.  Returns ``h`` ``[N, L, C]`` in ``x``'s dtype, and with ``return_state`` also the state after the last row walked,
-    ``[N, C]`` fp32 (pass it as ``h0`` of the next piece of a long recording).  The state is fp32 throughout.  Differentiable
-    (once) in ``x``, ``gate`` and ``h0``."""
+    ``[N, C]`` fp32 (pass it as ``h0`` of the next piece of a long recording).  The state is fp32 throughout, and
+    memories of any length keep their rate (1 - f is not rounded beside 1); what a row changes by less than half an ulp of the state is
+    lost in ``gated_scan_step``, and within 8 rows here.  Differentiable (once) in ``x``, ``gate`` and ``h0``."""
     _check_scan("gated_scan", x, gate, h0, 3)
     if x.numel() == 0:                      # nothing to launch: empty rows leave the state as it was
         h = x * torch.sigmoid(gate)
