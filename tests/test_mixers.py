@@ -182,3 +182,34 @@ def test_training_run_with_8bit_moments(kind):
     other.step(ob, tgt, ids)
     for (name, a), b in zip(eager_model.named_parameters(), other_model.parameters()):
         assert torch.equal(a, b), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("bidirectional", [False, True])
+def test_recurrence_alone_follows_its_optimizer(bits, bidirectional):
+    """A module of its own, in the mode it is born in: every call without gradients sees the weights of the last step (the native
+    optimizer writes them without telling their version counters), as does an eval() after it."""
+    from unet_amd.optim import ClipAdamW
+    m = _module("recurrent", 64, bidirectional=bidirectional)
+    opt = ClipAdamW(m.parameters(), lr=0.05, state_bits=bits)
+    x = torch.randn(2, 64, 50, device="cuda")
+
+    def calls(mod):
+        with torch.no_grad():
+            out = [mod(x)]
+            if not bidirectional:
+                state = torch.zeros(2, 64, device="cuda")
+                out += [mod.forward_step(x[:, :, 0], state), state]
+        return out
+
+    for it in range(4):
+        if it == 3:
+            m.eval()
+        fresh = _module("recurrent", 64, seed=1, bidirectional=bidirectional)
+        fresh.load_state_dict(m.state_dict())
+        for a, b in zip(calls(m), calls(fresh)):
+            assert torch.equal(a, b), it
+        opt.zero_grad()
+        m(x).square().sum().backward()
+        opt.step()

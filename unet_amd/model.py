@@ -267,9 +267,10 @@ class GatedRecurrence1D(nn.Module):
             ops.clear_pack_cache()          # as CondUNet1D.train: fused optimizers do not bump the parameters' versions
         return super().train(mode)
 
-    @staticmethod
-    def _proj(m: nn.Conv1d, x: Tensor, x2: Optional[Tensor] = None) -> Tensor:
-        return ops.conv(x, m.weight.permute(2, 0, 1), m.bias, ops.geom_conv(1), x.shape[1], x2=x2, params=(m.weight, m.bias))
+    def _proj(self, m: nn.Conv1d, x: Tensor, x2: Optional[Tensor] = None) -> Tensor:
+        # packed weights are kept for inference only: between two calls in training mode an optimizer may have written them
+        return ops.conv(x, m.weight.permute(2, 0, 1), m.bias, ops.geom_conv(1), x.shape[1], x2=x2,
+                        params=None if self.training else (m.weight, m.bias))
 
     def forward_nlc(self, x: Tensor) -> Tensor:
         h = [ops.gated_scan(self._proj(v, x), self._proj(f, x), reverse=bool(i)) for i, (v, f) in enumerate(zip(self.value, self.forget))]
