@@ -421,3 +421,45 @@ def test_gradient_norms_that_are_not_finite(bad):
             assert 0 < float((p - p0)[keep].abs().max()) < 4e-3
         else:
             assert bool(torch.isnan(p).all())
+
+
+def check_changed_threshold(dev, step):
+    """min_8bit_numel of a group that has its tables: the next step, or the next look at its buffers, goes by the new value, and
+    no moment is lost on the way."""
+    from unet_amd.optim import ClipAdamW
+    gen = torch.Generator().manual_seed(2)
+    params = [torch.nn.Parameter(torch.randn(s, generator=gen).to(dev)) for s in ((50, 100), (3000,), (10,))]
+    opt = ClipAdamW(params, lr=1e-3, betas=BETAS, weight_decay=0.0, state_bits=8)
+    opt.moment_buffers()
+    step(opt, params, gen)
+    for numel, coded in ((2048, (True, True, False)), (6000, (False, False, False)), (0, (True, True, True)), (4096, (True, False, False))):
+        before = snapshot(opt, params)
+        opt.param_groups[0]["min_8bit_numel"] = numel
+        assert opt.moment_buffers()["exp_avg8"].numel() == sum(-(-p.numel() // BLOCK) * BLOCK for p, c in zip(params, coded) if c)
+        after = snapshot(opt, params)
+        assert tuple(small for _, _, small, _ in after) == coded
+        for p, (m, v, _, t), (m1, v1, _, t1) in zip(params, before, after):
+            assert t == t1
+            flat = torch.nn.functional.pad(torch.stack([m, v.sqrt()]).view(2, -1).abs(), (0, -p.numel() % BLOCK)).view(2, -1, BLOCK)
+            half = 2.0 ** -4 * flat.amax(2).repeat_interleave(BLOCK, 1)[:, :p.numel()].view(2, *p.shape)
+            assert bool(((m1 - m).abs() <= half[0]).all()) and bool(((v1.sqrt() - v.sqrt()).abs() <= half[1]).all())
+        step(opt, params, gen)
+        assert tuple(small for _, _, small, _ in snapshot(opt, params)) == coded
+
+
+def test_a_changed_threshold_takes_effect_on_cpu():
+    def step(opt, params, gen):                 # no kernel here: moments written as a loaded state would be
+        for p in params:
+            st = opt.state[p]
+            if "exp_avg_sq" in st:
+                st["exp_avg"].copy_(torch.randn(p.shape, generator=gen))
+                st["exp_avg_sq"].copy_(torch.rand(p.shape, generator=gen))
+    check_changed_threshold("cpu", step)
+
+
+@pytest.mark.gpu
+def test_a_changed_threshold_takes_effect():
+    def step(opt, params, gen):
+        set_grads(params, gen, 1.0)
+        opt.step()
+    check_changed_threshold("cuda", step)

@@ -123,7 +123,7 @@ class _Group8:
 
     def __init__(self, params: List[torch.nn.Parameter], min_numel: int):
         dev = params[0].device
-        self.params = params
+        self.params, self.min_numel = params, min_numel
         start, slot, blocks, self.end8, self.end32 = [], [], 0, 0, 0
         for p in params:
             if p.dtype != torch.float32 or not p.is_contiguous() or p.device != dev:
@@ -259,7 +259,7 @@ class ClipAdamW(torch.optim.Optimizer):
     def _tables8(self, gi: int, group) -> Optional[_Group8]:
         g = self._groups.get(gi)
         ptrs = [p.data_ptr() for p in group["params"] if p.requires_grad]
-        if not isinstance(g, _Group8) or g.ptrs != ptrs:
+        if not isinstance(g, _Group8) or g.ptrs != ptrs or g.min_numel != group["min_8bit_numel"]:
             params = [p for p in group["params"] if p.requires_grad]
             if not params:
                 return None
@@ -325,7 +325,7 @@ class ClipAdamW(torch.optim.Optimizer):
         ``exp_avg_sq``, tensors padded to 4 elements.  ``state_bits=8``: those hold the tensors below ``min_8bit_numel``; the
         others are in ``exp_avg8`` / ``exp_avg_sq_root8`` (e4m3 codes, tensors padded to 256 elements) with one fp32 scale per
         256 codes in ``exp_avg8_scale`` / ``exp_avg_sq_root8_scale``."""
-        g = self._groups.get(group_index) or self._tables(group_index, self.param_groups[group_index])
+        g = self._tables(group_index, self.param_groups[group_index])
         if g is None:
             return {}
         if not isinstance(g, _Group8):
