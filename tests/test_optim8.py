@@ -463,3 +463,48 @@ def test_a_changed_threshold_takes_effect():
         set_grads(params, gen, 1.0)
         opt.step()
     check_changed_threshold("cuda", step)
+
+
+def check_loaded_codes(dev):
+    """A loaded state is what the checkpoint holds: e4m3 codes at one byte an element, also before the first step; the checkpoint itself is
+    left alone, and a second one saved from it is the same."""
+    from unet_amd.optim import ClipAdamW, quantise_moment
+    gen = torch.Generator().manual_seed(3)
+    params = [torch.nn.Parameter(torch.zeros(s, device=dev)) for s in ((50, 100), (8192,), (10,))]
+    opt = ClipAdamW(params, state_bits=8)
+    saved = opt.state_dict()
+    names = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
+    saved["state"] = {i: dict(zip(names, quantise_moment(torch.randn(s, generator=gen), False) +
+                                  quantise_moment(torch.rand(s, generator=gen), True)), step=torch.tensor(4.0))
+                      for i, s in enumerate(((50, 100), (8192,)))}
+    keep = copy.deepcopy(saved)
+    for bits in (8, 32):
+        opt = ClipAdamW(params, state_bits=bits)
+        opt.load_state_dict(saved)
+        again = opt.state_dict()
+        for i in (0, 1):
+            assert set(saved["state"][i]) == set(keep["state"][i]) == set(again["state"][i])
+            for k, t in keep["state"][i].items():
+                for got in (saved["state"][i][k], again["state"][i][k], opt.state[params[i]][k]):
+                    assert got.dtype == t.dtype and torch.equal(got.cpu().float(), t.float()), k
+                if k != "step":
+                    assert opt.state[params[i]][k].device == params[i].device
+        buf = opt.moment_buffers()
+        if bits == 8:
+            assert torch.equal(buf["exp_avg8"][5120:].cpu().view(torch.uint8), keep["state"][1]["exp_avg"].view(torch.uint8))
+    # codes that an earlier load had cast to fp32 on their way into a file
+    for st in saved["state"].values():
+        for k in ("exp_avg", "exp_avg_sq_root"):
+            st[k] = st[k].float()
+    opt = ClipAdamW(params, state_bits=8)
+    opt.load_state_dict(saved)
+    assert torch.equal(opt.state[params[0]]["exp_avg"].cpu().view(torch.uint8), keep["state"][0]["exp_avg"].view(torch.uint8))
+
+
+def test_loaded_codes_keep_their_type_on_cpu():
+    check_loaded_codes("cpu")
+
+
+@pytest.mark.gpu
+def test_loaded_codes_keep_their_type():
+    check_loaded_codes("cuda")

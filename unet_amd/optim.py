@@ -75,6 +75,7 @@ class _Group:
 
 BLOCK = 256                 # csrc/optim8.hip: elements of a tensor that share one scale
 FP8_MAX, FP8_LEAST = 448.0, 2.0 ** -9
+CODES = ("exp_avg", "exp_avg_sq_root")         # the e4m3 entries of a tensor's state
 TINY = 2.0 ** -100          # a block below this is stored as zeros
 WIDE = 0x80000000           # include/unet_hip.h unet_adamw8_apply: slot of a tensor with fp32 moments
 
@@ -197,15 +198,15 @@ class _Group8:
         coded = [(st, v) for st, v in zip(states, self.views) if "exp_avg_scale" in v]
         if coded and all("exp_avg_scale" in st for st, _ in coded):
             # the usual case, all of the large tensors held in codes already: one gather a buffer
-            for names, flat, code in ((("exp_avg", "exp_avg_sq_root"), (self.m8, self.r8), True),
-                                      (("exp_avg_scale", "exp_avg_sq_root_scale"), (self.m_scale, self.r_scale), False)):
-                for name, buf in zip(names, flat):
-                    parts = []
-                    for st, v in coded:
-                        parts.append(st[name].reshape(-1).float())
-                        if code and v[name].numel() % BLOCK:
-                            parts.append(parts[-1].new_zeros(-v[name].numel() % BLOCK))
-                    buf[:self.end8 if code else self.end8 // BLOCK].copy_(torch.cat(parts))
+            for name, buf in zip(CODES, (self.m8, self.r8)):
+                parts = []
+                for st, v in coded:
+                    parts.append(st[name].reshape(-1).to(torch.float8_e4m3fn).view(torch.uint8))
+                    if v[name].numel() % BLOCK:
+                        parts.append(parts[-1].new_zeros(-v[name].numel() % BLOCK))
+                torch.cat(parts, out=buf[:self.end8].view(torch.uint8))
+            for name, buf in zip(("exp_avg_scale", "exp_avg_sq_root_scale"), (self.m_scale, self.r_scale)):
+                torch.cat([st[name].reshape(-1) for st, _ in coded], out=buf[:self.end8 // BLOCK])
         else:                                   # some of them have not been stepped yet, or come from fp32
             for st, v in coded:
                 if "exp_avg_scale" in st:
@@ -301,12 +302,23 @@ class ClipAdamW(torch.optim.Optimizer):
         return g
 
     def load_state_dict(self, state_dict):
-        """As ``torch.optim.Optimizer.load_state_dict``, except for two things torch's version loses: it replaces
+        """As ``torch.optim.Optimizer.load_state_dict``, except for three things torch's version loses: it replaces
         every param_group by the saved one, so a ``torch.optim.AdamW`` checkpoint of the reference (no
-        ``max_grad_norm`` key) would silently switch the clip off, and a device-scalar ``lr`` (graph-captured steps
-        read it through its pointer) would become a float no captured step sees."""
+        ``max_grad_norm`` key) would silently switch the clip off, a device-scalar ``lr`` (graph-captured steps
+        read it through its pointer) would become a float no captured step sees, and the codes of 8-bit moments would be
+        cast to the parameters' fp32."""
         before = [(g.get("max_grad_norm"), g.get("lr"), g["state_bits"], g["min_8bit_numel"]) for g in self.param_groups]
-        super().load_state_dict(state_dict)
+        bare, codes = dict(state_dict, state={}), {}
+        for i, st in state_dict["state"].items():
+            if "exp_avg_scale" in st:
+                codes[i] = {k: st[k] for k in CODES}
+                st = {k: v for k, v in st.items() if k not in CODES}
+            bare["state"][i] = st
+        super().load_state_dict(bare)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(saved, [p for g in self.param_groups for p in g["params"]]):
+            if i in codes:
+                self.state[p].update({k: t.to(p.device, torch.float8_e4m3fn) for k, t in codes[i].items()})
         for group, (max_norm, lr, bits, min_numel) in zip(self.param_groups, before):
             group["state_bits"], group["min_8bit_numel"] = bits, min_numel     # the moments convert, see _load_moments
             if "max_grad_norm" not in group:
