@@ -508,3 +508,71 @@ def test_loaded_codes_keep_their_type_on_cpu():
 @pytest.mark.gpu
 def test_loaded_codes_keep_their_type():
     check_loaded_codes("cuda")
+
+
+def step_in_torch(p, g, codes, lr, wd, clip, t):
+    """One step of a tensor from its codes in 32-bit torch operations, in the kernel's order: (parameter, codes, scales, size of the
+    parameter's step).  The bias corrections are 64-bit numbers rounded once."""
+    from unet_amd.optim import dequantise_moment
+    b1, b2 = BETAS
+    f32 = lambda v: torch.tensor(v, dtype=torch.float64, device=p.device).float()
+    pad = lambda x: torch.nn.functional.pad(x.reshape(-1), (0, -x.numel() % BLOCK)).view(-1, BLOCK)
+    m, r = (pad(dequantise_moment(*codes[i:i + 2])) for i in (0, 2))
+    gc = pad(g) * clip
+    m = m * f32(b1) + gc * f32(1 - b1)
+    r = torch.sqrt(r * r * f32(b2) + gc * f32(1 - b2) * gc)
+    out = []
+    for x in (m, r):
+        top = x.abs().amax(1, keepdim=True)
+        y = x * ((1.0 / top) * 448.0)
+        if x is r:
+            y = torch.where(r > 0, y.clamp_min(2.0 ** -9), y)
+        out += [y.to(torch.float8_e4m3fn).view(-1)[:p.numel()].view(p.shape), (top * f32(1 / 448).item()).view(-1)]
+    step = f32(lr / (1 - b1 ** t)) * (m / (r * f32(1 / math.sqrt(1 - b2 ** t)) + 1e-8))
+    return p * (1 - f32(lr) * f32(wd)) - step.view(-1)[:p.numel()].view(p.shape), out, step.view(-1)[:p.numel()].view(p.shape)
+
+
+def clip_of(grads, max_norm, ulps=0):
+    """(norm, clip) with the squares summed in 64 bits, and the norm moved by some units in its last place."""
+    norm = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt().float()
+    for _ in range(ulps):
+        norm = torch.nextafter(norm, torch.full_like(norm, math.inf))
+    return norm, torch.clamp(max_norm * (1.0 / (norm + 1e-6)), max=1.0)
+
+
+def test_codes_show_an_ulp_of_the_norm_on_cpu():
+    """What the next test compares is sensitive enough: with a norm a few units off in its last place, as a sum in 32 bits may leave it,
+    some of 2 M codes differ."""
+    gen = torch.Generator().manual_seed(4)
+    g = torch.randn(2 ** 21, generator=gen)
+    zero = [torch.zeros(2 ** 21).to(torch.float8_e4m3fn), torch.zeros(2 ** 13)] * 2
+    a, b = (step_in_torch(torch.zeros(2 ** 21), g, zero, 1e-3, 0.0, clip_of([g], 1.0, ulps)[1], 1)[1] for ulps in (0, 2))
+    assert any(int((x.view(torch.uint8) != y.view(torch.uint8)).sum()) > 0 for x, y in ((a[0], b[0]), (a[2], b[2])))
+    assert not torch.equal(a[1], b[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm,wd", [(1.0, 0.01), (1e6, 0.0)])
+def test_a_clipped_step_has_the_bits_of_32_bit_torch(max_norm, wd):
+    """Codes and scales to the bit, the norm as the rounding of its 64-bit sum; a parameter differs by single roundings.  The step:
+    here the root's product, + eps, the division and the product with lr / (1 - b1^t), 4 u; there one fma, a reciprocal of one unit (2 u), two
+    products, 5 u; and lr is rounded there before it is divided, and both quotients are, 3 u: 12 u.  p keep - step: either side
+    rounds 1 - lr wd (together u), the product and the difference (u each on either side): 5 u of the larger of p before and after."""
+    from unet_amd.optim import ClipAdamW
+    params, gen = make(11, [(1024, 1030), (300, 7, 129), (4097,), (512, 512, 7)])
+    opt = ClipAdamW(params, lr=2e-3, betas=BETAS, weight_decay=wd, max_grad_norm=max_norm, state_bits=8)
+    opt.moment_buffers()
+    names = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
+    for t in (1, 2, 3):
+        set_grads(params, gen, 0.3)
+        norm, clip = clip_of([p.grad for p in params], max_norm)
+        old = [p.detach().clone() for p in params]
+        want = [step_in_torch(p.detach().clone(), p.grad, [opt.state[p][k].clone() for k in names], 2e-3, wd, clip, t) for p in params]
+        opt.step()
+        assert torch.equal(opt.total_norm(), norm)
+        for p, p0, (p1, codes, step) in zip(params, old, want):
+            for k, x in zip(names, codes):
+                got = opt.state[p][k]
+                assert torch.equal(got.view(torch.uint8), x.view(torch.uint8)), (t, k, int((got.float() != x.float()).sum()))
+            off, size = (p.detach().double() - p1.double()).abs(), torch.maximum(p0.double().abs(), p1.double().abs())
+            assert float((off - 5 * U * size - 12 * U * step.double().abs()).max()) <= 0
