@@ -483,3 +483,42 @@ def test_infinite_inputs_stay_infinite(dtype):
         state = last.clone()
         ops.gated_scan_step(x[:, 0], g[:, 0], state)
         assert torch.equal(torch.isinf(state), torch.isinf(last)) and not bool(torch.isnan(state).any())
+
+
+def one_row_views(dev, dtype):
+    """[N, 1, C] whose only row has a stride of 2^23, and [1, C] and [N, C] rows that far apart: views of what a caller holds."""
+    c, far = 8, 1 << 23
+    rows = torch.randn(2 * far, generator=torch.Generator().manual_seed(0)).to(dtype).to(dev)
+    return rows.as_strided((3, 1, c), (c, far, 1)), rows.as_strided((2, c), (far, 1)), rows.as_strided((1, c), (far, 1))
+
+
+def test_strides_of_an_only_row_are_ignored_on_cpu(monkeypatch):
+    """Neither refused (a transposed [1, N, C] has such a stride) nor copied; single rows go in as they are, whatever lies between them."""
+    from unet_amd import ops
+    calls = []
+    monkeypatch.setattr(ops, "_run", lambda *a: calls.append(a))
+    monkeypatch.setattr(ops, "_need_cuda", lambda *a: None)
+    wide, rows, one = one_row_views("cpu", torch.float32)
+    ops.gated_scan(wide, wide)
+    assert calls[0][3:9] == (wide.data_ptr(), 8, 8, wide.data_ptr(), 8, 8)
+    for x in (rows, one):
+        ops.gated_scan_step(x, x, torch.zeros(x.shape))
+        assert calls[-1][3:7] == (x.data_ptr(), 1 << 23, x.data_ptr(), 1 << 23)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_of_an_only_row(dtype):
+    from unet_amd import ops
+    wide, rows, one = one_row_views("cuda", dtype)
+    state = torch.randn(3, 8, device="cuda")
+    dlast = torch.randn(3, 8, device="cuda")
+    got, want = call(wide, wide, state, wide, dlast, True), oracle(wide, wide, state, wide, dlast, True)
+    for k in got:
+        near(got[k], want[k], k)
+    for x in (rows, one):
+        s = state[:x.shape[0]].clone()
+        h = ops.gated_scan_step(x, x, s)
+        w = oracle(x[:, None], x[:, None], state[:x.shape[0]], None, None, False)
+        near(h[:, None], w["h"], "row")
+        near(s, w["last"], "state")

@@ -1705,8 +1705,14 @@ def _once_differentiable(what: str):
 
 
 def _dense_channels(t: Tensor) -> Tensor:
-    """Any window and row stride will do up to 2^22 elements a row; the channels of a row must be adjacent."""
-    return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-2) <= 1 << 22 else t.contiguous()
+    """The channels of a row must be adjacent; any other strides will do, but for rows of a window more than 2^22 elements apart."""
+    dense = t.stride(-1) == 1 or t.shape[-1] == 1
+    return t if dense and (t.dim() == 2 or _scan_pitch(t) <= 1 << 22) else t.contiguous()
+
+
+def _scan_pitch(t: Tensor) -> int:
+    """Row pitch of [N, L, C]; the stride of an only row means nothing and may be anything."""
+    return t.stride(1) if t.shape[1] > 1 else t.shape[2]
 
 
 def _check_scan(what: str, x: Tensor, gate: Tensor, state: Optional[Tensor], dims: int):
@@ -1740,8 +1746,8 @@ def _scan_forward(x: Tensor, gate: Tensor, h0: Optional[Tensor], reverse: bool, 
     size, kept = _scan_sizes(_dt(x), n, l, c)
     states = torch.empty((n, kept, c), dtype=torch.float32, device=x.device) if keep else None
     ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-    _run("unet_gated_scan_fwd", x.device.index, _dt(x), x.data_ptr(), x.stride(0), x.stride(1), gate.data_ptr(), gate.stride(0),
-         gate.stride(1), _ptr(h0), reverse, n, l, c, h.data_ptr(), last.data_ptr(), _ptr(states), _ptr(ws), size)
+    _run("unet_gated_scan_fwd", x.device.index, _dt(x), x.data_ptr(), x.stride(0), _scan_pitch(x), gate.data_ptr(), gate.stride(0),
+         _scan_pitch(gate), _ptr(h0), reverse, n, l, c, h.data_ptr(), last.data_ptr(), _ptr(states), _ptr(ws), size)
     return h, last, states
 
 
@@ -1771,8 +1777,8 @@ class GatedScanFn(torch.autograd.Function):
         dh0 = torch.empty((n, c), dtype=torch.float32, device=x.device) if ctx.needs_input_grad[2] else None
         size, _ = _scan_sizes(_dt(x), n, l, c)
         ws = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
-        _run("unet_gated_scan_bwd", x.device.index, _dt(x), x.data_ptr(), x.stride(0), x.stride(1), gate.data_ptr(), gate.stride(0),
-             gate.stride(1), states.data_ptr(), dh.data_ptr(), dh.stride(0), dh.stride(1), _ptr(dlast), ctx.reverse, n, l, c,
+        _run("unet_gated_scan_bwd", x.device.index, _dt(x), x.data_ptr(), x.stride(0), _scan_pitch(x), gate.data_ptr(), gate.stride(0),
+             _scan_pitch(gate), states.data_ptr(), dh.data_ptr(), dh.stride(0), _scan_pitch(dh), _ptr(dlast), ctx.reverse, n, l, c,
              dx.data_ptr(), dg.data_ptr(), _ptr(dh0), _ptr(ws), size)
         return dx, dg, dh0, None
 
