@@ -522,3 +522,33 @@ def test_strides_of_an_only_row(dtype):
         w = oracle(x[:, None], x[:, None], state[:x.shape[0]], None, None, False)
         near(h[:, None], w["h"], "row")
         near(s, w["last"], "state")
+
+
+def test_sizes_past_the_librarys_counters_are_refused_on_cpu(monkeypatch):
+    """2^32 + 5 rows are not 5 rows, and a launch holds 2^32 threads."""
+    from unet_amd import _lib, ops
+    monkeypatch.setattr(ops, "_run", lambda *a: pytest.fail("called"))
+    monkeypatch.setattr(ops, "_need_cuda", lambda *a: None)
+    for shape in ((1, (1 << 32) + 5, 1), ((1 << 32) + 5, 1, 1)):
+        x = torch.zeros(1).expand(shape)
+        with pytest.raises(ValueError, match="below 2\\^31"):
+            ops.gated_scan(x, x)
+    x, state = torch.zeros(1).expand(1 << 31, 1), torch.zeros(1).expand(1 << 31, 1)
+    with pytest.raises(ValueError, match="below 2\\^31"):
+        ops.gated_scan_step(x, x, state)
+    for shape in ((1, (1 << 32) + 8, 8), ((1 << 32) + 1, 1, 8)):
+        q = torch.zeros(1).expand(shape)
+        with pytest.raises(ValueError, match="below 2\\^31"):
+            ops.rel_bias_attention(q, q, q, torch.zeros(8, 1), 1, max_distance=5)
+    lib = _lib.load()
+    for dtype, n in ((1, 1 << 23), (0, 1 << 23)):
+        assert lib.unet_gated_scan_fwd(dtype, 16, 1, 1, 16, 1, 1, None, 0, n, 1, 1, 16, None, None, None, 0, None) == -1
+        assert b"2^32 threads" in lib.unet_last_error()
+        assert lib.unet_gated_scan_bwd(dtype, 16, 1, 1, 16, 1, 1, 16, 16, 1, 1, None, 0, n, 1, 1, 16, 16, None, None, 0, None) == -1
+        assert b"2^32 threads" in lib.unet_last_error()
+        assert lib.unet_gated_scan_step(dtype, 16, 1 << 20, 16, 1 << 20, 16, 16, 1 << 12, 1 << 20, None) == -1
+        assert b"2^32 threads" in lib.unet_last_error()
+        st = (C.c_int32 * 2)(0, 1)
+        rows = 129 if dtype == 0 else 65
+        assert lib.unet_rel_attn_fwd(dtype, 16, 16, 16, 16, 1, 4, st, None, 65535, rows, 2048, 256, 1.0, 16, None, None, None, 0, None) == -1
+        assert b"workgroups" in lib.unet_last_error()

@@ -955,7 +955,8 @@ int make_rel(const char* what, RelK& p, int32_t dtype, int32_t n, int32_t l, int
                "%s: head_dim %d must be a multiple of %d and at most 256 (c=%d heads=%d)", what, c / nh, unit, c, nh);
   UNET_REQUIRE((long long)l * c * (dtype == UNET_BF16 ? 2 : 4) < (1ll << 31), "%s: one [L, C] slab of %lld bytes exceeds a buffer descriptor",
                what, (long long)l * c * (dtype == UNET_BF16 ? 2 : 4));
-  UNET_REQUIRE((long long)n * nh * cdiv(l, 32) < (1ll << 31), "%s: grid too large", what);
+  UNET_REQUIRE((long long)n * nh * cdiv(l, dtype == UNET_BF16 ? AT_BQ : 64) < (1ll << 24),      // 256 threads each, counted in 32 bits
+               "%s: n=%d windows of l=%d rows with %d heads take 2^24 workgroups or more", what, n, l, nh);
   UNET_REQUIRE(scale > 0.f && scale * REL_LOG2E < INFINITY, "%s: scale must be positive and finite (also times log2 e), got %g", what,
                (double)scale);
   UNET_REQUIRE(buckets >= 4 && buckets % 2 == 0 && buckets <= 2 * UNET_REL_MAX_SIDE, "%s: %d buckets, must be even and 4 .. %d", what,

@@ -546,6 +546,12 @@ int check_scan(const char* what, int32_t dtype, int64_t n, int64_t l, int64_t c)
   return 0;
 }
 
+// threads of a launch are counted in 32 bits
+int check_grid(const char* what, long long workgroups, int threads) {
+  UNET_REQUIRE(workgroups * threads < (1ll << 32), "%s: %lld workgroups of %d threads, at most 2^32 threads in all", what, workgroups, threads);
+  return 0;
+}
+
 // a tile's rows lie within one buffer descriptor's 31 bits
 int check_pitch(const char* what, int64_t ld) {
   UNET_REQUIRE(ld >= 0 && ld <= (1ll << 22), "%s: row pitch %lld, must be 0 .. 2^22 elements", what, (long long)ld);
@@ -592,6 +598,7 @@ extern "C" int unet_gated_scan_fwd(int32_t dtype, const void* x, int64_t x_ns, i
   if (check_pitch("gated_scan_fwd", x_ld) || check_pitch("gated_scan_fwd", g_ld)) return -1;
   const bool even = c % 2 == 0 && even4(x, x_ns, x_ld) && even4(g, g_ns, g_ld) && even4(h, 0, 0);
   const Plan q = make_plan(dtype, n, l, c, even);
+  if (check_grid("gated_scan_fwd", (long long)n * q.ncb, SC_THREADS)) return -1;
   UNET_REQUIRE(q.segs == 1 || (workspace && ws_bytes >= (size_t)n * q.segs * c * sizeof(Pair)),
                "gated_scan_fwd: workspace of %zu bytes, %zu needed", ws_bytes, (size_t)n * q.segs * c * sizeof(Pair));
   ScanK p = {};
@@ -615,6 +622,7 @@ extern "C" int unet_gated_scan_bwd(int32_t dtype, const void* x, int64_t x_ns, i
   const bool even = c % 2 == 0 && even4(x, x_ns, x_ld) && even4(g, g_ns, g_ld) && even4(dh, dh_ns, dh_ld) && even4(dx, 0, 0) &&
                     even4(dg, 0, 0);
   const Plan q = make_plan(dtype, n, l, c, even);
+  if (check_grid("gated_scan_bwd", (long long)n * q.ncb, SC_THREADS)) return -1;
   UNET_REQUIRE(q.segs == 1 || (workspace && ws_bytes >= (size_t)n * q.segs * c * sizeof(Pair)),
                "gated_scan_bwd: workspace of %zu bytes, %zu needed", ws_bytes, (size_t)n * q.segs * c * sizeof(Pair));
   ScanK p = {};
@@ -633,6 +641,7 @@ extern "C" int unet_gated_scan_step(int32_t dtype, const void* x, int64_t x_ld, 
   if (check_scan("gated_scan_step", dtype, n, 1, c)) return -1;
   UNET_REQUIRE(x && g && state && h, "gated_scan_step: null pointer");
   const long long total = (long long)n * c;
+  if (check_grid("gated_scan_step", (total + 255) / 256, 256)) return -1;
   const dim3 grid((unsigned)((total + 255) / 256));
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == UNET_F32)

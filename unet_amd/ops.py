@@ -1715,6 +1715,12 @@ def _scan_pitch(t: Tensor) -> int:
     return t.stride(1) if t.shape[1] > 1 else t.shape[2]
 
 
+def _check_sizes(what: str, t: Tensor):
+    """The library counts in 32 bits, and what does not fit would arrive as another number."""
+    if max(t.shape) >= 1 << 31:
+        raise ValueError(f"{what}: every size must be below 2^31, got {tuple(t.shape)}")
+
+
 def _check_scan(what: str, x: Tensor, gate: Tensor, state: Optional[Tensor], dims: int):
     _dt(x)
     if x.dim() != dims or gate.shape != x.shape:
@@ -1728,6 +1734,7 @@ def _check_scan(what: str, x: Tensor, gate: Tensor, state: Optional[Tensor], dim
             raise ValueError(f"{what}: the state must be [N, C] = {(x.shape[0], x.shape[-1])}, got {tuple(state.shape)}")
         if state.dtype != torch.float32 or state.device != x.device:
             raise TypeError(f"{what}: the state must be float32 on {x.device}, got {state.dtype} on {state.device}")
+    _check_sizes(what, x)
     _need_cuda(x)
 
 
@@ -1962,6 +1969,7 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
         if lengths.shape != (n,) or lengths.dtype != torch.int32 or lengths.device != q.device:
             raise ValueError(f"rel_bias_attention: lengths must be int32 [{n}] on {q.device}")
         lengths = lengths.contiguous()
+    _check_sizes("rel_bias_attention", q)
     _need_cuda(q)
     if q.numel() == 0:
         return q * k * v + 0 * table.sum().to(q.dtype)
