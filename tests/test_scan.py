@@ -511,9 +511,11 @@ def test_strides_of_an_only_row_are_ignored_on_cpu(monkeypatch):
 def test_strides_of_an_only_row(dtype):
     from unet_amd import ops
     wide, rows, one = one_row_views("cuda", dtype)
-    state = torch.randn(3, 8, device="cuda")
-    dlast = torch.randn(3, 8, device="cuda")
+    state, dlast = torch.randn(2, 3, 8, generator=torch.Generator().manual_seed(1)).cuda()
     got, want = call(wide, wide, state, wide, dlast, True), oracle(wide, wide, state, wide, dlast, True)
+    # dh passes the gate rounded to 32 bits, dlast the span's a + rest: half an ulp of the gate apart, u relative, which shows where
+    # the two cancel and the bound of their sum does not cover it
+    want["dh0"] = (want["dh0"][0], want["dh0"][1] + U * wide[:, 0].double().cpu().abs())
     for k in got:
         near(got[k], want[k], k)
     for x in (rows, one):
