@@ -554,3 +554,22 @@ def test_sizes_past_the_librarys_counters_are_refused_on_cpu(monkeypatch):
         rows = 129 if dtype == 0 else 65
         assert lib.unet_rel_attn_fwd(dtype, 16, 16, 16, 16, 1, 4, st, None, 65535, rows, 2048, 256, 1.0, 16, None, None, None, 0, None) == -1
         assert b"workgroups" in lib.unet_last_error()
+
+
+@pytest.mark.gpu
+def test_rows_up_to_the_last_int():
+    """2^31 - 4097 rows in 512 segments: the last one would end past 2^31 if it were whole.  Checked where it begins (backward
+    passes its adjoint on) and where it ends."""
+    from unet_amd import ops
+    l = 2 ** 31 - 4097
+    gen = torch.Generator(device="cuda").manual_seed(41)
+    x, g, dh = (torch.randn((1, l, 1), generator=gen, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+    h, last = ops.gated_scan(x.requires_grad_(), g.requires_grad_(), return_state=True)
+    dx, dg = torch.autograd.grad(h, (x, g), dh)
+    for mid, hi in ((511 * 65536 * 64, 511 * 65536 * 64 + 300), (l - 200, l)):
+        cut = slice(mid - 600, hi)             # 300 rows on either side forget what lies beyond them
+        want = oracle(x.detach()[:, cut], g.detach()[:, cut], None, dh[:, cut], None, False)
+        inner = slice(300, 700 if hi < l else None)
+        for k, t in (("h", h), ("dx", dx), ("dg", dg)):
+            near(t[:, cut][:, inner], tuple(v[:, inner] for v in want[k]), (k, mid))
+    near(last, want["last"], "last")

@@ -419,7 +419,7 @@ __global__ __launch_bounds__(SC_THREADS) void scan_segment_kernel(const ScanK p)
   const T* g = static_cast<const T*>(p.g) + n * p.g_ns + cc;
   const T* y = BWD ? static_cast<const T*>(p.dh) + n * p.dh_ns + cc : static_cast<const T*>(p.x) + n * p.x_ns + cc;
   const long long y_ld = BWD ? p.dh_ld : p.x_ld;
-  const int row0 = seg * p.seg_tiles * SC_TILE, row1 = min(p.l, row0 + p.seg_tiles * SC_TILE);
+  const int row0 = seg * p.seg_tiles * SC_TILE, row1 = row0 + min(p.l - row0, p.seg_tiles * SC_TILE);
   const int per = ((row1 - row0 + G - 1) / G + R - 1) / R * R;
   const int lo = min(row1, row0 + grp * per), hi = min(row1, lo + per);
   Span<V> span;
