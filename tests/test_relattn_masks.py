@@ -96,3 +96,34 @@ def test_rows_that_see_only_a_finite_mask(l, hd, name, fill, dtype):
 def test_finite_masks_in_a_padded_batch(fill, dtype):
     check(300, 32, dtype, "far_behind_open", fill, lengths=[300, 0, 129, 1])
     check(200, 32, dtype, "all", fill, lengths=[77, 200])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("top", [1e9, torch.finfo(torch.float32).max])
+@pytest.mark.parametrize("l,hd", [(100, 32), (1600, 64)])
+def test_biases_of_the_highest_value(l, hd, top, dtype):
+    """The other end: where two far buckets hold a bias beside which scores vanish, every row weighs the keys of those alike, as if the
+    others were removed."""
+    q, k, v, table, dout = inputs(1, l, 2, hd, 16, dtype, seed=l)
+    q = q / 4
+    t, only = table.clone(), torch.full_like(table, -math.inf)
+    t[[7, 15]] = top
+    got = call(q, k, v, t, dout, n_heads=2, max_distance=30)
+    # equal scores: those of q = 0 and a zero bias; dk needs q, so the rows' share of it is rebuilt from dS = P (dP - delta)
+    only[[7, 15]] = 0.0
+    want = oracle(torch.zeros_like(q), k, v, only, 2, hd ** -0.5, 30, None, dout)
+    for key in ("out", "dq", "dv", "dtable"):
+        near(got[key], want[key], (key, top))
+    real = oracle(q, k, v, only, 2, hd ** -0.5, 30, None, dout)["dk"][1]
+    row = torch.tensor([bucket_by_definition(o, 16, 30) for o in range(1 - l, l)], device="cuda")
+    pos = torch.arange(l, device="cuda")
+    far = torch.isin(row[pos[None, :] - pos[:, None] + l - 1], torch.tensor([7, 15], device="cuda")).double()
+    P = far / far.sum(1, keepdim=True)
+    dk = torch.zeros_like(real)
+    for h in range(2):
+        cols = slice(h * hd, (h + 1) * hd)
+        Q, V, D = (x[0, :, cols].double() for x in (q, v, dout))
+        dP = D @ V.T
+        dk[0, :, cols] = hd ** -0.5 * (P * (dP - (P * dP).sum(1, keepdim=True))).T @ Q
+    near(got["dk"], (dk, real), ("dk", top))

@@ -34,21 +34,22 @@ namespace {
 __host__ __forceinline__ int rel32_rows(int n, int l, int nh, int hd) { return hd <= 128 && (long long)n * nh * cdiv(l, 64) <= 128 ? 16 : 64; }
 
 constexpr float REL_LOG2E = 1.4426950408889634f;
-constexpr float REL_LOWEST = -1e30f;    // finite biases stop here (log2 domain): the type's lowest value must not become -inf
+constexpr float REL_LOWEST = -1e30f;    // finite biases stop here and at 1e30: the type's lowest and highest values, or sums with them,
+                                        // must not become infinite
 // LDS copy of a head's biases by offset: index REL_PAD + sat + offset, flat beyond +-sat for REL_PAD entries each way, so a
 // tile that touches the band between -sat and sat reads it without clamping
 constexpr int REL_PAD = 96;
 __device__ __host__ __forceinline__ int rel_width(int sat) { return (2 * sat + 1 + 2 * REL_PAD + 3) & ~3; }      // 16-byte multiple
 
 // Bias of key j seen from query i, off = j - i, times `unit`: log2(e) for scores in the log2 domain (bf16), 1 for natural ones
-// (fp32).  A NaN entry stays NaN; a finite one is held above REL_LOWEST (the type's lowest value times log2(e), or with a score
-// added, would be -inf, which means "never").
+// (fp32).  An infinite entry or a NaN stays what it is; a finite one is held within +-1e30 (the type's lowest value times log2(e), or
+// with a score added, would be -inf, which means "never"; its highest +inf, which makes NaN).
 __device__ __forceinline__ float rel_bias(const RelK& p, int head, int off, float unit = REL_LOG2E) {
   const int a = min(abs(off), p.sat);
   const int b = p.bucket[a] + (off > 0 ? p.buckets >> 1 : 0);
   const float v = p.table_f32 ? static_cast<const float*>(p.table)[b * p.nh + head]
                               : (float)static_cast<const __bf16*>(p.table)[b * p.nh + head];
-  return v == -INFINITY || v != v ? v : fmaxf(v * unit, REL_LOWEST);
+  return fabsf(v) < INFINITY ? fminf(fmaxf(v * unit, REL_LOWEST), -REL_LOWEST) : v;
 }
 
 __device__ __forceinline__ long long rel_logs(const RelK& p) { return (long long)p.n * p.nh * p.l; }      // lse: start of the logs

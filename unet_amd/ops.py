@@ -1941,7 +1941,7 @@ def rel_bias_attention(q: Tensor, k: Tensor, v: Tensor, table: Tensor, n_heads: 
     ``q``, ``k``, ``v``: ``[N, L, C]``, all bf16 or all fp32; head h owns columns ``h*hd .. h*hd+hd-1``, ``hd = C / n_heads`` a
     multiple of 8 (bf16) or 4 (fp32), at most 256; at most 65535 windows.  ``table``: ``[n_buckets, n_heads]`` fp32 or bf16 (``rel_bucket`` gives the
     buckets; ``max_distance`` at most 512); an entry of -inf removes its pairs, and in bf16 a far bucket of -inf also their cost.
-    Finite entries are held above -1e30; a row that sees nothing but a large one (-1e9, the type's lowest value) weighs its keys alike,
+    Finite entries are held within +-1e30; a row that sees nothing but a large one (-1e9, the type's lowest value) weighs its keys alike,
     as the 32-bit sum of bias and score does.
     ``lengths``: ``[N]`` int32 valid positions of a padded batch (values are clamped to 0 .. L): positions behind them are
     neither keys nor queries, their outputs and gradients are zero.  A row with nothing to see gives zeros.  ``scale`` defaults
