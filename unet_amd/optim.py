@@ -337,7 +337,10 @@ class ClipAdamW(torch.optim.Optimizer):
         ``exp_avg_sq``, tensors padded to 4 elements.  ``state_bits=8``: those hold the tensors below ``min_8bit_numel``; the
         others are in ``exp_avg8`` / ``exp_avg_sq_root8`` (e4m3 codes, tensors padded to 256 elements) with one fp32 scale per
         256 codes in ``exp_avg8_scale`` / ``exp_avg_sq_root8_scale``."""
-        g = self._tables(group_index, self.param_groups[group_index])
+        g, group = self._groups.get(group_index), self.param_groups[group_index]
+        eight = group["state_bits"] == 8
+        if g is None or isinstance(g, _Group8) != eight or (eight and g.min_numel != group["min_8bit_numel"]):
+            g = self._tables(group_index, group)      # nothing yet, or other options than the last step's
         if g is None:
             return {}
         if not isinstance(g, _Group8):
