@@ -14,10 +14,10 @@
 // own LDS array by offset, one diagonal of the tile a lane.  Workgroups write their sums by offset, a last launch adds them in a
 // fixed order: no atomics, the same bits every time.  A few rows in a long window split the walked axis (rel_splits).
 //
-// At [32, 1024, 1024], 8 heads of 128 (69 GFLOP a product; a large matrix product of this card runs at 1247 TFLOP/s):
-// forward 0.18 ms for inference and 0.235 in front of a backward pass, dQ 0.29, dK and dV 0.34, table 0.015: 0.7 to
-// 0.88 PFLOP/s in each walk.  Two waves a SIMD share the matrix pipe (busy 35 to 38 % of the cycles) and the vector pipe (42 %,
-// exponentials and conversions first); neither is full, what is left is one wave waiting for its own scores between the products.
+// At [32, 1024, 1024], 8 heads of 128 (69 GFLOP a product; a large matrix product of this card runs at 1247 TFLOP/s), medians
+// under the profiler: forward 0.243 ms in front of a backward pass (0.17 for inference), dQ 0.311, dK and dV 0.369, table 0.014: 0.66 to
+// 0.85 PFLOP/s in each walk.  Two waves a SIMD share the matrix pipe (busy 47, 35 and 38 % of the cycles) and the vector pipe (issuing in
+// 52, 40 and 33 %); neither is full, what is left is one wave waiting for its own scores between the products.
 #include "attn_tiles.h"
 #include "relattn.h"
 
@@ -624,7 +624,8 @@ __global__ __launch_bounds__(AT_THREADS, HDP <= REL_OCC2 ? 2 : 1) void rel_attn_
 // backward 2/3: dK = scale dS^T Q, dV = P^T dO.  A workgroup owns 128 keys, 32 a wave, and walks the query rows 32 at a time (Q and
 // dO tiles, double-buffered).  X = Q K^T has the key on the lane and the rows in the registers, so P and dS are the next products'
 // B operands as they stand: dV^T += dO^T P, dK^T += Q^T dS (transposed reads of the tiles).  The accumulators take 128 registers
-// at head size 128; the keys' K rows are read from LDS, their V rows stay in registers, and two workgroups fit a CU.
+// at head size 128; the keys' K rows are read from LDS, their V rows stay in registers, and two workgroups fit a CU.  At that size the
+// kernel fills its 256 registers and keeps 4 more in scratch (20 with P and dS in 16 bits).
 // ---------------------------------------------------------------------------------------------
 constexpr int KV_KEYS = 128;
 constexpr int KV_STATS = 4 * BW_ROWS;               // of a tile's rows: maximum, log2 of the sum, delta, and the first two added up
@@ -914,7 +915,7 @@ template <int HDP, bool FINE> int launch_dkv(const RelK& p, hipStream_t st) {
 // error is that of one more rounding of the result: 1.41 times the error of the final rounding alone, averaged over many rows.
 //  - Forward in front of a backward pass: delta = <dO, O> must match the fp32 P that backward recomputes, or dP - delta loses its
 //    leading digits where one key dominates (dQ, dK and the table's gradient had up to 7 times the error of a 32-bit form).
-//    [32, 1024, 1024]: forward 176 -> 235 us, of a training pass of 0.86 ms; at [32, 1024], 8 heads of 32, 66 -> 92.
+//    [32, 1024, 1024]: forward 171 -> 233 us, of a training pass of 0.85 ms; at [32, 1024], 8 heads of 32, 64 -> 90.
 //  - Windows of one row tile, whose few rows average nothing: [32, 128], 8 heads of 128, forward 12.1 -> 12.6 us, backward 76 us
 //    either way.
 //  - dQ of heads up to 32, where the sum of dS K cancels most (1.6 times at heads of 8): backward of [32, 1024], 8 heads of 32,

@@ -17,14 +17,15 @@
 //
 // HBM-bound.  Inputs and outputs are touched once and are larger than the caches where it matters: their accesses are
 // non-temporal (forward at [64, 1024, 1024] bf16 83 -> 71 us, and a kernel that reads h afterwards does not lose it).  Measured
-// there: forward 71 us (403 MB, 5.7 TB/s), backward 123 us (671 MB, 5.5 TB/s); [1, 75000, 1024] forward 134 us, of which the
-// segment launch takes 55 (461 + 307 MB).
+// there, medians under the profiler: forward 74 us (403 MB, 5.4 TB/s), backward 132 us (671 MB, 5.1 TB/s); [1, 75000, 1024] forward 65 us
+// for the segments and 83 for the walk (307 and 461 MB; 137 us for both in a row of calls).
 //
 // Everything between loads and stores is fp32.  sigmoid: with t = exp(-|g|), small = t / (1 + t), big = 1 - small; keep = 1 - f
 // has full relative precision on both sides.  A long memory lives in 1 - f, which fp32 rounds to multiples of 2^-24 next to 1: 1 - f
 // would be 0.07 % off at g = 10 and nothing at g = 17.4, so that a state would settle beside its input or never forget.  So the
 // complement C = 1 - A of a span is summed beside A, C + A keep a row; where it is below a half, A is 1 - C and the rest that this
 // rounding left, and h = A h + (rest h + B) rounds once.  Within eight rows, whose errors end with their span, f is used as it is.
+// (A rest in every row took 86 and 146 us forward and backward, one across spans 72..75 and 129, none 72 and 126.)
 #include "common.h"
 #include <cfloat>
 
