@@ -576,3 +576,26 @@ def test_a_clipped_step_has_the_bits_of_32_bit_torch(max_norm, wd):
                 assert torch.equal(got.view(torch.uint8), x.view(torch.uint8)), (t, k, int((got.float() != x.float()).sum()))
             off, size = (p.detach().double() - p1.double()).abs(), torch.maximum(p0.double().abs(), p1.double().abs())
             assert float((off - 5 * U * size - 12 * U * step.double().abs()).max()) <= 0
+
+
+@pytest.mark.gpu
+def test_a_state_loaded_before_its_parameters_moved():
+    """A checkpoint loaded beside parameters on the CPU that then move to the device: the codes follow at the next look or step."""
+    from unet_amd.optim import ClipAdamW, quantise_moment
+    gen = torch.Generator().manual_seed(6)
+    net = torch.nn.Linear(90, 77)
+    opt = ClipAdamW(net.parameters(), state_bits=8)
+    saved = opt.state_dict()
+    codes = quantise_moment(torch.randn(77, 90, generator=gen), False) + quantise_moment(torch.rand(77, 90, generator=gen), True)
+    names = ("exp_avg", "exp_avg_scale", "exp_avg_sq_root", "exp_avg_sq_root_scale")
+    saved["state"] = {0: dict(zip(names, codes), step=torch.tensor(2.0))}
+    opt.load_state_dict(saved)
+    net.cuda()
+    opt.moment_buffers()
+    for k, t in zip(names, codes):
+        got = opt.state[net.weight][k]
+        assert got.is_cuda and torch.equal(got.cpu().view(torch.uint8), t.view(torch.uint8)), k
+    for p in net.parameters():
+        p.grad = torch.zeros_like(p)
+    opt.step()
+    assert float(opt.state[net.weight]["step"]) == 3

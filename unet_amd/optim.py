@@ -204,9 +204,9 @@ class _Group8:
                     parts.append(st[name].reshape(-1).to(torch.float8_e4m3fn).view(torch.uint8))
                     if v[name].numel() % BLOCK:
                         parts.append(parts[-1].new_zeros(-v[name].numel() % BLOCK))
-                torch.cat(parts, out=buf[:self.end8].view(torch.uint8))
+                buf[:self.end8].view(torch.uint8).copy_(torch.cat(parts))        # (from wherever the states were loaded)
             for name, buf in zip(("exp_avg_scale", "exp_avg_sq_root_scale"), (self.m_scale, self.r_scale)):
-                torch.cat([st[name].reshape(-1) for st, _ in coded], out=buf[:self.end8 // BLOCK])
+                buf[:self.end8 // BLOCK].copy_(torch.cat([st[name].reshape(-1) for st, _ in coded]))
         else:                                   # some of them have not been stepped yet, or come from fp32
             for st, v in coded:
                 if "exp_avg_scale" in st:
